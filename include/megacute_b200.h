@@ -219,6 +219,60 @@ int mk_noalloc_status(int device, void* stream, int32_t status[MK_ST_WORDS]);
  * static device array); two calls whose kernels may overlap on the GPU share it: serialise them. */
 int mk_argmax(const void* logits, int dtype, int rows, int cols, long long ld, long long* out, void* stream);
 
+/* ---- operators over a paged key/value cache ---------------------------------------------------------------------------------
+ * (No counterpart in the reference, whose decode ops keep one contiguous cache and add one token per sequence.)
+ *
+ * The tokens of a call are rows of a packed batch: sequence s has rows starts[s] .. starts[s + 1] - 1 (never decreasing), or, with
+ * starts NULL, rows / seqs rows each.  Its first row is at position pos[s * pos_ld], the next one behind it.  Rows in front of the first
+ * sequence and behind the last one are neither read nor written.  All arrays are device memory, read when the kernel runs, so a captured call
+ * replays with the values of that time.  Every entry runs on `device`, whichever device is current, and is asynchronous
+ * on `stream`; it allocates nothing and keeps nothing, so calls on different streams do not disturb one another.  dtype: 0 bf16, 1 fp32, 2 fp16. */
+typedef struct mk_batch {
+    const int32_t* pos;
+    const int32_t* starts;       /* seqs + 1 entries, or NULL */
+    int64_t pos_ld;              /* elements between two sequences' positions; 0: one position for all */
+    int32_t rows, seqs;
+} mk_batch;
+
+/* cos / sin of a rotation: row p is position p, column i the angle of pair i; columns = half of the rotated part of a head.
+ * interleaved 0: pair i is elements (i, i + columns) of a head, else (2 i, 2 i + 1).  columns % 8 == 0, ld % 8 == 0 and 16-byte aligned bases. */
+typedef struct mk_rotation {
+    const void* cos;
+    const void* sin;
+    int64_t ld_cos, ld_sin;
+    int32_t rows, columns, dtype, interleaved;
+} mk_rotation;
+
+/* Cache of `pages` pages of `page_size` rows (a power of two from 16 up), the kv heads of a token side by side in a row.
+ * Row p of sequence s is row p % page_size of page table[s * table_ld + p / page_size].  An entry outside [0, pages) is an absent page: nothing
+ * is read from it or written to it. */
+typedef struct mk_paged_cache {
+    void* k;
+    void* v;
+    const int32_t* table;
+    int64_t ld_k, ld_v, table_ld;
+    int32_t pages, page_size, table_cols, kv_heads, head_dim, dtype;
+} mk_paged_cache;
+
+/* out = x with each of `heads` heads (side by side in a row) rotated by its row's position; what is behind the first 2 * columns
+ * elements of a head is copied.  A row whose position is outside the tables becomes zeros.  out may be x (same address and ld). */
+int mk_rotary(int device, const mk_batch* batch, const mk_rotation* rot, const void* x, int64_t ld_x, void* out, int64_t ld_out, int dtype,
+              int heads, int head_dim, void* stream);
+
+/* Rotates the q and k heads of each row of qkv (heads + 2 kv_heads heads side by side), writes q to q_out and k and v to the row of
+ * the cache that the row's position has.  A row whose position is outside the tables or the page table is not appended, and its
+ * q becomes zeros; one whose page is absent is not appended.  No two rows of a call may have one cache row. */
+int mk_paged_append(int device, const mk_batch* batch, const mk_rotation* rot, const mk_paged_cache* cache, const void* qkv, int64_t ld_qkv,
+                    void* q_out, int64_t ld_q, int heads, void* stream);
+
+/* out[r, h] = softmax(scale * q[r, h] K^T) V over the cache rows [max(0, p + 1 - window), p] of the row's sequence (p: the row's
+ * position; window 0: from row 0), those of absent pages left out; a row that sees none becomes zeros.  max_new: the largest number of
+ * rows of a sequence, which the choice of kernel goes by; results are right whatever it is.  `workspace`: device memory of at least
+ * mk_paged_attention_workspace() bytes, 16-byte aligned, used by this call alone until it has run. */
+long long mk_paged_attention_workspace(int device, int heads, const mk_paged_cache* cache, int max_new);
+int mk_paged_attention(int device, const mk_batch* batch, const mk_paged_cache* cache, const void* q, int64_t ld_q, void* out, int64_t ld_out,
+                       int heads, float scale, int window, int max_new, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -41,11 +41,32 @@ class Caps(ctypes.Structure):
                                               "kernel_threads", "kernel_regs", "reserved")]
 
 
+class Batch(ctypes.Structure):
+    """mk_batch"""
+    _fields_ = [("pos", ctypes.c_void_p), ("starts", ctypes.c_void_p), ("pos_ld", ctypes.c_int64), ("rows", ctypes.c_int32),
+                ("seqs", ctypes.c_int32)]
+
+
+class Rotation(ctypes.Structure):
+    """mk_rotation"""
+    _fields_ = [("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p), ("ld_cos", ctypes.c_int64), ("ld_sin", ctypes.c_int64),
+                ("rows", ctypes.c_int32), ("columns", ctypes.c_int32), ("dtype", ctypes.c_int32), ("interleaved", ctypes.c_int32)]
+
+
+class PagedCache(ctypes.Structure):
+    """mk_paged_cache"""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("table", ctypes.c_void_p), ("ld_k", ctypes.c_int64),
+                ("ld_v", ctypes.c_int64), ("table_ld", ctypes.c_int64), ("pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("table_cols", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
 assert ctypes.sizeof(OpDesc) == 256
+assert (ctypes.sizeof(Batch), ctypes.sizeof(Rotation), ctypes.sizeof(PagedCache)) == (32, 48, 72)
 
 # name -> (restype, argtypes); every symbol include/megacute_b200.h declares
 _P = ctypes.c_void_p
 _I32P = ctypes.POINTER(ctypes.c_int32)
+_BATCH, _ROTATION, _CACHE = ctypes.POINTER(Batch), ctypes.POINTER(Rotation), ctypes.POINTER(PagedCache)
 SYMBOLS = {
     "mk_strerror": (ctypes.c_char_p, [ctypes.c_int]),
     "mk_last_cuda_error": (ctypes.c_char_p, []),
@@ -71,6 +92,12 @@ SYMBOLS = {
     "mk_launch_noalloc": (ctypes.c_int, [ctypes.c_int, _P, ctypes.c_int, _P, ctypes.c_int, _P, ctypes.c_int, _P, ctypes.c_int,
                                          ctypes.c_int, ctypes.c_int, _P, _I32P]),
     "mk_noalloc_status": (ctypes.c_int, [ctypes.c_int, _P, _I32P]),
+    "mk_rotary": (ctypes.c_int, [ctypes.c_int, _BATCH, _ROTATION, _P, ctypes.c_int64, _P, ctypes.c_int64, ctypes.c_int, ctypes.c_int,
+                                 ctypes.c_int, _P]),
+    "mk_paged_append": (ctypes.c_int, [ctypes.c_int, _BATCH, _ROTATION, _CACHE, _P, ctypes.c_int64, _P, ctypes.c_int64, ctypes.c_int, _P]),
+    "mk_paged_attention_workspace": (ctypes.c_longlong, [ctypes.c_int, ctypes.c_int, _CACHE, ctypes.c_int]),
+    "mk_paged_attention": (ctypes.c_int, [ctypes.c_int, _BATCH, _CACHE, _P, ctypes.c_int64, _P, ctypes.c_int64, ctypes.c_int, ctypes.c_float,
+                                          ctypes.c_int, ctypes.c_int, _P, ctypes.c_size_t, _P]),
     "mk_argmax": (ctypes.c_int, [_P, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_longlong, _P, _P]),
 }
 

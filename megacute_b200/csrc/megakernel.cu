@@ -1063,3 +1063,11 @@ extern "C" int mk_noalloc_status(int device, void* stream, int32_t status[MK_ST_
     MK_CUDA(cudaStreamSynchronize(st));
     return status[MK_ST_CODE] != 0 ? MK_E_DEVICE : MK_OK;
 }
+
+// For the entry points in other files: what mk_last_cuda_error returns next on this thread.
+namespace mk {
+int report(int code, const char* text) {
+    snprintf(g_cuda_err, sizeof g_cuda_err, "%s", text);
+    return code;
+}
+}  // namespace mk
