@@ -1,0 +1,183 @@
+// How attention over a paged cache is divided among workers, and what its kernels share.
+//
+// An item is up to `tokens` consecutive new tokens of one sequence and `group` query heads of one kv head: rows token * group + head of one
+// operand tile.  (Where more heads share a kv head than the tile has rows, `shared` such blocks of heads read it.)  Its keys are cut into units of 2^shift keys, aligned in the sequence.  All units of all items -- in the order
+// sequence, block of heads, tokens -- make one list, which is dealt out evenly: worker w has units [w N / W, (w + 1) N / W).  Lengths are known on
+// the device only, so every block works out its part itself, and batches of the most unlike lengths load all SMs alike.
+// A worker that has an item's units from the first to the last writes results.  Else it leaves the running maximum, the sum and the products of its
+// part in the workspace (slot 0 of the worker: a part that does not begin the item; slot 1: one that begins it), and a second kernel
+// (paged_attention.cu) joins them, always in the same order.
+#pragma once
+#include "paged.cuh"
+
+namespace mk {
+
+struct AttnArgs {
+    Batch batch;
+    Pages pages;
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    uint16_t* out;
+    long long ld_q, ld_k, ld_v, ld_out;
+    int blocks, shared, group, window;                // blocks of `group` heads; blocks that share a kv head
+    float scale2;                                     // scale * log2(e)
+    int tokens;                                       // new tokens of an item
+    int workers, part_rows;                           // ... and rows of a part in the workspace
+    int4* joins;                                      // of each worker: parts of the item that it begins and does not end (0: none), its first
+                                                      // row, its rows, its block of heads
+    float* stats;                                     // [worker][2][part_rows][2]: maximum (log2 domain) and sum
+    float* parts;                                     // [worker][2][part_rows][head_dim]
+};
+
+struct Item {
+    int lo, hi;                                       // keys some token sees (lo > hi: none)
+    int first, units;                                 // units; at least one
+};
+
+template <int SHIFT>
+__device__ __forceinline__ Item item_at(const AttnArgs& a, long long p0, int tokens) {
+    const long long cap = a.pages.capacity();
+    Item it;
+    it.hi = (int)min(max(p0 + tokens - 1, -1ll), cap - 1);
+    it.lo = a.window > 0 ? (int)min(max(p0 + 1 - a.window, 0ll), cap) : 0;
+    it.first = it.hi < it.lo ? 0 : it.lo >> SHIFT;
+    it.units = it.hi < it.lo ? 1 : (it.hi >> SHIFT) - it.first + 1;
+    return it;
+}
+
+// units of one block of heads of sequence s
+template <int SHIFT>
+__device__ __forceinline__ long long sequence_units(const AttnArgs& a, int s) {
+    const int r0 = a.batch.first(s), n = a.batch.count(s, r0);
+    if (n == 0) return 0;
+    const long long p = a.batch.position(s);
+    long long sum = 0;
+    for (int t = 0; t < n; t += a.tokens) sum += item_at<SHIFT>(a, p + t, min(a.tokens, n - t)).units;
+    return sum;
+}
+
+// Where a worker starts in the list.  Walks on from item to item.
+template <int SHIFT>
+struct Walk {
+    int s, kv, t;                                     // sequence, block of heads, first token of the item in the sequence
+    int r0, n;                                        // rows of the sequence
+    long long p;                                      // its position
+    int unit;                                         // next unit of the item
+    long long left;                                   // units that the worker still has, this item's among them
+    Item item;
+
+    __device__ __forceinline__ int item_tokens(const AttnArgs& a) const { return min(a.tokens, n - t); }
+    __device__ __forceinline__ void enter(const AttnArgs& a) { item = item_at<SHIFT>(a, p + t, item_tokens(a)); }
+    __device__ __forceinline__ void sequence(const AttnArgs& a, int seq) {
+        s = seq;
+        r0 = a.batch.first(s);
+        n = a.batch.count(s, r0);
+        p = a.batch.position(s);
+    }
+    // to unit `at` of the sequence's list (of `per` units a block of heads)
+    __device__ __forceinline__ void start(const AttnArgs& a, int seq, long long at, long long per) {
+        sequence(a, seq);
+        kv = (int)(at / per);
+        at -= kv * per;
+        t = 0;
+        enter(a);
+        while (at >= item.units && t + a.tokens < n) {
+            at -= item.units;
+            t += a.tokens;
+            enter(a);
+        }
+        unit = (int)at;
+    }
+    // behind the units [unit, unit + count) of this item
+    __device__ __forceinline__ void next(const AttnArgs& a, int count) {
+        unit += count;
+        left -= count;
+        if (unit < item.units || left <= 0) return;
+        unit = 0;
+        t += a.tokens;
+        if (t >= n) {
+            t = 0;
+            if (++kv == a.blocks) {
+                kv = 0;
+                do sequence(a, s + 1);
+                while (n == 0 && s + 1 < a.batch.seqs);
+            }
+        }
+        enter(a);
+    }
+};
+
+// The worker that has the unit in front of `end`.
+__device__ __forceinline__ int worker_before(long long end, long long total, int workers) {
+    return (int)((end * workers + total - 1) / total) - 1;
+}
+
+template <int THREADS>
+struct PlanScratch {
+    long long sums[THREADS / 32];
+    long long ends[THREADS];                          // inclusive sums of a round's sequences
+};
+
+// Every thread of the block calls it with its warp's worker.  Returns the number of workers among which the units are dealt out, at least `least`
+// to each, and their total; `walk` is set where the warp's worker has some (walk.left > 0).
+template <int SHIFT, int THREADS>
+__device__ __forceinline__ int plan(const AttnArgs& a, PlanScratch<THREADS>* sc, int worker, int least, Walk<SHIFT>& walk, long long& total) {
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int rounds = (a.batch.seqs + THREADS - 1) / THREADS;
+    long long mine = 0, sum = 0;
+    for (int r = 0; r < rounds; ++r) {
+        const int s = r * THREADS + t;
+        mine = s < a.batch.seqs ? sequence_units<SHIFT>(a, s) * a.blocks : 0;
+        sum += mine;
+    }
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == 0) sc->sums[warp] = sum;
+    __syncthreads();
+    total = 0;
+    for (int w = 0; w < THREADS / 32; ++w) total += sc->sums[w];
+    const int workers = (int)min((long long)a.workers, (total + least - 1) / least);
+    const long long begin = worker < workers ? worker * total / workers : total;
+    walk.left = worker < workers ? (worker + 1) * total / workers - begin : 0;
+    long long base = 0;
+    for (int r = 0; r < rounds; ++r) {
+        if (rounds > 1) {
+            const int s = r * THREADS + t;
+            mine = s < a.batch.seqs ? sequence_units<SHIFT>(a, s) * a.blocks : 0;
+        }
+        long long run = mine;
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long up = __shfl_up_sync(0xffffffffu, run, d);
+            if (lane >= d) run += up;
+        }
+        __syncthreads();                              // (the previous round's sums have been read)
+        if (lane == 31) sc->sums[warp] = run;
+        __syncthreads();
+        long long before = base, all = 0;
+        for (int w = 0; w < THREADS / 32; ++w) {
+            if (w < warp) before += sc->sums[w];
+            all += sc->sums[w];
+        }
+        sc->ends[t] = before + run;
+        __syncthreads();
+        if (walk.left > 0 && begin >= base && begin < base + all) {
+            int at = 0;                               // sequences of the round that end at or in front of `begin`
+            for (int i = lane; i < THREADS; i += 32) at += sc->ends[i] <= begin;
+            for (int d = 16; d; d >>= 1) at += __shfl_xor_sync(0xffffffffu, at, d);
+            const long long first = at > 0 ? sc->ends[at - 1] : base;
+            walk.start(a, r * THREADS + at, begin - first, (sc->ends[at] - first) / a.blocks);
+        }
+        base += all;
+    }
+    return workers;
+}
+
+// items of few rows (paged_attention_few.cu): rows of an item, workers of a block
+constexpr int kFewRows = 16;
+constexpr int kFewWarps = 8;
+cudaError_t launch_few(const AttnArgs& a, int head_dim, int dtype, int blocks, cudaStream_t stream);
+
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_kernel_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+}  // namespace mk

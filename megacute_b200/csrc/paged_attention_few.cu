@@ -1,0 +1,310 @@
+// Attention over a paged cache for items of at most 16 rows (new tokens x heads of a group): single tokens, a few speculative ones.
+//
+// Bound by memory: K and V are read once (heads of a group and tokens of a sequence share them), 2 * 2 * head_dim bytes a key, for 4 * 16 * head_dim
+// products, far below what warp-level matrix instructions give.  So every warp is a worker of its own (paged_attention.cuh): it
+// copies units of 8 KB (16 keys of head_dim 128, 32 of 64) into its own ring of three with 16-byte asynchronous copies, which follow the
+// page table row by row and write zeros for keys that are not there, and meets no other warp.  16 rows x unit:
+//   S = Q K^T   mma m16n8k16, K rows through ldmatrix (16-byte pieces swizzled by row: no bank conflicts), fp32
+//   P = 2^(S scale log2(e) - m), rounded to the operand type, in registers the A operand of
+//   O += P V    V through transposing ldmatrix
+// The maximum is only raised when it grows by more than 2^8, so that O is seldom scaled.
+#include "mma.cuh"
+#include "paged_attention.cuh"
+
+namespace mk {
+namespace {
+
+constexpr int kStagesFew = 3;
+constexpr int kUnitBytes = 8192;                      // K and V of a unit
+constexpr float kRaise = 8.0f;
+constexpr int kLeastUnits = 2;                        // units that a worker has at least, where there are few
+
+template <int D> constexpr int unit_shift = D == 128 ? 4 : 5;
+
+__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
+template <int DT>
+__device__ __forceinline__ void mma16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    if (DT == DT_F16) mma_f16(c, a, b0, b1);
+    else mma_bf16(c, a, b0, b1);
+}
+// infinity or NaN in one of two 16-bit values
+template <int DT>
+__device__ __forceinline__ bool not_finite(uint32_t w) {
+    constexpr uint32_t E = DT == DT_F16 ? 0x7c00u : 0x7f80u;
+    return (w & E) == E || ((w >> 16) & E) == E;
+}
+
+template <int DT, int D>
+__global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_constant__ AttnArgs a) {
+    constexpr int SHIFT = unit_shift<D>, U = 1 << SHIFT, NT = U / 8, KS = U / 16, DK = D / 16, DN = D / 8;
+    constexpr int CH = D / 8, ROWS_PER_COPY = 32 / CH;          // 16-byte pieces of a row; rows that 32 lanes copy
+    constexpr float NEG_INF = -__builtin_huge_valf();
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ PlanScratch<kFewWarps * 32> scratch;
+    wait_for_previous_kernel();
+    let_next_kernel_launch();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, worker = blockIdx.x * kFewWarps + warp;
+    Walk<SHIFT> w;
+    long long total;
+    const int workers = plan<SHIFT, kFewWarps * 32>(a, &scratch, worker, kLeastUnits, w, total);
+    if (lane == 0) a.joins[worker] = make_int4(0, 0, 0, 0);
+    const uint32_t ring = smem_u32(smem) + warp * (kStagesFew * kUnitBytes);
+    const int quad = lane >> 2, pair = (lane & 3) * 2;           // this thread's rows quad, quad + 8; columns pair, pair + 1 of each 8
+    const long long end = (long long)(worker + 1) * total / max(workers, 1);
+
+    while (w.left > 0) {
+        const int tokens = w.item_tokens(a), rows = tokens * a.group, u0 = w.unit;
+        const int count = (int)min((long long)(w.item.units - u0), w.left), base_row = w.r0 + w.t, kv = w.kv, s = w.s;
+        const Item it = w.item;
+        const long long p0 = w.p + w.t;
+        const int first_key = (it.first + u0) << SHIFT;
+        // ---- Q fragments
+        uint32_t q[DK][4];
+        long long row_at[2];                                     // element offset of this thread's two rows, -1: none
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = quad + 8 * i, tok = row / a.group;
+            row_at[i] = row < rows ? (long long)(base_row + tok) : -1;
+            const uint16_t* src = a.q + row_at[i] * a.ld_q + (kv * a.group + row - tok * a.group) * D + pair;
+#pragma unroll
+            for (int k = 0; k < DK; ++k) {
+                q[k][i] = row < rows ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16)) : 0u;
+                q[k][i + 2] = row < rows ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16 + 8)) : 0u;
+            }
+        }
+        // keys that this thread's rows see
+        int lo_r[2], hi_r[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const long long p = p0 + (quad + 8 * i) / a.group;
+            hi_r[i] = (int)min(max(p, -1ll), (long long)it.hi);
+            lo_r[i] = a.window > 0 ? (int)min(max(p + 1 - a.window, 0ll), 0x7fffffffll) : 0;
+        }
+        const int hi_all = (int)min(max(p0, -1ll), (long long)it.hi);                              // keys that every row sees
+        const int lo_all = a.window > 0 ? (int)min(max(p0 + tokens - a.window, 0ll), 0x7fffffffll) : 0;
+
+        // ---- the page table, 32 blocks of 16 keys at a time, a block per lane
+        int block0 = first_key >> 4, held = -1;
+        auto hold = [&](int at) {
+            block0 = at;
+            const int key = (at + lane) << 4;
+            held = -1;
+            if ((at + lane) >= 0 && key <= it.hi) {
+                const int f = a.pages.page_row(s, key >> a.pages.shift);
+                if (f >= 0) held = f + (key & ((1 << a.pages.shift) - 1));
+            }
+        };
+        hold(block0);
+        uint32_t absent = 0;                                     // two bits of unit u from bit 2 (u % 16): blocks that are not there
+        const uint16_t* kp = a.k + kv / a.shared * D + (lane % CH) * 8;
+        const uint16_t* vp = a.v + kv / a.shared * D + (lane % CH) * 8;
+        auto request = [&](int u) {                              // unit u of this part
+            if (u < count) {
+                const int key0 = first_key + (u << SHIFT);
+                if ((key0 >> 4) + U / 16 > block0 + 32) hold(key0 >> 4);
+                const uint32_t stage = ring + (u % kStagesFew) * kUnitBytes;
+                uint32_t gone = 0;
+#pragma unroll
+                for (int b = 0; b < U / 16; ++b) {
+                    const int f = __shfl_sync(0xffffffffu, held, (key0 >> 4) + b - block0);
+                    gone |= (f < 0 ? 1u : 0u) << b;
+#pragma unroll
+                    for (int i = 0; i < 16 / ROWS_PER_COPY; ++i) {
+                        const int row = i * ROWS_PER_COPY + lane / CH, key = key0 + b * 16 + row;
+                        const bool there = f >= 0 && key >= it.lo && key <= it.hi;
+                        const long long at = there ? f + row : 0;
+                        const uint32_t to = stage + (b * 16 + row) * (D * 2) + (((lane % CH) ^ (row & 7)) << 4);
+                        copy16_or_zero(to, kp + at * a.ld_k, there);
+                        copy16_or_zero(to + kUnitBytes / 2, vp + at * a.ld_v, there);
+                    }
+                }
+                absent = (absent & ~(3u << 2 * (u & 15))) | gone << 2 * (u & 15);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+
+        float o[DN][4];
+#pragma unroll
+        for (int i = 0; i < DN; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+        float m[2] = {NEG_INF, NEG_INF}, l[2] = {0.f, 0.f};
+        for (int u = 0; u < kStagesFew - 1; ++u) request(u);
+        for (int u = 0; u < count; ++u) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStagesFew - 2) : "memory");
+            __syncwarp();                                        // ... of every lane; and all have read the stage that is requested next
+            request(u + kStagesFew - 1);
+            const uint32_t ks = ring + (u % kStagesFew) * kUnitBytes, vs = ks + kUnitBytes / 2;
+            const int key0 = first_key + (u << SHIFT);
+            float sc[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+                const int row = n * 8 + (lane & 7);
+#pragma unroll
+                for (int k = 0; k < DK; k += 2) {
+                    uint32_t b[4];
+                    ldmatrix_x4(ks + row * (D * 2) + (((k * 2 + (lane >> 3)) ^ (row & 7)) << 4), b[0], b[1], b[2], b[3]);
+                    mma16<DT>(sc[n], q[k], b[0], b[1]);
+                    mma16<DT>(sc[n], q[k + 1], b[2], b[3]);
+                }
+            }
+            const bool partial = key0 < lo_all || key0 + U - 1 > hi_all;      // keys that some row does not see
+            const uint32_t gone = (absent >> 2 * (u & 15)) & 3u;
+            float mx[2] = {NEG_INF, NEG_INF};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[n][e] *= a.scale2;
+                if (partial || gone) {
+                    const bool here = !((gone >> (n / 2)) & 1u);
+                    const int key = key0 + n * 8 + pair;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int j = key + (e & 1);
+                        if (!here || j < lo_r[e >> 1] || j > hi_r[e >> 1]) sc[n][e] = NEG_INF;
+                    }
+                }
+                mx[0] = fmaxf(mx[0], fmaxf(sc[n][0], sc[n][1]));
+                mx[1] = fmaxf(mx[1], fmaxf(sc[n][2], sc[n][3]));
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+                mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+            }
+            const bool raise = mx[0] > m[0] + kRaise || (m[0] == NEG_INF && mx[0] > NEG_INF) || mx[1] > m[1] + kRaise ||
+                               (m[1] == NEG_INF && mx[1] > NEG_INF);
+            if (__any_sync(0xffffffffu, raise)) {
+                float f[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float to = fmaxf(m[i], mx[i]);
+                    f[i] = m[i] == NEG_INF ? 0.f : ex2(m[i] - to);
+                    m[i] = to;
+                    l[i] *= f[i];
+                }
+#pragma unroll
+                for (int i = 0; i < DN; ++i) {
+                    o[i][0] *= f[0]; o[i][1] *= f[0];
+                    o[i][2] *= f[1]; o[i][3] *= f[1];
+                }
+            }
+            const float off[2] = {m[0] == NEG_INF ? 0.f : m[0], m[1] == NEG_INF ? 0.f : m[1]};     // (no key so far: every score is -inf)
+            uint32_t p[KS][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[n][e] = ex2(sc[n][e] - off[e >> 1]);
+                l[0] += sc[n][0] + sc[n][1];
+                l[1] += sc[n][2] + sc[n][3];
+                p[n >> 1][(n & 1) * 2] = pack16<DT>(sc[n][0], sc[n][1]);
+                p[n >> 1][(n & 1) * 2 + 1] = pack16<DT>(sc[n][2], sc[n][3]);
+            }
+            // a value that is no number must not reach the tokens that do not see its key through 0 * it
+            bool odd = false;
+            if (partial && tokens > 1) {
+                for (int i = lane; i < U * CH; i += 32) {
+                    uint32_t x[4];
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(vs + i * 16) : "memory");
+                    odd |= not_finite<DT>(x[0]) || not_finite<DT>(x[1]) || not_finite<DT>(x[2]) || not_finite<DT>(x[3]);
+                }
+                odd = __any_sync(0xffffffffu, odd);
+            }
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+#pragma unroll
+                for (int n = 0; n < DN; n += 2) {
+                    const int row = k * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+                    uint32_t b[4];
+                    ldmatrix_x4_trans(vs + row * (D * 2) + (((n + (lane >> 4)) ^ (row & 7)) << 4), b[0], b[1], b[2], b[3]);
+                    if (!odd) {
+                        mma16<DT>(o[n], p[k], b[0], b[1]);
+                        mma16<DT>(o[n + 1], p[k], b[2], b[3]);
+                        continue;
+                    }
+                    for (int t = 0; t < tokens; ++t) {           // token by token, its rows and the values it sees
+                        const long long at = p0 + t;
+                        const int hi = (int)min(max(at, -1ll), (long long)it.hi);
+                        const int lo = a.window > 0 ? (int)min(max(at + 1 - a.window, 0ll), 0x7fffffffll) : 0;
+                        const bool r0 = quad / a.group == t, r1 = (quad + 8) / a.group == t;
+                        uint32_t bt[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = key0 + k * 16 + (e & 1) * 8 + pair;
+                            bt[e] = b[e] & ((key >= lo && key <= hi ? 0xffffu : 0u) | (key + 1 >= lo && key + 1 <= hi ? 0xffff0000u : 0u));
+                        }
+                        float c[2][4] = {};
+                        mma16<DT>(c[0], p[k], bt[0], bt[1]);
+                        mma16<DT>(c[1], p[k], bt[2], bt[3]);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (e & 2 ? r1 : r0) o[n + (e >> 2)][e & 3] += c[e >> 2][e & 3];
+                    }
+                }
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncwarp();                                            // the ring is free for the next part
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        }
+        // ---- results, or this part's statistics and products
+        const bool whole = u0 == 0 && count == it.units;
+        const int slot = worker * 2 + (u0 == 0 ? 1 : 0);
+        if (!whole && u0 == 0 && lane == 0) {
+            const long long item_end = end + (it.units - count);               // (the item is not finished: the worker's last)
+            a.joins[worker] = make_int4(worker_before(item_end, total, workers) - worker + 1, base_row, rows, kv);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = quad + 8 * i;
+            if (row >= rows) continue;
+            if (whole) {
+                const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+                uint16_t* to = a.out + row_at[i] * a.ld_out + (kv * a.group + row % a.group) * D + pair;
+#pragma unroll
+                for (int n = 0; n < DN; ++n) *reinterpret_cast<uint32_t*>(to + n * 8) = pack16<DT>(o[n][2 * i] * inv, o[n][2 * i + 1] * inv);
+            } else {
+                const long long at = (long long)slot * a.part_rows + row;
+                // (no score but NaN, which no maximum shows: a finite one, so that the part counts)
+                if ((lane & 3) == 0) reinterpret_cast<float2*>(a.stats)[at] = make_float2(l[i] != l[i] && m[i] == NEG_INF ? 0.f : m[i], l[i]);
+#pragma unroll
+                for (int n = 0; n < DN; ++n) *reinterpret_cast<float2*>(a.parts + at * D + n * 8 + pair) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+            }
+        }
+        w.next(a, count);
+    }
+}
+
+template <int DT, int D>
+cudaError_t launch(const AttnArgs& a, int blocks, cudaStream_t stream) {
+    constexpr int bytes = kFewWarps * kStagesFew * kUnitBytes;
+    const cudaError_t e = cudaFuncSetAttribute(attend_few<DT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute pdl;
+    pdl.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    pdl.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(kFewWarps * 32);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = stream;
+    cfg.attrs = &pdl;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attend_few<DT, D>, a);
+}
+
+}  // namespace
+
+cudaError_t launch_few(const AttnArgs& a, int head_dim, int dtype, int blocks, cudaStream_t stream) {
+    if (dtype == DT_F16) return head_dim == 64 ? launch<DT_F16, 64>(a, blocks, stream) : launch<DT_F16, 128>(a, blocks, stream);
+    return head_dim == 64 ? launch<DT_BF16, 64>(a, blocks, stream) : launch<DT_BF16, 128>(a, blocks, stream);
+}
+
+}  // namespace mk
