@@ -273,6 +273,10 @@ long long mk_paged_attention_workspace(int device, int heads, const mk_paged_cac
 int mk_paged_attention(int device, const mk_batch* batch, const mk_paged_cache* cache, const void* q, int64_t ld_q, void* out, int64_t ld_out,
                        int heads, float scale, int window, int max_new, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Waits for `stream`; MK_E_DEVICE if a kernel of mk_paged_attention on `device` gave up waiting inside since the last call (its results
+ * are not to be used; no wait of a kernel lasts longer than two seconds). */
+int mk_paged_attention_status(int device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

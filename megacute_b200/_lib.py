@@ -11,6 +11,7 @@ import os
 import pathlib
 import shutil
 import subprocess
+import tempfile
 
 PKG = pathlib.Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
@@ -25,6 +26,9 @@ LIB_PATH = pathlib.Path(os.environ.get("MEGACUTE_B200_LIB", PKG / ("libmegacute_
 # not see the kernel's __launch_bounds__.
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-rdc=true",
               "-maxrregcount=168", "-shared", "-Xcompiler", "-fPIC"]
+# Sources of kernels of their own, compiled as whole programs: ptxas ignores setmaxnreg in relocatable device code.
+WHOLE_PROGRAM = ("rotary.cu", "paged_attention.cu", "paged_attention_few.cu", "paged_attention_chunk.cu")
+WHOLE_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-c"]
 
 ST_WORDS = 16
 MAX_PTRS = 12
@@ -98,6 +102,7 @@ SYMBOLS = {
     "mk_paged_attention_workspace": (ctypes.c_longlong, [ctypes.c_int, ctypes.c_int, _CACHE, ctypes.c_int]),
     "mk_paged_attention": (ctypes.c_int, [ctypes.c_int, _BATCH, _CACHE, _P, ctypes.c_int64, _P, ctypes.c_int64, ctypes.c_int, ctypes.c_float,
                                           ctypes.c_int, ctypes.c_int, _P, ctypes.c_size_t, _P]),
+    "mk_paged_attention_status": (ctypes.c_int, [ctypes.c_int, _P]),
     "mk_argmax": (ctypes.c_int, [_P, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_longlong, _P, _P]),
 }
 
@@ -122,15 +127,22 @@ def build(force: bool = False, verbose: bool = False, check: bool | None = None)
     if not force and not needs_build_of(out):
         return out
     nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
-    cmd = [nvcc, *NVCC_FLAGS, *(["-DMK_CHECK"] if check else []), "-o", str(out), *[str(f) for f in sorted(CSRC.glob("*.cu"))]]
-    if verbose:
-        cmd.insert(1, "-Xptxas")
-        cmd.insert(2, "-v")
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"nvcc failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
-    if verbose:
-        print(r.stderr)
+    define, loud = ["-DMK_CHECK"] if check else [], ["-Xptxas", "-v"] if verbose else []
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = [pathlib.Path(tmp) / f"{name}.o" for name in WHOLE_PROGRAM]
+        cmds = [[nvcc, *loud, *WHOLE_FLAGS, *define, "-o", str(o), str(CSRC / name)] for o, name in zip(objects, WHOLE_PROGRAM)]
+        rest = [str(f) for f in sorted(CSRC.glob("*.cu")) if f.name not in WHOLE_PROGRAM]
+        link = [nvcc, *loud, *NVCC_FLAGS, *define, "-o", str(out), *rest, *[str(o) for o in objects]]
+        running = [subprocess.Popen(c, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True) for c in cmds]
+        done = [(c, *r.communicate(), r.returncode) for c, r in zip(cmds, running)]
+        if all(rc == 0 for *_, rc in done):
+            r = subprocess.run(link, capture_output=True, text=True)
+            done.append((link, r.stdout, r.stderr, r.returncode))
+    for cmd, stdout, stderr, rc in done:
+        if rc != 0:
+            raise RuntimeError(f"nvcc failed:\n{' '.join(cmd)}\n{stdout}\n{stderr}")
+        if verbose:
+            print(stderr)
     return out
 
 

@@ -113,15 +113,19 @@ int heads_of_block(int group, int rows) {
     return n;
 }
 
+// Which kernel takes a call: the one for few rows where an item of 16 rows holds all new tokens of a sequence (then every key is read once).
+bool few_rows(int group, long long max_new) { return max_new * group <= kFewRows; }
+
 // what the workspace holds, one behind the other: joins, stats, parts
 struct Layout {
-    int workers, part_rows;
+    int workers, part_rows, per_block;
     size_t stats, parts, bytes;
 };
-Layout layout_of(int sms, int head_dim) {
+Layout layout_of(int sms, int head_dim, bool few) {
     Layout l;
-    l.workers = sms * kFewWarps;
-    l.part_rows = kFewRows;
+    l.per_block = few ? kFewWarps : 1;
+    l.workers = sms * l.per_block;
+    l.part_rows = few ? kFewRows : 2 * kChunkTile;
     l.stats = (size_t)l.workers * sizeof(int4);
     l.parts = l.stats + (size_t)l.workers * 2 * l.part_rows * 2 * sizeof(float);
     l.bytes = l.parts + (size_t)l.workers * 2 * l.part_rows * head_dim * sizeof(float);
@@ -152,7 +156,9 @@ extern "C" long long mk_paged_attention_workspace(int device, int heads, const m
     if (why) return report(MK_E_ARG, why);
     const int sms = sm_count(device);
     if (!sms) return report(MK_E_CUDA, "no such device");
-    return (long long)layout_of(sms, cache->head_dim).bytes;
+    const size_t few = layout_of(sms, cache->head_dim, true).bytes, chunk = layout_of(sms, cache->head_dim, false).bytes;
+    // (a scale that is not positive is for the kernel for few rows, whatever max_new)
+    return (long long)(few_rows(heads / cache->kv_heads, max_new) || few > chunk ? few : chunk);
 }
 
 extern "C" int mk_paged_attention(int device, const mk_batch* batch, const mk_paged_cache* cache, const void* q, int64_t ld_q, void* out,
@@ -170,7 +176,8 @@ extern "C" int mk_paged_attention(int device, const mk_batch* batch, const mk_pa
     if (!workspace || ((uintptr_t)workspace & 15)) return report(MK_E_ARG, "paged attention: workspace of 16-byte aligned device memory");
     const int sms = sm_count(device);
     if (!sms) return report(MK_E_CUDA, "no such device");
-    const Layout lay = layout_of(sms, D);
+    const bool few = few_rows(group, max_new) || !(scale > 0.f) || scale > 1e30f;
+    const Layout lay = layout_of(sms, D, few);
     if (workspace_bytes < lay.bytes) return report(MK_E_ARG, "paged attention: workspace smaller than mk_paged_attention_workspace()");
     OnDevice on(device);
     if (!on.ok) return report(MK_E_CUDA, "cudaSetDevice");
@@ -185,7 +192,7 @@ extern "C" int mk_paged_attention(int device, const mk_batch* batch, const mk_pa
     a.ld_k = cache->ld_k;
     a.ld_v = cache->ld_v;
     a.ld_out = ld_out;
-    a.group = heads_of_block(group, kFewRows);
+    a.group = heads_of_block(group, few ? kFewRows : kChunkTile);
     a.shared = group / a.group;
     a.blocks = heads / a.group;
     a.window = window;
@@ -196,13 +203,25 @@ extern "C" int mk_paged_attention(int device, const mk_batch* batch, const mk_pa
     a.stats = (float*)((uint8_t*)workspace + lay.stats);
     a.parts = (float*)((uint8_t*)workspace + lay.parts);
     cudaStream_t st = (cudaStream_t)stream;
-    a.tokens = kFewRows / a.group;
-    cudaError_t e = launch_few(a, D, cache->dtype, sms, st);
+    a.tokens = few ? kFewRows / a.group : kChunkTile / a.group * 2;
+    cudaError_t e = few ? launch_few(a, D, cache->dtype, sms, st) : launch_chunk(a, cache, heads, st);
     if (e == cudaSuccess) {
-        if (cache->dtype == DT_F16) e = D == 64 ? launch_join<DT_F16, 64>(a, kFewWarps, st) : launch_join<DT_F16, 128>(a, kFewWarps, st);
-        else e = D == 64 ? launch_join<DT_BF16, 64>(a, kFewWarps, st) : launch_join<DT_BF16, 128>(a, kFewWarps, st);
+        if (cache->dtype == DT_F16) e = D == 64 ? launch_join<DT_F16, 64>(a, lay.per_block, st) : launch_join<DT_F16, 128>(a, lay.per_block, st);
+        else e = D == 64 ? launch_join<DT_BF16, 64>(a, lay.per_block, st) : launch_join<DT_BF16, 128>(a, lay.per_block, st);
     }
     if (e == cudaSuccess) return MK_OK;
     (void)cudaGetLastError();
     return report(MK_E_CUDA, cudaGetErrorString(e));
+}
+
+extern "C" int mk_paged_attention_status(int device, void* stream) {
+    OnDevice on(device);
+    if (!on.ok) return report(MK_E_CUDA, "cudaSetDevice");
+    int failed = 0;
+    const cudaError_t e = chunk_status(&failed, (cudaStream_t)stream);
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        return report(MK_E_CUDA, cudaGetErrorString(e));
+    }
+    return failed ? MK_E_DEVICE : MK_OK;
 }

@@ -177,6 +177,11 @@ constexpr int kFewRows = 16;
 constexpr int kFewWarps = 8;
 cudaError_t launch_few(const AttnArgs& a, int head_dim, int dtype, int blocks, cudaStream_t stream);
 
+// items of up to 256 rows, a positive scale (paged_attention_chunk.cu): two tiles of 128 rows, a worker per block
+constexpr int kChunkTile = 128;
+cudaError_t launch_chunk(const AttnArgs& a, const mk_paged_cache* cache, int heads, cudaStream_t stream);
+cudaError_t chunk_status(int* failed, cudaStream_t stream);
+
 __device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_kernel_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -1,0 +1,648 @@
+// Attention over a paged cache for items of up to 256 rows (new tokens x heads of a group): chunks of prompts, whole prompts, batches that
+// mix them with single tokens.
+//
+// An item is two tiles of 128 query rows that share every tile of 128 keys (paged_attention.cuh: a unit).  One block per SM, one worker per block:
+//   warps 0-3, 4-7   softmax of tile 0 and 1, one thread per row (a lane of tensor memory): the row's 128 scores are held in registers, so
+//                    nothing is exchanged between threads; log2 domain, scale * log2(e) folded into the subtraction; the maximum is only
+//                    raised when it grows by more than 2^8, and then the row of O in tensor memory is scaled down; results
+//   warp 8           loader: Q as boxes of 64 columns x group heads x tokens, K and V as boxes of 64 columns x the rows of a page (at most 128), found
+//                    through the page table, into one ring of tiles in the order K, V, K, V, ...
+//   warp 9           products: S = Q K^T and O += P V on tcgen05, S, P (over S) and O in tensor memory
+//   warps 10, 11     look at every V tile before it is multiplied: rows that no token of the item sees become zeros (they may hold anything, and
+//                    0 * inf is no number); where some tokens see a row and others do not, values that are no numbers are taken out and added back
+//                    to the rows that see them when the item ends
+// A score product of 128 x 128 x 64 takes 256 cycles, its exponentials 1024 (16 a cycle), so for head_dim 64 the special function units
+// bound it, for 128 both do.
+// Every wait has a limit, after which the block raises a flag that all its waits ask for, waits for its copies, frees its tensor memory and ends;
+// mk_paged_attention_status tells.
+#include <cuda.h>          // CUtensorMap
+
+#include "paged_attention.cuh"
+#include "tc.cuh"
+
+namespace mk {
+
+__device__ int g_paged_failed;                        // a block gave up waiting (read and cleared by mk_paged_attention_status)
+
+namespace {
+
+constexpr int kChunkThreads = 384;
+constexpr float kLazy = 8.0f;
+constexpr unsigned long long kWaitNs = 2000000000ull;
+constexpr int kTileRows = 128;
+constexpr int kSubBytes = kTileRows * 128;            // 64 columns of a tile of 128 rows
+constexpr int kSeen = 32;                             // entries of the ring of tile descriptions, far more than tiles in flight
+constexpr int kRingBars = 8;                          // barriers of key tiles, more than tiles in the ring
+constexpr int kOddItems = 4, kOddTiles = 8;           // items, and tiles of an item, whose odd values are remembered
+
+template <int D> struct Map {
+    static constexpr int kSubs = D / 64;
+    static constexpr int kTile = kSubs * kSubBytes;
+    static constexpr int kSlots = D == 64 ? 10 : 5;   // tiles in the ring
+    static constexpr int kQ = 0, kRing = 2 * kTile, kBytes = kRing + kSlots * kTile;       // (Sync lies behind)
+    static constexpr int kScores = D == 64 ? 3 : 2;   // tensor-memory buffers of scores, 128 columns each from column 0
+    static constexpr uint32_t kO = kScores * 128;     // ... then O of tile 0 and of tile 1
+};
+
+struct Sync {
+    // (by parity a wait only tells a phase from the one in front of it: a barrier's phases are all waited for by the same threads, one after the
+    // other, or the one in front is known to be over)
+    unsigned long long q_full, q_free;                // one per item
+    unsigned long long k_full[kRingBars], v_full[kRingBars], v_ready[kRingBars];           // key tile c: c % kRingBars
+    unsigned long long slot_free[10];                 // slots of the ring of tiles
+    unsigned long long s_full[2][4], pv_done[2][4];   // tile t's k-th block of scores: k % 4
+    unsigned long long p_full[2], o_free[2], item_done[kOddItems];
+    uint32_t tmem;
+    int abort;
+    uint32_t there[kSeen];                            // bit b: keys [16 b, 16 b + 16) of the tile are loaded
+    uint32_t odd[kOddItems][kOddTiles][4];            // keys of the item's n-th partial tile with values that are no numbers
+    int odd_any[kOddItems][2];
+};
+
+__device__ __forceinline__ bool wait_bar(Sync* s, unsigned long long* bar, uint32_t parity) {
+    for (int i = 0; i < 64; ++i)
+        if (mbar_test_wait(bar, parity)) return true;
+    const unsigned long long t0 = globaltimer();
+    while (!mbar_try_wait(bar, parity)) {
+        if (*(volatile int*)&s->abort) return false;
+        if (globaltimer() - t0 > kWaitNs) {
+            *(volatile int*)&s->abort = 1;
+            atomicExch(&g_paged_failed, 1);
+            return false;
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ bool warp_wait(Sync* s, unsigned long long* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, wait_bar(s, bar, parity));
+}
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* m, int x, int y, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(m),
+                 "r"(x), "r"(y), "r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* m, int x, int y, int z, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(m),
+                 "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* w) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at),
+        "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "r"(w[8]), "r"(w[9]), "r"(w[10]),
+        "r"(w[11]), "r"(w[12]), "r"(w[13]), "r"(w[14]), "r"(w[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D (+)= A B with A in tensor memory
+__device__ __forceinline__ void mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b),
+                 "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ float2 fma_2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{ .reg .b64 x, y, z, w; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7}; fma.rn.f32x2 w, x, y, z; mov.b64 {%0, %1}, w; }"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add_2(float2 a, float2 b) {
+    float2 d;
+    asm("{ .reg .b64 x, y, w; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 w, x, y; mov.b64 {%0, %1}, w; }"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float max_3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+template <int DT>
+__device__ __forceinline__ bool odd_value(uint32_t h) {                        // a 16-bit value that is no number
+    constexpr uint32_t E = DT == DT_F16 ? 0x7c00u : 0x7f80u;
+    return (h & E) == E;
+}
+
+struct Maps {
+    CUtensorMap q, k, v;
+};
+
+// What one worker does to one item, as every role sees it.
+struct Part {
+    long long p0;                                     // position of the item's first token
+    int tokens, row0, block, s;                       // its tokens, first row of the packed batch, block of heads, sequence
+    int lo, hi, key0, units, tiles;                   // keys some token sees; first key of the part; key tiles; query tiles
+    bool begins, ends;
+};
+constexpr int kShift = 7;
+__device__ __forceinline__ Part part_of(const AttnArgs& a, const Walk<kShift>& w) {
+    Part p;
+    p.p0 = w.p + w.t;
+    p.tokens = w.item_tokens(a);
+    p.row0 = w.r0 + w.t;
+    p.block = w.kv;
+    p.s = w.s;
+    p.lo = w.item.lo;
+    p.hi = w.item.hi;
+    p.key0 = (w.item.first + w.unit) << kShift;
+    p.units = (int)min((long long)(w.item.units - w.unit), w.left);
+    p.tiles = p.tokens > a.tokens / 2 ? 2 : 1;
+    p.begins = w.unit == 0;
+    p.ends = w.unit + p.units == w.item.units;
+    return p;
+}
+// keys that every token of [t0, t1) sees
+__device__ __forceinline__ void seen_by_all(const AttnArgs& a, const Part& p, int t0, int t1, int& lo, int& hi) {
+    hi = (int)min(max(p.p0 + t0, -1ll), (long long)p.hi);
+    lo = a.window > 0 ? (int)min(max(p.p0 + t1 - a.window, 0ll), 0x7fffffffll) : 0;
+}
+__device__ __forceinline__ void seen_by(const AttnArgs& a, const Part& p, int token, int& lo, int& hi) { seen_by_all(a, p, token, token + 1, lo, hi); }
+
+// ---- loader -------------------------------------------------------------------------------------------------------------------
+template <int D>
+__device__ __forceinline__ void load_role(const AttnArgs& a, const Maps& m, uint8_t* smem, Sync* sy, Walk<kShift> w) {
+    using M = Map<D>;
+    const int lane = threadIdx.x & 31;
+    const int box = min(1 << a.pages.shift, kTileRows), boxes = kTileRows / box, tile_tokens = a.tokens / 2;
+    const uint32_t base = smem_u32(smem);
+    const uint32_t block_bits = (box == 128 ? 0xffu : (1u << (box >> 4)) - 1u);
+    uint32_t c = 0, items = 0;                        // tiles and parts so far
+    bool ok = true;
+    for (; w.left > 0 && ok; ++items) {
+        const Part p = part_of(a, w);
+        const int kv = p.block / a.shared;
+        ok = warp_wait(sy, &sy->q_free, (items & 1u) ^ 1u);
+        if (!ok) break;
+        if (lane == 0) {
+            const uint32_t bytes = (uint32_t)(a.group * tile_tokens) * 128u * M::kSubs;
+            mbar_arrive_expect_tx(&sy->q_full, bytes * p.tiles);
+            for (int t = 0; t < p.tiles; ++t)
+                for (int i = 0; i < M::kSubs; ++i)
+                    tma_3d(base + M::kQ + t * M::kTile + i * kSubBytes, &m.q, i * 64, p.block * a.group, p.row0 + t * tile_tokens, &sy->q_full);
+        }
+        auto find = [&](int u) {                      // cache row of this lane's box of key tile u, -1: none
+            const int key = p.key0 + (u << kShift) + lane * box;
+            int row = -1;
+            if (lane < boxes && u < p.units && key <= p.hi && key + box - 1 >= p.lo) {
+                row = a.pages.page_row(p.s, key >> a.pages.shift);
+                if (row >= 0) row += key & ((1 << a.pages.shift) - 1);
+            }
+            return row;
+        };
+        int row = find(0);
+        for (int u = 0; u < p.units && ok; ++u, ++c) {
+            const int next = find(u + 1);             // (under way while this tile waits for its slot)
+            const uint32_t got = __ballot_sync(0xffffffffu, row >= 0);
+            const uint32_t bytes = __popc(got) * (uint32_t)box * 128u * M::kSubs;
+            if (lane == 0) {
+                uint32_t bits = 0;
+                for (int b = 0; b < boxes; ++b)
+                    if ((got >> b) & 1u) bits |= block_bits << (b * (box >> 4));
+                sy->there[c % kSeen] = bits;
+            }
+#pragma unroll
+            for (int kvt = 0; kvt < 2 && ok; ++kvt) {
+                const uint32_t n = 2 * c + kvt, slot = n % M::kSlots;
+                unsigned long long* const full = kvt ? &sy->v_full[c % kRingBars] : &sy->k_full[c % kRingBars];
+                ok = warp_wait(sy, &sy->slot_free[slot], ((n / M::kSlots) & 1u) ^ 1u);
+                if (!ok) break;
+                if (lane == 0) mbar_arrive_expect_tx(full, bytes);
+                __syncwarp();
+                if (row >= 0) {
+#pragma unroll
+                    for (int i = 0; i < M::kSubs; ++i)
+                        tma_2d(base + M::kRing + slot * M::kTile + i * kSubBytes + lane * box * 128, kvt ? &m.v : &m.k, kv * D + i * 64, row, full);
+                }
+                __syncwarp();
+            }
+            row = next;
+        }
+        w.next(a, p.units);
+    }
+    if (!ok) {                                        // copies that are under way land before the block's memory goes
+        if (lane == 0) {
+            auto landed = [&](unsigned long long* bar, uint32_t parity) {
+                const unsigned long long t0 = globaltimer();
+                while (!mbar_try_wait(bar, parity) && globaltimer() - t0 < 10000000ull) {}
+            };
+            if (items > 0) landed(&sy->q_full, (items - 1) & 1u);
+            landed(&sy->q_full, items & 1u);
+            for (uint32_t n = c > 6 ? c - 6 : 0; n <= c; ++n) {
+                landed(&sy->k_full[n % kRingBars], (n / kRingBars) & 1u);
+                landed(&sy->v_full[n % kRingBars], (n / kRingBars) & 1u);
+            }
+        }
+        __syncwarp();
+    }
+}
+
+// ---- products -----------------------------------------------------------------------------------------------------------------
+template <int DT, int D>
+__device__ __forceinline__ void product_role(const AttnArgs& a, uint8_t* smem, Sync* sy, Walk<kShift> w, uint32_t tmem) {
+    using M = Map<D>;
+    const uint32_t fmt = DT == DT_F16 ? 0u : 1u;
+    // fp32 accumulator, M = 128; S: N = 128, both operands K-major; O: N = D, B MN-major
+    const uint32_t basic = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 4) << 24);
+    const uint32_t idesc_s = basic | ((128u >> 3) << 17), idesc_o = basic | (1u << 16) | (((uint32_t)D >> 3) << 17);
+    const uint64_t d0 = tc_smem_desc(smem_u32(smem));
+    // MN-major: 8-key groups 1024 bytes apart (the descriptor's stride), sub-tiles of 64 columns 16 KB apart (its leading offset)
+    const uint64_t v0 = D == 64 ? d0 : d0 - (1ull << 16) + ((uint64_t)(kSubBytes >> 4) << 16);
+    uint32_t c = 0, items = 0, scores_done = 0, blocks[2] = {0, 0}, outs[2] = {0, 0};
+    for (; w.left > 0; ++items) {
+        const Part p = part_of(a, w);
+        const int total = p.units * p.tiles;
+        int done[2] = {0, 0};                         // blocks of this item whose P V has been issued (`blocks`: of all)
+        auto scores = [&](int n) {
+            const int t = p.tiles == 2 ? n & 1 : 0, j = p.tiles == 2 ? n >> 1 : n;
+            const uint32_t kt = c + (uint32_t)j, slot = 2 * kt % M::kSlots, buf = scores_done % M::kScores;
+            if (!warp_wait(sy, &sy->k_full[kt % kRingBars], (kt / kRingBars) & 1u)) return false;
+            tc_fence_after();
+            const uint64_t qd = d0 + (uint32_t)((M::kQ + t * M::kTile) >> 4), kd = d0 + (uint32_t)((M::kRing + slot * M::kTile) >> 4);
+            if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t off = (k & 3) * 2 + (k >> 2) * (kSubBytes >> 4);
+                    tc_mma(tmem + 128 * buf, qd + off, kd + off, idesc_s, k ? 1u : 0u);
+                }
+                tc_commit(&sy->s_full[t][(blocks[t] + (uint32_t)(j - done[t])) & 3u]);
+                if (t == p.tiles - 1) tc_commit(&sy->slot_free[slot]);
+                if (n == total - 1) tc_commit(&sy->q_free);
+            }
+            __syncwarp();
+            ++scores_done;
+            return true;
+        };
+        const uint32_t first = scores_done;
+        if (!warp_wait(sy, &sy->q_full, items & 1u)) return;
+        for (int n = 0; n < M::kScores && n < total; ++n)
+            if (!scores(n)) return;
+        for (int n = 0; n < total; ++n) {
+            const int t = p.tiles == 2 ? n & 1 : 0, j = p.tiles == 2 ? n >> 1 : n;
+            const uint32_t kt = c + (uint32_t)j, slot = (2 * kt + 1) % M::kSlots, buf = (first + (uint32_t)n) % M::kScores;
+            if (!warp_wait(sy, &sy->p_full[t], blocks[t] & 1u)) return;
+            if (!warp_wait(sy, &sy->v_ready[kt % kRingBars], (kt / kRingBars) & 1u)) return;
+            // (the first product of an item overwrites O: the one before has been read)
+            if (j == 0 && !warp_wait(sy, &sy->o_free[t], (outs[t] & 1u) ^ 1u)) return;
+            tc_fence_after();
+            const uint64_t vd = v0 + (uint32_t)((M::kRing + slot * M::kTile) >> 4);
+            if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)            // 16 keys: 8 columns of P, 2048 bytes of V
+                    mma_ta(tmem + M::kO + D * t, tmem + 128 * buf + 8 * k, vd + 128 * k, idesc_o, j > 0 || k > 0 ? 1u : 0u);
+                tc_commit(&sy->pv_done[t][blocks[t] & 3u]);
+                if (t == p.tiles - 1) tc_commit(&sy->slot_free[slot]);
+            }
+            __syncwarp();
+            ++blocks[t];
+            ++done[t];
+            if (n + M::kScores < total && !scores(n + M::kScores)) return;
+        }
+        c += (uint32_t)p.units;
+        for (int t = 0; t < p.tiles; ++t) ++outs[t];
+        w.next(a, p.units);
+    }
+}
+
+// ---- values -------------------------------------------------------------------------------------------------------------------
+template <int DT, int D>
+__device__ __forceinline__ void value_role(const AttnArgs& a, uint8_t* smem, Sync* sy, Walk<kShift> w) {
+    using M = Map<D>;
+    const int lane = threadIdx.x & 31, half = (threadIdx.x >> 5) & 1;
+    uint32_t c = 0, items = 0;
+    for (; w.left > 0; ++items) {
+        const Part p = part_of(a, w);
+        int lo_all, hi_all, partial = 0;
+        seen_by_all(a, p, 0, p.tokens, lo_all, hi_all);
+        const uint32_t mem = items % kOddItems;
+        if (!warp_wait(sy, &sy->item_done[mem], ((items / kOddItems) & 1u) ^ 1u)) return;      // (the item that used it last has ended)
+        if (lane < kOddTiles * 2) sy->odd[mem][lane >> 1][half * 2 + (lane & 1)] = 0;
+        if (lane == 0) sy->odd_any[mem][half] = 0;
+        __syncwarp();
+        for (int u = 0; u < p.units; ++u, ++c) {
+            const uint32_t slot = (2 * c + 1) % M::kSlots;
+            if (!warp_wait(sy, &sy->v_full[c % kRingBars], (c / kRingBars) & 1u)) return;
+            const int key0 = p.key0 + (u << kShift);
+            const bool some = key0 < lo_all || key0 + 127 > hi_all;          // keys that some token does not see
+            const uint32_t there = *(volatile uint32_t*)&sy->there[c % kSeen];
+            if (some || there != 0xffu) {
+                const uint32_t tile = smem_u32(smem) + M::kRing + slot * M::kTile;
+                const bool look = some && p.tokens > 1;
+                for (int i = lane; i < 64 * 8 * M::kSubs; i += 32) {          // a warp has half of the rows
+                    const int sub = i >> 9, row = half * 64 + ((i >> 3) & 63), key = key0 + row;
+                    const uint32_t at = tile + sub * kSubBytes + row * 128 + (i & 7) * 16;
+                    if (key < p.lo || key > p.hi || !((there >> (row >> 4)) & 1u)) {
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+                    } else if (look) {
+                        uint32_t x[4];
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
+                        bool odd = false;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const bool l = odd_value<DT>(x[e]), h = odd_value<DT>(x[e] >> 16);
+                            odd |= l || h;
+                            x[e] &= (l ? 0u : 0xffffu) | (h ? 0u : 0xffff0000u);
+                        }
+                        if (odd && partial < kOddTiles) {
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+                            atomicOr(&sy->odd[mem][partial][row >> 5], 1u << (row & 31));
+                            *(volatile int*)&sy->odd_any[mem][half] = 1;
+                        }
+                    }
+                }
+                partial += some ? 1 : 0;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+            }
+            if (lane == 0) mbar_arrive(&sy->v_ready[c % kRingBars]);
+        }
+        w.next(a, p.units);
+    }
+}
+
+// ---- softmax ------------------------------------------------------------------------------------------------------------------
+template <int DT, int D>
+__device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<kShift> w, uint32_t tmem, int worker, int workers, long long total) {
+    using M = Map<D>;
+    constexpr float NEG_INF = -__builtin_huge_valf();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = warp >> 2, i = threadIdx.x & 127;     // tile and its row
+    const int tile_tokens = a.tokens / 2, my_token = i / a.group, my_head = i - my_token * a.group;
+    const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), ocol = tl + M::kO + D * t;
+    const long long end = (long long)(worker + 1) * total / workers;
+    uint32_t c = 0, items = 0, seq0 = 0, blocks = 0;
+    for (; w.left > 0; ++items) {
+        const Part p = part_of(a, w);
+        if (t < p.tiles) {
+            const int token = t * tile_tokens + my_token;
+            const bool mine = my_token < tile_tokens && token < p.tokens;
+            int lo, hi, lo_all, hi_all;
+            seen_by(a, p, min(token, p.tokens - 1), lo, hi);
+            seen_by_all(a, p, t * tile_tokens, min(p.tokens, (t + 1) * tile_tokens), lo_all, hi_all);
+            float m = NEG_INF, l = 0.f;
+            for (int u = 0; u < p.units; ++u) {
+                const uint32_t n = seq0 + (uint32_t)(u * p.tiles + t), buf = n % M::kScores;
+                const uint32_t scol = tl + 128 * buf;
+                if (!warp_wait(sy, &sy->s_full[t][blocks & 3u], (blocks >> 2) & 1u)) return;
+                tc_fence_after();
+                float s[128];
+#pragma unroll
+                for (int ch = 0; ch < 4; ++ch) tc_ld32(scol + ch * 32, s + ch * 32);
+                const int key0 = p.key0 + (u << kShift);
+                const uint32_t there = *(volatile uint32_t*)&sy->there[(c + (uint32_t)u) % kSeen];
+                if (key0 < lo_all || key0 + 127 > hi_all || there != 0xffu) {
+                    const int from = lo - key0, to = hi - key0;
+#pragma unroll
+                    for (int e = 0; e < 128; ++e)
+                        if (e < from || e > to || !((there >> (e >> 4)) & 1u)) s[e] = NEG_INF;
+                }
+                // (the scale is positive)
+                float m4[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+#pragma unroll
+                for (int e = 0; e < 128; e += 8) {
+                    m4[0] = max_3(m4[0], s[e], s[e + 1]); m4[1] = max_3(m4[1], s[e + 2], s[e + 3]);
+                    m4[2] = max_3(m4[2], s[e + 4], s[e + 5]); m4[3] = max_3(m4[3], s[e + 6], s[e + 7]);
+                }
+                const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale2;
+                float factor = 1.f;
+                if (mx > m + kLazy || (m == NEG_INF && mx != NEG_INF)) {
+                    factor = m == NEG_INF ? 0.f : ex2(m - mx);
+                    m = mx;
+                }
+                if (u > 0 && __any_sync(0xffffffffu, factor != 1.f)) {
+                    if (!warp_wait(sy, &sy->pv_done[t][(blocks - 1u) & 3u], ((blocks - 1u) >> 2) & 1u)) return;      // O is complete up to here
+                    tc_fence_after();
+                    l *= factor;
+#pragma unroll 1
+                    for (int ch = 0; ch < D / 16; ++ch) {
+                        float o[16];
+                        uint32_t x[16];
+                        tc_ld16(ocol + ch * 16, o);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(o[e] * factor);
+                        tmem_st16(ocol + ch * 16, x);
+                    }
+                }
+                const float mm = m == NEG_INF ? 0.f : m;                       // (no key so far: every score is -inf)
+                const float2 scale2 = make_float2(a.scale2, a.scale2), off2 = make_float2(-mm, -mm);
+                float2 l4[4] = {};
+#pragma unroll
+                for (int ch = 0; ch < 4; ++ch) {
+                    uint32_t x[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float2 y = fma_2(make_float2(s[ch * 32 + e], s[ch * 32 + e + 1]), scale2, off2);
+                        const float2 q = make_float2(ex2(y.x), ex2(y.y));
+                        l4[(e >> 1) & 3] = add_2(l4[(e >> 1) & 3], q);
+                        x[e >> 1] = pack16<DT>(q.x, q.y);
+                    }
+                    tmem_st16(scol + ch * 16, x);
+                }
+                l += ((l4[0].x + l4[0].y) + (l4[1].x + l4[1].y)) + ((l4[2].x + l4[2].y) + (l4[3].x + l4[3].y));
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sy->p_full[t]);                    // S read, P written
+                ++blocks;
+            }
+            // ---- results, or this part's statistics and products
+            if (!warp_wait(sy, &sy->pv_done[t][(blocks - 1u) & 3u], ((blocks - 1u) >> 2) & 1u)) return;
+            tc_fence_after();
+            const bool whole = p.begins && p.ends;
+            const long long slot_row = ((long long)worker * 2 + (p.begins ? 1 : 0)) * a.part_rows + token * a.group + my_head;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            if (p.begins && !p.ends && i == 0 && t == 0) {
+                const long long item_end = end + (w.item.units - p.units);     // (the item is not finished: the worker's last)
+                a.joins[worker] = make_int4(worker_before(item_end, total, workers) - worker + 1, p.row0, p.tokens * a.group, p.block);
+            }
+            uint16_t* const to = a.out + (long long)(p.row0 + token) * a.ld_out + (p.block * a.group + my_head) * D;
+            float* const part = a.parts + slot_row * D;
+            const uint32_t mem = items % kOddItems;
+            const bool odd = (*(volatile int*)&sy->odd_any[mem][0] | *(volatile int*)&sy->odd_any[mem][1]) != 0;
+            if (mine && !whole) reinterpret_cast<float2*>(a.stats)[slot_row] = make_float2(l != l && m == NEG_INF ? 0.f : m, l);
+#pragma unroll 1
+            for (int ch = 0; ch < D / 16; ++ch) {
+                float o[16];
+                tc_ld16(ocol + ch * 16, o);
+                if (ch == D / 16 - 1) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sy->o_free[t]);
+                }
+                if (odd && mine) {                                                     // values that are no numbers, for the tokens that see them
+                    int n = 0, alo, ahi;
+                    seen_by_all(a, p, 0, p.tokens, alo, ahi);
+                    for (int u = 0; u < p.units; ++u) {
+                        const int key0 = p.key0 + (u << kShift);
+                        if (!(key0 < alo || key0 + 127 > ahi)) continue;
+                        for (int r = 0; r < 128 && n < kOddTiles; ++r) {
+                            const int key = key0 + r;
+                            if (!((*(volatile uint32_t*)&sy->odd[mem][n][r >> 5] >> (r & 31)) & 1u) || key < lo || key > hi) continue;
+                            const int first = a.pages.page_row(p.s, key >> a.pages.shift);
+                            if (first < 0) continue;
+                            const uint16_t* v = a.v + (long long)(first + (key & ((1 << a.pages.shift) - 1))) * a.ld_v + p.block / a.shared * D + ch * 16;
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                const uint32_t h = v[e];
+                                if (odd_value<DT>(h)) o[e] += unpack16<DT>(h).x;
+                            }
+                        }
+                        ++n;
+                    }
+                }
+                if (mine && whole) {
+                    uint32_t x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = pack16<DT>(o[2 * e] * inv, o[2 * e + 1] * inv);
+                    reinterpret_cast<uint4*>(to + ch * 16)[0] = make_uint4(x[0], x[1], x[2], x[3]);
+                    reinterpret_cast<uint4*>(to + ch * 16)[1] = make_uint4(x[4], x[5], x[6], x[7]);
+                } else if (mine) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        reinterpret_cast<float4*>(part + ch * 16)[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                }
+                __syncwarp();
+            }
+            // (eight arrivals an item, all from warps that took part: one that passes an item by must not run ahead into the barrier's next phase)
+            if (lane == 0) {
+                mbar_arrive(&sy->item_done[items % kOddItems]);
+                if (p.tiles == 1) mbar_arrive(&sy->item_done[items % kOddItems]);
+            }
+        }
+        seq0 += (uint32_t)(p.units * p.tiles);
+        c += (uint32_t)p.units;
+        w.next(a, p.units);
+    }
+}
+
+template <int DT, int D>
+__global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk(const __grid_constant__ AttnArgs a, const __grid_constant__ Maps m) {
+    using M = Map<D>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    Sync& sy = *reinterpret_cast<Sync*>(smem + M::kBytes);
+    const int warp = threadIdx.x >> 5, worker = blockIdx.x;
+    if (threadIdx.x == 0) {
+        mbar_init(&sy.q_full, 1);
+        mbar_init(&sy.q_free, 1);
+        for (int i = 0; i < kRingBars; ++i) {
+            mbar_init(&sy.k_full[i], 1);
+            mbar_init(&sy.v_full[i], 1);
+            mbar_init(&sy.v_ready[i], 2);
+        }
+        for (int i = 0; i < M::kSlots; ++i) mbar_init(&sy.slot_free[i], 1);
+        for (int t = 0; t < 2; ++t) {
+            for (int i = 0; i < 4; ++i) {
+                mbar_init(&sy.s_full[t][i], 1);
+                mbar_init(&sy.pv_done[t][i], 1);
+            }
+            mbar_init(&sy.p_full[t], 4);
+            mbar_init(&sy.o_free[t], 4);
+        }
+        for (int i = 0; i < kOddItems; ++i) mbar_init(&sy.item_done[i], 8);
+        sy.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sy.tmem)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    wait_for_previous_kernel();
+    let_next_kernel_launch();
+    Walk<kShift> w;
+    long long total;
+    const int workers = plan<kShift, kChunkThreads>(a, reinterpret_cast<PlanScratch<kChunkThreads>*>(smem), worker, 1, w, total);
+    if (threadIdx.x == 0) a.joins[worker] = make_int4(0, 0, 0, 0);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");              // (copies go where the plan's sums were)
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *(volatile uint32_t*)&sy.tmem;
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        softmax_role<DT, D>(a, &sy, w, tmem, worker, max(workers, 1), total);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (warp == 8) load_role<D>(a, m, smem, &sy, w);
+        else if (warp == 9) product_role<DT, D>(a, smem, &sy, w, tmem);
+        else value_role<DT, D>(a, smem, &sy, w);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 9) {
+        if (*(volatile int*)&sy.abort) __nanosleep(200000);                    // (products that were issued have ended)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------------
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess;
+        (void)cudaGetLastError();
+        return ok ? reinterpret_cast<EncodeTiled>(ptr) : nullptr;
+    }();
+    return fn;
+}
+// boxes of 64 columns, 128-byte swizzle, zeros outside
+bool encode(CUtensorMap* m, int dtype, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+    const cuuint32_t ones[3] = {1, 1, 1};
+    return encode_tiled()(m, dtype == DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base),
+                          dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DT, int D>
+cudaError_t launch(const AttnArgs& a, const Maps& m, cudaStream_t stream) {
+    constexpr int bytes = Map<D>::kBytes + sizeof(Sync);
+    static_assert(bytes <= 232448, "shared memory of a block");
+    const cudaError_t e = cudaFuncSetAttribute(attend_chunk<DT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute pdl;
+    pdl.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    pdl.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)a.workers);
+    cfg.blockDim = dim3(kChunkThreads);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = stream;
+    cfg.attrs = &pdl;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attend_chunk<DT, D>, a, m);
+}
+
+}  // namespace
+
+cudaError_t launch_chunk(const AttnArgs& a, const mk_paged_cache* c, int heads, cudaStream_t stream) {
+    if (!encode_tiled()) return cudaErrorNotSupported;
+    Maps m;
+    const int D = c->head_dim, box_rows = c->page_size < kTileRows ? c->page_size : kTileRows;
+    const cuuint64_t qd[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)a.batch.rows}, qs[2] = {(cuuint64_t)D * 2, (cuuint64_t)a.ld_q * 2};
+    const cuuint32_t qb[3] = {64, (cuuint32_t)a.group, (cuuint32_t)(a.tokens / 2)};
+    const cuuint64_t cd[2] = {(cuuint64_t)c->kv_heads * D, (cuuint64_t)c->pages * c->page_size}, ks[1] = {(cuuint64_t)a.ld_k * 2}, vs[1] = {(cuuint64_t)a.ld_v * 2};
+    const cuuint32_t cb[2] = {64, (cuuint32_t)box_rows};
+    const bool empty = c->pages == 0;                  // (then no box is ever asked for)
+    if (!encode(&m.q, c->dtype, 3, a.q, qd, qs, qb)) return cudaErrorInvalidValue;
+    if (empty) m.k = m.v = m.q;
+    else if (!encode(&m.k, c->dtype, 2, a.k, cd, ks, cb) || !encode(&m.v, c->dtype, 2, a.v, cd, vs, cb)) return cudaErrorInvalidValue;
+    if (c->dtype == DT_F16) return D == 64 ? launch<DT_F16, 64>(a, m, stream) : launch<DT_F16, 128>(a, m, stream);
+    return D == 64 ? launch<DT_BF16, 64>(a, m, stream) : launch<DT_BF16, 128>(a, m, stream);
+}
+
+cudaError_t chunk_status(int* failed, cudaStream_t stream) {
+    const int zero = 0;
+    cudaError_t e = cudaMemcpyFromSymbolAsync(failed, g_paged_failed, sizeof(int), 0, cudaMemcpyDeviceToHost, stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+    if (e == cudaSuccess && *failed) {
+        e = cudaMemcpyToSymbolAsync(g_paged_failed, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+    }
+    return e;
+}
+
+}  // namespace mk

@@ -457,6 +457,26 @@ def test_paged_attention_repeats(cuda, new, seqs, ctx):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D,H,KVH,dtype,window", [(64, 4, 4, BF, 0), (128, 8, 4, HALF, 0), (128, 14, 2, BF, 50), (64, 32, 8, BF, 0)])
+def test_paged_attention_many_items(cuda, D, H, KVH, dtype, window):
+    """More items than SMs by far, of one and two operand tiles and of one and several key tiles, one behind the other in a block: single tokens
+    between chunks, sequences without rows."""
+    seqs = 260
+    pos = [(37 * i) % 300 for i in range(seqs)]
+    new = [(1, 0, 40, 1, 1, 2, 90, 1, 1, 1, 1, 1, 9)[i % 13] for i in range(seqs)]
+    new[17] = 200
+    args, kw = make_attention(pos, new, H, KVH, D, 16, dtype, seed=D + H)
+    for hint in (1, 200):
+        got = mc.paged_attention(**on(cuda, args), **kw, window=window, max_new=hint).cpu()
+        assert _lib.load().mk_paged_attention_status(0, torch.cuda.current_stream().cuda_stream) == 0
+        for s in list(range(0, seqs, 23)) + [17, 18, 19]:
+            r0, r1 = int(args["starts"][s]), int(args["starts"][s + 1])
+            one = dict(args, q=args["q"][r0:r1], pos=args["pos"][s:s + 1], pages=args["pages"][s:s + 1], starts=None)
+            if r1 > r0:
+                check_attention(cuda, one, dict(kw, window=window), got=got[r0:r1])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [1, 24])
 def test_captured_steps_follow_their_arguments(cuda, new):
     """A captured append and attention: each replay works with the positions, pages and rows of its own time; two graphs beside each other."""
