@@ -50,8 +50,8 @@ struct Sync {
     unsigned long long q_full, q_free;                // one per item
     unsigned long long k_full[kRingBars], v_full[kRingBars], v_ready[kRingBars];           // key tile c: c % kRingBars
     unsigned long long slot_free[10];                 // slots of the ring of tiles
-    unsigned long long s_full[2][4], pv_done[2][4];   // tile t's k-th block of scores: k % 4
-    unsigned long long p_full[2], o_free[2], item_done[kOddItems];
+    unsigned long long s_full[2][4], p_full[2][4], pv_done[2][4];                          // tile t's k-th block of scores: k % 4
+    unsigned long long o_free[2], item_done[kOddItems];
     uint32_t tmem;
     int abort;
     uint32_t there[kSeen];                            // bit b: keys [16 b, 16 b + 16) of the tile are loaded
@@ -93,6 +93,19 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* w) {
         "r"(w[11]), "r"(w[12]), "r"(w[13]), "r"(w[14]), "r"(w[15])
         : "memory");
 }
+// 32 columns of this thread's lane, not waited for
+__device__ __forceinline__ void tmem_ld32(uint32_t at, float* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+        "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+          "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
+          "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]),
+          "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // D (+)= A B with A in tensor memory
 __device__ __forceinline__ void mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -281,7 +294,7 @@ __device__ __forceinline__ void product_role(const AttnArgs& a, uint8_t* smem, S
         for (int n = 0; n < total; ++n) {
             const int t = p.tiles == 2 ? n & 1 : 0, j = p.tiles == 2 ? n >> 1 : n;
             const uint32_t kt = c + (uint32_t)j, slot = (2 * kt + 1) % M::kSlots, buf = (first + (uint32_t)n) % M::kScores;
-            if (!warp_wait(sy, &sy->p_full[t], blocks[t] & 1u)) return;
+            if (!warp_wait(sy, &sy->p_full[t][blocks[t] & 3u], (blocks[t] >> 2) & 1u)) return;
             if (!warp_wait(sy, &sy->v_ready[kt % kRingBars], (kt / kRingBars) & 1u)) return;
             // (the first product of an item overwrites O: the one before has been read)
             if (j == 0 && !warp_wait(sy, &sy->o_free[t], (outs[t] & 1u) ^ 1u)) return;
@@ -387,7 +400,10 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
                 tc_fence_after();
                 float s[128];
 #pragma unroll
-                for (int ch = 0; ch < 4; ++ch) tc_ld32(scol + ch * 32, s + ch * 32);
+                for (int ch = 0; ch < 4; ++ch) tmem_ld32(scol + ch * 32, s + ch * 32);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 128; ++e) asm volatile("" : "+f"(s[e]));       // (used behind the wait)
                 const int key0 = p.key0 + (u << kShift);
                 const uint32_t there = *(volatile uint32_t*)&sy->there[(c + (uint32_t)u) % kSeen];
                 if (key0 < lo_all || key0 + 127 > hi_all || there != 0xffu) {
@@ -442,7 +458,7 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sy->p_full[t]);                    // S read, P written
+                if (lane == 0) mbar_arrive(&sy->p_full[t][blocks & 3u]);                    // S read, P written
                 ++blocks;
             }
             // ---- results, or this part's statistics and products
@@ -533,9 +549,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk(const __grid_co
         for (int t = 0; t < 2; ++t) {
             for (int i = 0; i < 4; ++i) {
                 mbar_init(&sy.s_full[t][i], 1);
+                mbar_init(&sy.p_full[t][i], 4);
                 mbar_init(&sy.pv_done[t][i], 1);
             }
-            mbar_init(&sy.p_full[t], 4);
             mbar_init(&sy.o_free[t], 4);
         }
         for (int i = 0; i < kOddItems; ++i) mbar_init(&sy.item_done[i], 8);

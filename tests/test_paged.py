@@ -424,7 +424,7 @@ def test_paged_attention_far_rows(cuda):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("new,seqs,ctx", [(1, 1, 5000), (1, 70, 300), (3, 2, 2500), (200, 1, 3000), (33, 40, 100)])
+@pytest.mark.parametrize("new,seqs,ctx", [(1, 1, 5000), (1, 70, 300), (3, 2, 2500), (200, 1, 3000), (33, 40, 100), (16, 16, 1500)])
 def test_paged_attention_repeats(cuda, new, seqs, ctx):
     """Long and many sequences, against 64-bit torch on the GPU; a second call gives the same bits, on another stream beside other calls too."""
     H, KVH, D, page = 8, 2, 64, 32
