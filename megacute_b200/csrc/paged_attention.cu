@@ -8,80 +8,17 @@ namespace mk {
 namespace {
 
 constexpr int kJoinThreads = 256;
-constexpr int kJoinRows = 16;                         // rows of a block
 
-// Block (x, y): items that the workers [x * per_block, (x + 1) * per_block) begin and do not end, rows [y * kJoinRows, ...) of them.
-// With M the largest of the parts' maxima m_i: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, in the order of the parts.
-// A warp has a row; where there are fewer rows than warps, several warps share a row's parts and add through shared memory.
-template <int DT, int D>
-__global__ void __launch_bounds__(kJoinThreads) join_parts(const __grid_constant__ AttnArgs a, int per_block) {
-    constexpr int V = D / 32, WARPS = kJoinThreads / 32;
-    __shared__ float sums[WARPS][D];
+// Block (x, y): the item that block x begins and does not end, rows [y * ROWS, (y + 1) * ROWS) of it.
+template <int DT, int D, int ROWS>
+__global__ void __launch_bounds__(kJoinThreads) join_parts(const __grid_constant__ AttnArgs a) {
+    __shared__ Join<D, ROWS, kJoinThreads> join;
     wait_for_previous_kernel();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int w = blockIdx.x * per_block; w < (blockIdx.x + 1) * per_block; ++w) {
-        const int4 j = __ldcg(a.joins + w);
-        const int first = blockIdx.y * kJoinRows, rows = min(kJoinRows, j.z - first);
-        if (j.x == 0 || rows <= 0) continue;
-        int across = 1;                               // rows side by side
-        while (across < rows && across < WARPS) across <<= 1;
-        const int split = warp / across, splits = WARPS / across;
-        for (int r = warp % across; r < (rows + across - 1) / across * across; r += across) {
-            const int row = first + min(r, rows - 1);
-            auto slot = [&](int i) { return (long long)(i == 0 ? 2 * w + 1 : 2 * (w + i)) * a.part_rows + row; };
-            float m = -__builtin_huge_valf(), l = 0.f;
-            for (int i = lane; i < j.x; i += 32) {
-                const float2 st = __ldcg(reinterpret_cast<const float2*>(a.stats) + slot(i));
-                const float to = fmaxf(m, st.x);
-                if (to != -__builtin_huge_valf()) l = l * (m == to ? 1.f : ex2(m - to)) + st.y * (st.x == to ? 1.f : ex2(st.x - to));
-                m = to;
-            }
-#pragma unroll
-            for (int d = 16; d; d >>= 1) {
-                const float m2 = __shfl_xor_sync(0xffffffffu, m, d), l2 = __shfl_xor_sync(0xffffffffu, l, d), to = fmaxf(m, m2);
-                if (to != -__builtin_huge_valf()) l = l * (m == to ? 1.f : ex2(m - to)) + l2 * (m2 == to ? 1.f : ex2(m2 - to));
-                m = to;
-            }
-            float o[V];
-#pragma unroll
-            for (int e = 0; e < V; ++e) o[e] = 0.f;
-            if (m != -__builtin_huge_valf()) {
-#pragma unroll 4
-                for (int i = split; i < j.x; i += splits) {
-                    const long long at = slot(i);
-                    const float mi = __ldcg(a.stats + 2 * at), f = mi == m ? 1.f : ex2(mi - m);
-                    float x[V];
-                    if (V == 4) {
-                        const float4 t = __ldcg(reinterpret_cast<const float4*>(a.parts + at * D) + lane);
-                        x[0] = t.x; x[1] = t.y; x[V - 2] = t.z; x[V - 1] = t.w;
-                    } else {
-                        const float2 t = __ldcg(reinterpret_cast<const float2*>(a.parts + at * D) + lane);
-                        x[0] = t.x; x[1] = t.y;
-                    }
-                    if (mi != -__builtin_huge_valf()) {
-#pragma unroll
-                        for (int e = 0; e < V; ++e) o[e] += f * x[e];
-                    }
-                }
-            }
-            if (splits > 1) {                         // (one turn of the loop over rows: across >= rows)
-                __syncthreads();
-#pragma unroll
-                for (int e = 0; e < V; ++e) sums[warp][lane * V + e] = o[e];
-                __syncthreads();
-                if (split > 0) continue;
-                for (int k = 1; k < splits; ++k)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) o[e] += sums[warp + k * across][lane * V + e];
-            }
-            if (r >= rows) continue;
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            const int tok = row / a.group;
-            uint32_t* to = reinterpret_cast<uint32_t*>(a.out + (j.y + tok) * a.ld_out + (j.w * a.group + row - tok * a.group) * D) + lane * (V / 2);
-            if (V == 4) *reinterpret_cast<uint2*>(to) = make_uint2(pack16<DT>(o[0] * inv, o[1] * inv), pack16<DT>(o[V - 2] * inv, o[V - 1] * inv));
-            else *to = pack16<DT>(o[0] * inv, o[1] * inv);
-        }
-    }
+    const int w = blockIdx.x, first = blockIdx.y * ROWS;
+    const int4 j = __ldcg(a.joins + w);
+    if (j.x == 0 || first >= j.z) return;
+    join.run(a, a.stats, a.parts, j.x, first, min(first + ROWS, j.z), [&](int i) { return (long long)(i == 0 ? 2 * w + 1 : 2 * (w + i)); },
+             [&](int row, int col, float, float l, const float4& o) { write_result<DT, D>(a, j.y, j.w, row, col, l, o); });
 }
 
 const char* shape_error(const mk_paged_cache* cache, int heads) {
@@ -116,34 +53,36 @@ int heads_of_block(int group, int rows) {
 // Which kernel takes a call: the one for few rows where an item of 16 rows holds all new tokens of a sequence (then every key is read once).
 bool few_rows(int group, long long max_new) { return max_new * group <= kFewRows; }
 
-// what the workspace holds, one behind the other: joins, stats, parts
+// what the workspace holds, one behind the other: joins, stats and parts of the blocks, stats and parts of the warps (few rows)
 struct Layout {
-    int workers, part_rows, per_block;
-    size_t stats, parts, bytes;
+    int workers, part_rows;
+    size_t stats, parts, own_stats, own_parts, bytes;
 };
 Layout layout_of(int sms, int head_dim, bool few) {
     Layout l;
-    l.per_block = few ? kFewWarps : 1;
-    l.workers = sms * l.per_block;
+    l.workers = few ? sms * kFewWarps : sms;
     l.part_rows = few ? kFewRows : 2 * kChunkTile;
-    l.stats = (size_t)l.workers * sizeof(int4);
-    l.parts = l.stats + (size_t)l.workers * 2 * l.part_rows * 2 * sizeof(float);
-    l.bytes = l.parts + (size_t)l.workers * 2 * l.part_rows * head_dim * sizeof(float);
+    const size_t rows = (size_t)sms * 2 * l.part_rows, own_rows = few ? (size_t)l.workers * 2 * kFewRows : 0;
+    l.stats = (size_t)sms * sizeof(int4);
+    l.parts = l.stats + rows * sizeof(float2);
+    l.own_stats = l.parts + rows * head_dim * sizeof(float);
+    l.own_parts = l.own_stats + own_rows * sizeof(float2);
+    l.bytes = l.own_parts + own_rows * head_dim * sizeof(float);
     return l;
 }
 
-template <int DT, int D>
-cudaError_t launch_join(const AttnArgs& a, int per_block, cudaStream_t stream) {
+template <int DT, int D, int ROWS>
+cudaError_t launch_join(const AttnArgs& a, int blocks, cudaStream_t stream) {
     cudaLaunchAttribute pdl;
     pdl.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     pdl.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.workers / per_block), (unsigned)((a.part_rows + kJoinRows - 1) / kJoinRows));
+    cfg.gridDim = dim3((unsigned)blocks, (unsigned)((a.tokens * a.group + ROWS - 1) / ROWS));
     cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = stream;
     cfg.attrs = &pdl;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, join_parts<DT, D>, a, per_block);
+    return cudaLaunchKernelEx(&cfg, join_parts<DT, D, ROWS>, a);
 }
 
 }  // namespace
@@ -200,14 +139,18 @@ extern "C" int mk_paged_attention(int device, const mk_batch* batch, const mk_pa
     a.workers = lay.workers;
     a.part_rows = lay.part_rows;
     a.joins = (int4*)workspace;
-    a.stats = (float*)((uint8_t*)workspace + lay.stats);
+    a.stats = (float2*)((uint8_t*)workspace + lay.stats);
     a.parts = (float*)((uint8_t*)workspace + lay.parts);
     cudaStream_t st = (cudaStream_t)stream;
     a.tokens = few ? kFewRows / a.group : kChunkTile / a.group * 2;
-    cudaError_t e = few ? launch_few(a, D, cache->dtype, sms, st) : launch_chunk(a, cache, heads, st);
+    const FewParts own = {(float2*)((uint8_t*)workspace + lay.own_stats), (float*)((uint8_t*)workspace + lay.own_parts)};
+    cudaError_t e = few ? launch_few(a, own, D, cache->dtype, sms, st) : launch_chunk(a, cache, heads, st);
     if (e == cudaSuccess) {
-        if (cache->dtype == DT_F16) e = D == 64 ? launch_join<DT_F16, 64>(a, lay.per_block, st) : launch_join<DT_F16, 128>(a, lay.per_block, st);
-        else e = D == 64 ? launch_join<DT_BF16, 64>(a, lay.per_block, st) : launch_join<DT_BF16, 128>(a, lay.per_block, st);
+        // (few rows of many parts or many rows of few)
+        if (few && cache->dtype == DT_F16) e = D == 64 ? launch_join<DT_F16, 64, 4>(a, sms, st) : launch_join<DT_F16, 128, 4>(a, sms, st);
+        else if (few) e = D == 64 ? launch_join<DT_BF16, 64, 4>(a, sms, st) : launch_join<DT_BF16, 128, 4>(a, sms, st);
+        else if (cache->dtype == DT_F16) e = D == 64 ? launch_join<DT_F16, 64, 16>(a, sms, st) : launch_join<DT_F16, 128, 16>(a, sms, st);
+        else e = D == 64 ? launch_join<DT_BF16, 64, 16>(a, sms, st) : launch_join<DT_BF16, 128, 16>(a, sms, st);
     }
     if (e == cudaSuccess) return MK_OK;
     (void)cudaGetLastError();

@@ -5,8 +5,8 @@
 // sequence, block of heads, tokens -- make one list, which is dealt out evenly: worker w has units [w N / W, (w + 1) N / W).  Lengths are known on
 // the device only, so every block works out its part itself, and batches of the most unlike lengths load all SMs alike.
 // A worker that has an item's units from the first to the last writes results.  Else it leaves the running maximum, the sum and the products of its
-// part in the workspace (slot 0 of the worker: a part that does not begin the item; slot 1: one that begins it), and a second kernel
-// (paged_attention.cu) joins them, always in the same order.
+// part in the workspace (slot 0: a part that does not begin the item; slot 1: one that begins it); a block joins the parts that its
+// own workers have of an item, and a second kernel (paged_attention.cu) those of several blocks, always in the same order.
 #pragma once
 #include "paged.cuh"
 
@@ -24,10 +24,10 @@ struct AttnArgs {
     float scale2;                                     // scale * log2(e)
     int tokens;                                       // new tokens of an item
     int workers, part_rows;                           // ... and rows of a part in the workspace
-    int4* joins;                                      // of each worker: parts of the item that it begins and does not end (0: none), its first
+    int4* joins;                                      // of each block: parts of the item that it begins and does not end (0: none), its first
                                                       // row, its rows, its block of heads
-    float* stats;                                     // [worker][2][part_rows][2]: maximum (log2 domain) and sum
-    float* parts;                                     // [worker][2][part_rows][head_dim]
+    float2* stats;                                    // [block][2][part_rows]: maximum (log2 domain) and sum
+    float* parts;                                     // [block][2][part_rows][head_dim]
 };
 
 struct Item {
@@ -172,10 +172,76 @@ __device__ __forceinline__ int plan(const AttnArgs& a, PlanScratch<THREADS>* sc,
     return workers;
 }
 
+// Joins `count` parts of rows [row_begin, row_end) of an item, ROWS of them: part i has `slot(i)`.  With M the largest of their maxima m_i
+//   l = sum_i 2^(m_i - M) l_i,   o = sum_i 2^(m_i - M) o_i,   in the order of i.
+// A thread has four columns of a row; where that leaves threads over they share a row's parts and add through shared memory.  All threads of the block
+// call it.  `write(row, column, M, l, o)` takes four columns.
+template <int D, int ROWS, int THREADS>
+struct Join {
+    static constexpr int kLanes = D / 4, kTasks = ROWS * kLanes, kSplits = kTasks < THREADS ? THREADS / kTasks : 1;
+    static constexpr int kTurns = kTasks > THREADS ? kTasks / THREADS : 1;
+    float4 o[kSplits > 1 ? THREADS : 1];
+    float l[kSplits > 1 ? THREADS : 1];
+
+    template <class Slot, class Write>
+    __device__ __forceinline__ void run(const AttnArgs& a, const float2* stats, const float* parts, int count, int row_begin, int row_end, Slot slot,
+                                        Write write) {
+        const int t = threadIdx.x, lane = t % kLanes, split = kSplits > 1 ? t / kTasks : 0;
+#pragma unroll
+        for (int turn = 0; turn < kTurns; ++turn) {
+            const int row = row_begin + (t % kTasks) / kLanes + turn * (THREADS / kLanes);
+            const bool mine = row < row_end;
+            float m = -__builtin_huge_valf(), sum = 0.f;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (mine) {
+#pragma unroll 8
+                for (int i = 0; i < count; ++i) m = fmaxf(m, __ldcg(&stats[slot(i) * a.part_rows + row].x));
+#pragma unroll 8
+                for (int i = split; i < count; i += kSplits) {
+                    const long long at = slot(i) * a.part_rows + row;
+                    const float2 st = __ldcg(&stats[at]);
+                    const float4 v = __ldcg(reinterpret_cast<const float4*>(parts + at * D) + lane);
+                    const float f = st.x == m ? 1.f : ex2(st.x - m);
+                    if (st.x != -__builtin_huge_valf()) {                      // (a part that saw no key has nothing to add)
+                        sum += f * st.y;
+                        x.x += f * v.x; x.y += f * v.y; x.z += f * v.z; x.w += f * v.w;
+                    }
+                }
+            }
+            if (kSplits > 1) {
+                __syncthreads();                      // (what a call before this one left has been read)
+                o[t] = x;
+                l[t] = sum;
+                __syncthreads();
+                if (split > 0) continue;
+                for (int k = 1; k < kSplits; ++k) {
+                    const float4 v = o[t + k * kTasks];
+                    sum += l[t + k * kTasks];
+                    x.x += v.x; x.y += v.y; x.z += v.z; x.w += v.w;
+                }
+            }
+            if (mine) write(row, lane * 4, m, sum, x);
+        }
+    }
+};
+
+// four columns of an item's row (of `a.group` heads a token) of the result
+template <int DT, int D>
+__device__ __forceinline__ void write_result(const AttnArgs& a, int row0, int block, int row, int col, float l, const float4& o) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;       // (no key: zeros)
+    const int tok = row / a.group;
+    uint16_t* to = a.out + (long long)(row0 + tok) * a.ld_out + (block * a.group + row - tok * a.group) * D + col;
+    *reinterpret_cast<uint2*>(to) = make_uint2(pack16<DT>(o.x * inv, o.y * inv), pack16<DT>(o.z * inv, o.w * inv));
+}
+
 // items of few rows (paged_attention_few.cu): rows of an item, workers of a block
 constexpr int kFewRows = 16;
 constexpr int kFewWarps = 8;
-cudaError_t launch_few(const AttnArgs& a, int head_dim, int dtype, int blocks, cudaStream_t stream);
+struct FewParts {                                     // parts of the warps: [worker][2][kFewRows] and [worker][2][kFewRows][head_dim]
+    float2* stats;
+    float* parts;
+};
+cudaError_t launch_few(const AttnArgs& a, const FewParts& own, int head_dim, int dtype, int blocks, cudaStream_t stream);
 
 // items of up to 256 rows, a positive scale (paged_attention_chunk.cu): two tiles of 128 rows, a worker per block
 constexpr int kChunkTile = 128;

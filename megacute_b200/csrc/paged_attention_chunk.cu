@@ -28,6 +28,8 @@ namespace {
 
 constexpr int kChunkThreads = 384;
 constexpr float kLazy = 8.0f;
+constexpr uint32_t kFmaPairs = 0b01001001;            // of eight pairs of exponentials, those that the fp32 units take
+template <bool V> struct Const { static constexpr bool value = V; };
 constexpr unsigned long long kWaitNs = 2000000000ull;
 constexpr int kTileRows = 128;
 constexpr int kSubBytes = kTileRows * 128;            // 64 columns of a tile of 128 rows
@@ -74,6 +76,7 @@ __device__ __forceinline__ bool wait_bar(Sync* s, unsigned long long* bar, uint3
     return true;
 }
 __device__ __forceinline__ bool warp_wait(Sync* s, unsigned long long* bar, uint32_t parity) {
+    if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
     return __all_sync(0xffffffffu, wait_bar(s, bar, parity));
 }
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* m, int x, int y, unsigned long long* bar) {
@@ -105,6 +108,10 @@ __device__ __forceinline__ void tmem_ld32(uint32_t at, float* v) {
         : "r"(at)
         : "memory");
 }
+__device__ __forceinline__ void use32(float* v) {                             // what was loaded is read behind this point (the wait in front of it)
+#pragma unroll
+    for (int e = 0; e < 32; ++e) asm volatile("" : "+f"(v[e]));
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // D (+)= A B with A in tensor memory
@@ -127,9 +134,23 @@ __device__ __forceinline__ float2 add_2(float2 a, float2 b) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
+// 2^y of a pair without the special function units: y = n + f, n whole, |f| <= 1/2; 2^f by the polynomial of degree 4 whose relative error
+// is least over that range (2^-18.5, computed with Remez' exchange), n added to its exponent.  For y in [-inf, 127), as 2^-125 below that; not for NaN.
+__device__ __forceinline__ float2 ex2_fma(float2 y) {
+    const float2 big = make_float2(12582912.f, 12582912.f);                    // 1.5 * 2^23: the sum's last bit is one
+    y = make_float2(fmaxf(y.x, -125.f), fmaxf(y.y, -125.f));
+    const float2 t = add_2(y, big), n = add_2(t, make_float2(-big.x, -big.y)), f = fma_2(n, make_float2(-1.f, -1.f), y);
+    float2 q = fma_2(f, make_float2(0x1.3997d6p-7f, 0x1.3997d6p-7f), make_float2(0x1.ca1440p-5f, 0x1.ca1440p-5f));
+    q = fma_2(q, f, make_float2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+    q = fma_2(q, f, make_float2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+    q = fma_2(q, f, make_float2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+    return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
+}
+// the largest of three, NaN if one is
 __device__ __forceinline__ float max_3(float a, float b, float c) {
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 template <int DT>
@@ -267,11 +288,16 @@ __device__ __forceinline__ void product_role(const AttnArgs& a, uint8_t* smem, S
         const Part p = part_of(a, w);
         const int total = p.units * p.tiles;
         int done[2] = {0, 0};                         // blocks of this item whose P V has been issued (`blocks`: of all)
+        const uint32_t first = scores_done;
+        // K of the n-th block has landed (asked for ahead of its product, and for the first of two tiles only)
+        auto landed = [&](int n) {
+            const int t = p.tiles == 2 ? n & 1 : 0;
+            const uint32_t kt = c + (uint32_t)(p.tiles == 2 ? n >> 1 : n);
+            return t != 0 || warp_wait(sy, &sy->k_full[kt % kRingBars], (kt / kRingBars) & 1u);
+        };
         auto scores = [&](int n) {
             const int t = p.tiles == 2 ? n & 1 : 0, j = p.tiles == 2 ? n >> 1 : n;
-            const uint32_t kt = c + (uint32_t)j, slot = 2 * kt % M::kSlots, buf = scores_done % M::kScores;
-            if (!warp_wait(sy, &sy->k_full[kt % kRingBars], (kt / kRingBars) & 1u)) return false;
-            tc_fence_after();
+            const uint32_t slot = 2 * (c + (uint32_t)j) % M::kSlots, buf = scores_done % M::kScores;
             const uint64_t qd = d0 + (uint32_t)((M::kQ + t * M::kTile) >> 4), kd = d0 + (uint32_t)((M::kRing + slot * M::kTile) >> 4);
             if (elect_one()) {
 #pragma unroll
@@ -285,19 +311,22 @@ __device__ __forceinline__ void product_role(const AttnArgs& a, uint8_t* smem, S
             }
             __syncwarp();
             ++scores_done;
-            return true;
         };
-        const uint32_t first = scores_done;
         if (!warp_wait(sy, &sy->q_full, items & 1u)) return;
-        for (int n = 0; n < M::kScores && n < total; ++n)
-            if (!scores(n)) return;
+        for (int n = 0; n < M::kScores && n < total; ++n) {
+            if (!landed(n)) return;
+            tc_fence_after();
+            scores(n);
+        }
         for (int n = 0; n < total; ++n) {
             const int t = p.tiles == 2 ? n & 1 : 0, j = p.tiles == 2 ? n >> 1 : n;
             const uint32_t kt = c + (uint32_t)j, slot = (2 * kt + 1) % M::kSlots, buf = (first + (uint32_t)n) % M::kScores;
-            if (!warp_wait(sy, &sy->p_full[t][blocks[t] & 3u], (blocks[t] >> 2) & 1u)) return;
-            if (!warp_wait(sy, &sy->v_ready[kt % kRingBars], (kt / kRingBars) & 1u)) return;
+            const bool more = n + M::kScores < total;
+            if (t == 0 && !warp_wait(sy, &sy->v_ready[kt % kRingBars], (kt / kRingBars) & 1u)) return;
+            if (more && !landed(n + M::kScores)) return;
             // (the first product of an item overwrites O: the one before has been read)
             if (j == 0 && !warp_wait(sy, &sy->o_free[t], (outs[t] & 1u) ^ 1u)) return;
+            if (!warp_wait(sy, &sy->p_full[t][blocks[t] & 3u], (blocks[t] >> 2) & 1u)) return;
             tc_fence_after();
             const uint64_t vd = v0 + (uint32_t)((M::kRing + slot * M::kTile) >> 4);
             if (elect_one()) {
@@ -310,7 +339,7 @@ __device__ __forceinline__ void product_role(const AttnArgs& a, uint8_t* smem, S
             __syncwarp();
             ++blocks[t];
             ++done[t];
-            if (n + M::kScores < total && !scores(n + M::kScores)) return;
+            if (more) scores(n + M::kScores);
         }
         c += (uint32_t)p.units;
         for (int t = 0; t < p.tiles; ++t) ++outs[t];
@@ -340,24 +369,49 @@ __device__ __forceinline__ void value_role(const AttnArgs& a, uint8_t* smem, Syn
             const bool some = key0 < lo_all || key0 + 127 > hi_all;          // keys that some token does not see
             const uint32_t there = *(volatile uint32_t*)&sy->there[c % kSeen];
             if (some || there != 0xffu) {
-                const uint32_t tile = smem_u32(smem) + M::kRing + slot * M::kTile;
-                const bool look = some && p.tokens > 1;
-                for (int i = lane; i < 64 * 8 * M::kSubs; i += 32) {          // a warp has half of the rows
-                    const int sub = i >> 9, row = half * 64 + ((i >> 3) & 63), key = key0 + row;
-                    const uint32_t at = tile + sub * kSubBytes + row * 128 + (i & 7) * 16;
-                    if (key < p.lo || key > p.hi || !((there >> (row >> 4)) & 1u)) {
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
-                    } else if (look) {
+                const uint32_t tile = smem_u32(smem) + M::kRing + slot * M::kTile + half * 8192 + lane * 16;      // a warp has half of the rows
+                // rows 4 i + lane / 8 of the half: `none`: nobody sees them; `part`: some do
+                uint32_t none = 0, part = 0;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int row = half * 64 + 4 * i + (lane >> 3), key = key0 + row;
+                    const bool out = key < p.lo || key > p.hi || !((there >> (row >> 4)) & 1u);
+                    none |= (uint32_t)out << i;
+                    part |= (uint32_t)(!out && (key < lo_all || key > hi_all)) << i;
+                }
+                uint32_t odd = 0;                     // top bit of each 16 bits: an exponent of all ones
+                constexpr uint32_t E = DT == DT_F16 ? 0x7c007c00u : 0x7f807f80u, ONE = DT == DT_F16 ? 0x04000400u : 0x00800080u;
+#pragma unroll
+                for (int sub = 0; sub < M::kSubs; ++sub) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const uint32_t at = tile + sub * kSubBytes + i * 512;
+                        if ((none >> i) & 1u) {
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+                        } else if ((part >> i) & 1u) {
+                            uint32_t x[4];
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) odd |= (x[e] & E) + ONE;
+                        }
+                    }
+                }
+                if (__any_sync(0xffffffffu, odd & 0x80008000u) && partial < kOddTiles) {
+                    for (int k = 0; k < 16 * M::kSubs; ++k) {
+                        const int i = k & 15;
+                        const uint32_t at = tile + (k >> 4) * kSubBytes + i * 512;
+                        if (!((part >> i) & 1u)) continue;
                         uint32_t x[4];
                         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
-                        bool odd = false;
+                        bool any = false;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const bool l = odd_value<DT>(x[e]), h = odd_value<DT>(x[e] >> 16);
-                            odd |= l || h;
+                            any |= l || h;
                             x[e] &= (l ? 0u : 0xffffu) | (h ? 0u : 0xffff0000u);
                         }
-                        if (odd && partial < kOddTiles) {
+                        if (any) {
+                            const int row = half * 64 + 4 * i + (lane >> 3);
                             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
                             atomicOr(&sy->odd[mem][partial][row >> 5], 1u << (row & 31));
                             *(volatile int*)&sy->odd_any[mem][half] = 1;
@@ -398,62 +452,90 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
                 const uint32_t scol = tl + 128 * buf;
                 if (!warp_wait(sy, &sy->s_full[t][blocks & 3u], (blocks >> 2) & 1u)) return;
                 tc_fence_after();
-                float s[128];
-#pragma unroll
-                for (int ch = 0; ch < 4; ++ch) tmem_ld32(scol + ch * 32, s + ch * 32);
-                tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 128; ++e) asm volatile("" : "+f"(s[e]));       // (used behind the wait)
                 const int key0 = p.key0 + (u << kShift);
                 const uint32_t there = *(volatile uint32_t*)&sy->there[(c + (uint32_t)u) % kSeen];
-                if (key0 < lo_all || key0 + 127 > hi_all || there != 0xffu) {
-                    const int from = lo - key0, to = hi - key0;
+                const bool edge = key0 < lo_all || key0 + 127 > hi_all || there != 0xffu;      // keys that this row does not see
+                const int from = lo - key0, to = hi - key0;
+                float va[32], vb[32];
+                auto hide = [&](int ch, float* v) {                            // columns [32 ch, 32 ch + 32): those in [from, to], of blocks that are there
+                    const int f = min(max(from - ch * 32, 0), 32), n = min(max(to + 1 - ch * 32, 0), 32);
+                    const uint32_t below = n == 32 ? 0xffffffffu : (1u << n) - 1u, front = f == 32 ? 0xffffffffu : (1u << f) - 1u;
+                    const uint32_t two = there >> 2 * ch, w = below & ~front & ((two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u));
 #pragma unroll
-                    for (int e = 0; e < 128; ++e)
-                        if (e < from || e > to || !((there >> (e >> 4)) & 1u)) s[e] = NEG_INF;
-                }
-                // (the scale is positive)
+                    for (int e = 0; e < 32; ++e) v[e] = w & (1u << e) ? v[e] : NEG_INF;
+                };
                 float m4[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
-#pragma unroll
-                for (int e = 0; e < 128; e += 8) {
-                    m4[0] = max_3(m4[0], s[e], s[e + 1]); m4[1] = max_3(m4[1], s[e + 2], s[e + 3]);
-                    m4[2] = max_3(m4[2], s[e + 4], s[e + 5]); m4[3] = max_3(m4[3], s[e + 6], s[e + 7]);
-                }
-                const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale2;
-                float factor = 1.f;
-                if (mx > m + kLazy || (m == NEG_INF && mx != NEG_INF)) {
-                    factor = m == NEG_INF ? 0.f : ex2(m - mx);
-                    m = mx;
-                }
-                if (u > 0 && __any_sync(0xffffffffu, factor != 1.f)) {
-                    if (!warp_wait(sy, &sy->pv_done[t][(blocks - 1u) & 3u], ((blocks - 1u) >> 2) & 1u)) return;      // O is complete up to here
-                    tc_fence_after();
-                    l *= factor;
 #pragma unroll 1
-                    for (int ch = 0; ch < D / 16; ++ch) {
-                        float o[16];
-                        uint32_t x[16];
-                        tc_ld16(ocol + ch * 16, o);
+                for (int ch = 0; ch < 4; ch += 2) {
+                    tmem_ld32(scol + ch * 32, va);
+                    tmem_ld32(scol + ch * 32 + 32, vb);
+                    tmem_wait_ld();
+                    use32(va);
+                    use32(vb);
+                    if (edge) {
+                        hide(ch, va);
+                        hide(ch + 1, vb);
+                    }
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(o[e] * factor);
-                        tmem_st16(ocol + ch * 16, x);
+                    for (int e = 0; e < 32; e += 4) {
+                        m4[0] = max_3(m4[0], va[e], va[e + 1]); m4[1] = max_3(m4[1], va[e + 2], va[e + 3]);
+                        m4[2] = max_3(m4[2], vb[e], vb[e + 1]); m4[3] = max_3(m4[3], vb[e + 2], vb[e + 3]);
+                    }
+                }
+                tmem_ld32(scol, va);                                           // (under way meanwhile)
+                const float mx = max_3(m4[0], m4[1], max_3(m4[2], m4[2], m4[3])) * a.scale2;
+                // (a row that sees NaN or an infinite score has no result; said here, since what follows may lose it)
+                if (!(mx < -NEG_INF)) l = __int_as_float(0x7fffffff);
+                const bool raise = mx > m + kLazy || (m == NEG_INF && mx != NEG_INF);
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float factor = !raise ? 1.f : m == NEG_INF ? 0.f : ex2(m - mx);
+                    if (raise) m = mx;
+                    if (u > 0) {
+                        if (!warp_wait(sy, &sy->pv_done[t][(blocks - 1u) & 3u], ((blocks - 1u) >> 2) & 1u)) return;      // O is complete up to here
+                        tc_fence_after();
+                        l *= factor;
+#pragma unroll 1
+                        for (int ch = 0; ch < D / 16; ++ch) {
+                            float o[16];
+                            uint32_t x[16];
+                            tc_ld16(ocol + ch * 16, o);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(o[e] * factor);
+                            tmem_st16(ocol + ch * 16, x);
+                        }
                     }
                 }
                 const float mm = m == NEG_INF ? 0.f : m;                       // (no key so far: every score is -inf)
                 const float2 scale2 = make_float2(a.scale2, a.scale2), off2 = make_float2(-mm, -mm);
                 float2 l4[4] = {};
-#pragma unroll
-                for (int ch = 0; ch < 4; ++ch) {
+                // P of 32 columns: of each 16, the pairs of `fma` without the special function units (where every key is seen: a hidden one must be 0)
+                auto weigh = [&](int ch, float* v, auto edges) {
+                    constexpr bool EDGES = decltype(edges)::value;
+                    use32(v);
+                    if (EDGES) hide(ch, v);
                     uint32_t x[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        const float2 y = fma_2(make_float2(s[ch * 32 + e], s[ch * 32 + e + 1]), scale2, off2);
-                        const float2 q = make_float2(ex2(y.x), ex2(y.y));
+                        const float2 y = fma_2(make_float2(v[e], v[e + 1]), scale2, off2);
+                        const float2 q = !EDGES && ((kFmaPairs >> (e >> 1 & 7)) & 1) ? ex2_fma(y) : make_float2(ex2(y.x), ex2(y.y));
                         l4[(e >> 1) & 3] = add_2(l4[(e >> 1) & 3], q);
                         x[e >> 1] = pack16<DT>(q.x, q.y);
                     }
                     tmem_st16(scol + ch * 16, x);
-                }
+                };
+                auto weigh_all = [&](auto edges) {
+#pragma unroll 1
+                    for (int ch = 0; ch < 4; ch += 2) {
+                        tmem_wait_ld();
+                        tmem_ld32(scol + ch * 32 + 32, vb);
+                        weigh(ch, va, edges);
+                        tmem_wait_ld();
+                        if (ch == 0) tmem_ld32(scol + 64, va);
+                        weigh(ch + 1, vb, edges);
+                    }
+                };
+                if (edge) weigh_all(Const<true>{});
+                else weigh_all(Const<false>{});
                 l += ((l4[0].x + l4[0].y) + (l4[1].x + l4[1].y)) + ((l4[2].x + l4[2].y) + (l4[3].x + l4[3].y));
                 tmem_wait_st();
                 tc_fence_before();
@@ -475,7 +557,7 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
             float* const part = a.parts + slot_row * D;
             const uint32_t mem = items % kOddItems;
             const bool odd = (*(volatile int*)&sy->odd_any[mem][0] | *(volatile int*)&sy->odd_any[mem][1]) != 0;
-            if (mine && !whole) reinterpret_cast<float2*>(a.stats)[slot_row] = make_float2(l != l && m == NEG_INF ? 0.f : m, l);
+            if (mine && !whole) a.stats[slot_row] = make_float2(l != l && m == NEG_INF ? 0.f : m, l);
 #pragma unroll 1
             for (int ch = 0; ch < D / 16; ++ch) {
                 float o[16];
@@ -575,10 +657,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk(const __grid_co
     tc_fence_after();
     const uint32_t tmem = *(volatile uint32_t*)&sy.tmem;
     if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         softmax_role<DT, D>(a, &sy, w, tmem, worker, max(workers, 1), total);
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         if (warp == 8) load_role<D>(a, m, smem, &sy, w);
         else if (warp == 9) product_role<DT, D>(a, smem, &sy, w, tmem);
         else value_role<DT, D>(a, smem, &sy, w);

@@ -19,6 +19,12 @@ constexpr int kUnitBytes = 8192;                      // K and V of a unit
 constexpr float kRaise = 8.0f;
 constexpr int kLeastUnits = 2;                        // units that a worker has at least, where there are few
 
+struct Piece {                                        // a part that a warp has of an item (rows 0: none)
+    int rows, row0, block;
+    bool ends;                                        // it ends the item
+    int last;                                         // else, of one that begins it: the worker that does
+};
+
 template <int D> constexpr int unit_shift = D == 128 ? 4 : 5;
 
 __device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool there) {
@@ -38,7 +44,7 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
 }
 
 template <int DT, int D>
-__global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_constant__ AttnArgs a, const __grid_constant__ FewParts own) {
     constexpr int SHIFT = unit_shift<D>, U = 1 << SHIFT, NT = U / 8, KS = U / 16, DK = D / 16, DN = D / 8;
     constexpr int CH = D / 8, ROWS_PER_COPY = 32 / CH;          // 16-byte pieces of a row; rows that 32 lanes copy
     constexpr float NEG_INF = -__builtin_huge_valf();
@@ -50,7 +56,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
     Walk<SHIFT> w;
     long long total;
     const int workers = plan<SHIFT, kFewWarps * 32>(a, &scratch, worker, kLeastUnits, w, total);
-    if (lane == 0) a.joins[worker] = make_int4(0, 0, 0, 0);
+    if (threadIdx.x == 0) a.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
+    __shared__ Piece pieces[kFewWarps][2];
+    if (lane < 2) pieces[warp][lane].rows = 0;
+    __syncwarp();
     const uint32_t ring = smem_u32(smem) + warp * (kStagesFew * kUnitBytes);
     const int quad = lane >> 2, pair = (lane & 3) * 2;           // this thread's rows quad, quad + 8; columns pair, pair + 1 of each 8
     const long long end = (long long)(worker + 1) * total / max(workers, 1);
@@ -257,9 +266,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
         // ---- results, or this part's statistics and products
         const bool whole = u0 == 0 && count == it.units;
         const int slot = worker * 2 + (u0 == 0 ? 1 : 0);
-        if (!whole && u0 == 0 && lane == 0) {
-            const long long item_end = end + (it.units - count);               // (the item is not finished: the worker's last)
-            a.joins[worker] = make_int4(worker_before(item_end, total, workers) - worker + 1, base_row, rows, kv);
+        if (!whole && lane == 0) {
+            // (an item that is begun and not finished is the worker's last)
+            const bool ends = u0 + count == it.units;
+            const int last = ends || u0 > 0 ? 0 : worker_before(end + (it.units - count), total, workers);
+            pieces[warp][u0 == 0 ? 1 : 0] = Piece{rows, base_row, kv, ends, last};
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -271,19 +282,43 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
 #pragma unroll
                 for (int n = 0; n < DN; ++n) *reinterpret_cast<uint32_t*>(to + n * 8) = pack16<DT>(o[n][2 * i] * inv, o[n][2 * i + 1] * inv);
             } else {
-                const long long at = (long long)slot * a.part_rows + row;
+                const long long at = (long long)slot * kFewRows + row;
                 // (no score but NaN, which no maximum shows: a finite one, so that the part counts)
-                if ((lane & 3) == 0) reinterpret_cast<float2*>(a.stats)[at] = make_float2(l[i] != l[i] && m[i] == NEG_INF ? 0.f : m[i], l[i]);
+                if ((lane & 3) == 0) own.stats[at] = make_float2(l[i] != l[i] && m[i] == NEG_INF ? 0.f : m[i], l[i]);
 #pragma unroll
-                for (int n = 0; n < DN; ++n) *reinterpret_cast<float2*>(a.parts + at * D + n * 8 + pair) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+                for (int n = 0; n < DN; ++n) *reinterpret_cast<float2*>(own.parts + at * D + n * 8 + pair) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
             }
         }
         w.next(a, count);
     }
+    // ---- the warps' parts of an item: results where the block has all of them, else a part of the block
+    __shared__ Join<D, kFewRows, kFewWarps * 32> join;
+    __syncthreads();
+    for (int at = 0; at < 2 * kFewWarps; ++at) {
+        const int from = at >> 1, slot0 = at & 1;                 // a run of parts: this one and slot 0 of the warps behind, up to one that ends the item
+        const Piece head = pieces[from][slot0];
+        if (head.rows == 0 || (slot0 == 0 && from > 0)) continue;              // (slot 0 of a later warp continues a run)
+        int count = 1;
+        bool ends = head.ends;
+        while (!ends && from + count < kFewWarps && pieces[from + count][0].rows > 0) ends = pieces[from + count++][0].ends;
+        const int w0 = blockIdx.x * kFewWarps + from;
+        const long long to = blockIdx.x * 2 + slot0;
+        if (slot0 && !ends && threadIdx.x == 0)
+            a.joins[blockIdx.x] = make_int4(head.last / kFewWarps - (int)blockIdx.x + 1, head.row0, head.rows, head.block);
+        join.run(a, own.stats, own.parts, count, 0, head.rows, [&](int i) { return (long long)(i == 0 ? 2 * w0 + slot0 : 2 * (w0 + i)); },
+                 [&](int row, int col, float m, float l, const float4& o) {
+                     if (slot0 && ends) {
+                         write_result<DT, D>(a, head.row0, head.block, row, col, l, o);
+                     } else {
+                         if (col == 0) a.stats[to * kFewRows + row] = make_float2(m, l);
+                         *reinterpret_cast<float4*>(a.parts + (to * kFewRows + row) * D + col) = o;
+                     }
+                 });
+    }
 }
 
 template <int DT, int D>
-cudaError_t launch(const AttnArgs& a, int blocks, cudaStream_t stream) {
+cudaError_t launch(const AttnArgs& a, const FewParts& own, int blocks, cudaStream_t stream) {
     constexpr int bytes = kFewWarps * kStagesFew * kUnitBytes;
     const cudaError_t e = cudaFuncSetAttribute(attend_few<DT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
@@ -297,14 +332,14 @@ cudaError_t launch(const AttnArgs& a, int blocks, cudaStream_t stream) {
     cfg.stream = stream;
     cfg.attrs = &pdl;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attend_few<DT, D>, a);
+    return cudaLaunchKernelEx(&cfg, attend_few<DT, D>, a, own);
 }
 
 }  // namespace
 
-cudaError_t launch_few(const AttnArgs& a, int head_dim, int dtype, int blocks, cudaStream_t stream) {
-    if (dtype == DT_F16) return head_dim == 64 ? launch<DT_F16, 64>(a, blocks, stream) : launch<DT_F16, 128>(a, blocks, stream);
-    return head_dim == 64 ? launch<DT_BF16, 64>(a, blocks, stream) : launch<DT_BF16, 128>(a, blocks, stream);
+cudaError_t launch_few(const AttnArgs& a, const FewParts& own, int head_dim, int dtype, int blocks, cudaStream_t stream) {
+    if (dtype == DT_F16) return head_dim == 64 ? launch<DT_F16, 64>(a, own, blocks, stream) : launch<DT_F16, 128>(a, own, blocks, stream);
+    return head_dim == 64 ? launch<DT_BF16, 64>(a, own, blocks, stream) : launch<DT_BF16, 128>(a, own, blocks, stream);
 }
 
 }  // namespace mk
