@@ -53,21 +53,20 @@ int heads_of_block(int group, int rows) {
 // Which kernel takes a call: the one for few rows where an item of 16 rows holds all new tokens of a sequence (then every key is read once).
 bool few_rows(int group, long long max_new) { return max_new * group <= kFewRows; }
 
-// what the workspace holds, one behind the other: joins, stats and parts of the blocks, stats and parts of the warps (few rows)
+// what the workspace holds, one behind the other: joins, stats and parts of the blocks, parts of the warps (few rows)
 struct Layout {
     int workers, part_rows;
-    size_t stats, parts, own_stats, own_parts, bytes;
+    size_t stats, parts, own, bytes;
 };
 Layout layout_of(int sms, int head_dim, bool few) {
     Layout l;
     l.workers = few ? sms * kFewWarps : sms;
     l.part_rows = few ? kFewRows : 2 * kChunkTile;
-    const size_t rows = (size_t)sms * 2 * l.part_rows, own_rows = few ? (size_t)l.workers * 2 * kFewRows : 0;
+    const size_t rows = (size_t)sms * 2 * l.part_rows;
     l.stats = (size_t)sms * sizeof(int4);
     l.parts = l.stats + rows * sizeof(float2);
-    l.own_stats = l.parts + rows * head_dim * sizeof(float);
-    l.own_parts = l.own_stats + own_rows * sizeof(float2);
-    l.bytes = l.own_parts + own_rows * head_dim * sizeof(float);
+    l.own = l.parts + rows * head_dim * sizeof(float);
+    l.bytes = l.own + (few ? (size_t)l.workers * kFewRows * head_dim * sizeof(float) : 0);
     return l;
 }
 
@@ -132,6 +131,7 @@ extern "C" int mk_paged_attention(int device, const mk_batch* batch, const mk_pa
     a.ld_v = cache->ld_v;
     a.ld_out = ld_out;
     a.group = heads_of_block(group, few ? kFewRows : kChunkTile);
+    a.group_inverse = 65536 / a.group + 1;
     a.shared = group / a.group;
     a.blocks = heads / a.group;
     a.window = window;
@@ -143,7 +143,7 @@ extern "C" int mk_paged_attention(int device, const mk_batch* batch, const mk_pa
     a.parts = (float*)((uint8_t*)workspace + lay.parts);
     cudaStream_t st = (cudaStream_t)stream;
     a.tokens = few ? kFewRows / a.group : kChunkTile / a.group * 2;
-    const FewParts own = {(float2*)((uint8_t*)workspace + lay.own_stats), (float*)((uint8_t*)workspace + lay.own_parts)};
+    float* const own = (float*)((uint8_t*)workspace + lay.own);
     cudaError_t e = few ? launch_few(a, own, D, cache->dtype, sms, st) : launch_chunk(a, cache, heads, st);
     if (e == cudaSuccess) {
         // (few rows of many parts or many rows of few)

@@ -2,7 +2,8 @@
 //
 // An item is up to `tokens` consecutive new tokens of one sequence and `group` query heads of one kv head: rows token * group + head of one
 // operand tile.  (Where more heads share a kv head than the tile has rows, `shared` such blocks of heads read it.)  Its keys are cut into units of 2^shift keys, aligned in the sequence.  All units of all items -- in the order
-// sequence, block of heads, tokens -- make one list, which is dealt out evenly: worker w has units [w N / W, (w + 1) N / W).  Lengths are known on
+// sequence, block of heads, tokens -- make one list, which is dealt out evenly: each worker has the next N / W of them, the first N % W one
+// more.  Lengths are known on
 // the device only, so every block works out its part itself, and batches of the most unlike lengths load all SMs alike.
 // A worker that has an item's units from the first to the last writes results.  Else it leaves the running maximum, the sum and the products of its
 // part in the workspace (slot 0: a part that does not begin the item; slot 1: one that begins it); a block joins the parts that its
@@ -21,9 +22,11 @@ struct AttnArgs {
     uint16_t* out;
     long long ld_q, ld_k, ld_v, ld_out;
     int blocks, shared, group, window;                // blocks of `group` heads; blocks that share a kv head
+    int group_inverse;                                // 65536 / group + 1: row * group_inverse >> 16 is row / group for rows below 256
     float scale2;                                     // scale * log2(e)
     int tokens;                                       // new tokens of an item
     int workers, part_rows;                           // ... and rows of a part in the workspace
+    __device__ __forceinline__ int token_of(int row) const { return row * group_inverse >> 16; }
     int4* joins;                                      // of each block: parts of the item that it begins and does not end (0: none), its first
                                                       // row, its rows, its block of heads
     float2* stats;                                    // [block][2][part_rows]: maximum (log2 domain) and sum
@@ -33,6 +36,27 @@ struct AttnArgs {
 struct Item {
     int lo, hi;                                       // keys some token sees (lo > hi: none)
     int first, units;                                 // units; at least one
+};
+
+// (the 64-bit division takes a few hundred cycles, and numbers above 2^32 are rare)
+__device__ __forceinline__ long long divide(long long a, long long b) {
+    return (unsigned long long)(a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
+// Shares of the list of units.
+struct Shares {
+    long long total, per;
+    int workers, longer;                              // `longer` workers have per + 1 units, the others per
+    __device__ __forceinline__ Shares(long long units, int most, int least) {
+        total = units;
+        workers = (int)min((long long)most, divide(total + least - 1, least));
+        per = workers ? divide(total, workers) : 0;
+        longer = (int)(total - per * workers);
+    }
+    __device__ __forceinline__ long long begin(int w) const { return w * per + min(w, longer); }
+    __device__ __forceinline__ int worker_of(long long unit) const {
+        const long long border = (per + 1) * longer;
+        return (int)(unit < border ? divide(unit, per + 1) : longer + divide(unit - border, per));
+    }
 };
 
 template <int SHIFT>
@@ -78,7 +102,7 @@ struct Walk {
     // to unit `at` of the sequence's list (of `per` units a block of heads)
     __device__ __forceinline__ void start(const AttnArgs& a, int seq, long long at, long long per) {
         sequence(a, seq);
-        kv = (int)(at / per);
+        kv = (int)divide(at, per);
         at -= kv * per;
         t = 0;
         enter(a);
@@ -108,21 +132,16 @@ struct Walk {
     }
 };
 
-// The worker that has the unit in front of `end`.
-__device__ __forceinline__ int worker_before(long long end, long long total, int workers) {
-    return (int)((end * workers + total - 1) / total) - 1;
-}
-
 template <int THREADS>
 struct PlanScratch {
     long long sums[THREADS / 32];
     long long ends[THREADS];                          // inclusive sums of a round's sequences
 };
 
-// Every thread of the block calls it with its warp's worker.  Returns the number of workers among which the units are dealt out, at least `least`
-// to each, and their total; `walk` is set where the warp's worker has some (walk.left > 0).
+// Every thread of the block calls it with its warp's worker.  Returns how the units are dealt out, at least `least` to a worker; `walk` is set
+// where the warp's worker has some (walk.left > 0).
 template <int SHIFT, int THREADS>
-__device__ __forceinline__ int plan(const AttnArgs& a, PlanScratch<THREADS>* sc, int worker, int least, Walk<SHIFT>& walk, long long& total) {
+__device__ __forceinline__ Shares plan(const AttnArgs& a, PlanScratch<THREADS>* sc, int worker, int least, Walk<SHIFT>& walk) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int rounds = (a.batch.seqs + THREADS - 1) / THREADS;
     long long mine = 0, sum = 0;
@@ -134,11 +153,11 @@ __device__ __forceinline__ int plan(const AttnArgs& a, PlanScratch<THREADS>* sc,
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     if (lane == 0) sc->sums[warp] = sum;
     __syncthreads();
-    total = 0;
+    long long total = 0;
     for (int w = 0; w < THREADS / 32; ++w) total += sc->sums[w];
-    const int workers = (int)min((long long)a.workers, (total + least - 1) / least);
-    const long long begin = worker < workers ? worker * total / workers : total;
-    walk.left = worker < workers ? (worker + 1) * total / workers - begin : 0;
+    const Shares shares(total, a.workers, least);
+    const long long begin = worker < shares.workers ? shares.begin(worker) : total;
+    walk.left = worker < shares.workers ? shares.begin(worker + 1) - begin : 0;
     long long base = 0;
     for (int r = 0; r < rounds; ++r) {
         if (rounds > 1) {
@@ -165,11 +184,11 @@ __device__ __forceinline__ int plan(const AttnArgs& a, PlanScratch<THREADS>* sc,
             for (int i = lane; i < THREADS; i += 32) at += sc->ends[i] <= begin;
             for (int d = 16; d; d >>= 1) at += __shfl_xor_sync(0xffffffffu, at, d);
             const long long first = at > 0 ? sc->ends[at - 1] : base;
-            walk.start(a, r * THREADS + at, begin - first, (sc->ends[at] - first) / a.blocks);
+            walk.start(a, r * THREADS + at, begin - first, divide(sc->ends[at] - first, a.blocks));
         }
         base += all;
     }
-    return workers;
+    return shares;
 }
 
 // Joins `count` parts of rows [row_begin, row_end) of an item, ROWS of them: part i has `slot(i)`.  With M the largest of their maxima m_i
@@ -229,7 +248,7 @@ struct Join {
 template <int DT, int D>
 __device__ __forceinline__ void write_result(const AttnArgs& a, int row0, int block, int row, int col, float l, const float4& o) {
     const float inv = l == 0.f ? 0.f : 1.f / l;       // (no key: zeros)
-    const int tok = row / a.group;
+    const int tok = a.token_of(row);
     uint16_t* to = a.out + (long long)(row0 + tok) * a.ld_out + (block * a.group + row - tok * a.group) * D + col;
     *reinterpret_cast<uint2*>(to) = make_uint2(pack16<DT>(o.x * inv, o.y * inv), pack16<DT>(o.z * inv, o.w * inv));
 }
@@ -237,11 +256,7 @@ __device__ __forceinline__ void write_result(const AttnArgs& a, int row0, int bl
 // items of few rows (paged_attention_few.cu): rows of an item, workers of a block
 constexpr int kFewRows = 16;
 constexpr int kFewWarps = 8;
-struct FewParts {                                     // parts of the warps: [worker][2][kFewRows] and [worker][2][kFewRows][head_dim]
-    float2* stats;
-    float* parts;
-};
-cudaError_t launch_few(const AttnArgs& a, const FewParts& own, int head_dim, int dtype, int blocks, cudaStream_t stream);
+cudaError_t launch_few(const AttnArgs& a, float* own /* [worker][kFewRows][head_dim] */, int head_dim, int dtype, int blocks, cudaStream_t stream);
 
 // items of up to 256 rows, a positive scale (paged_attention_chunk.cu): two tiles of 128 rows, a worker per block
 constexpr int kChunkTile = 128;

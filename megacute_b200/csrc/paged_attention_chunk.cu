@@ -430,13 +430,13 @@ __device__ __forceinline__ void value_role(const AttnArgs& a, uint8_t* smem, Syn
 
 // ---- softmax ------------------------------------------------------------------------------------------------------------------
 template <int DT, int D>
-__device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<kShift> w, uint32_t tmem, int worker, int workers, long long total) {
+__device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<kShift> w, uint32_t tmem, int worker, const Shares& shares) {
     using M = Map<D>;
     constexpr float NEG_INF = -__builtin_huge_valf();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = warp >> 2, i = threadIdx.x & 127;     // tile and its row
-    const int tile_tokens = a.tokens / 2, my_token = i / a.group, my_head = i - my_token * a.group;
+    const int tile_tokens = a.tokens / 2, my_token = a.token_of(i), my_head = i - my_token * a.group;
     const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), ocol = tl + M::kO + D * t;
-    const long long end = (long long)(worker + 1) * total / workers;
+    const long long end = shares.begin(worker + 1);
     uint32_t c = 0, items = 0, seq0 = 0, blocks = 0;
     for (; w.left > 0; ++items) {
         const Part p = part_of(a, w);
@@ -551,7 +551,7 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
             const float inv = l == 0.f ? 0.f : 1.f / l;
             if (p.begins && !p.ends && i == 0 && t == 0) {
                 const long long item_end = end + (w.item.units - p.units);     // (the item is not finished: the worker's last)
-                a.joins[worker] = make_int4(worker_before(item_end, total, workers) - worker + 1, p.row0, p.tokens * a.group, p.block);
+                a.joins[worker] = make_int4(shares.worker_of(item_end - 1) - worker + 1, p.row0, p.tokens * a.group, p.block);
             }
             uint16_t* const to = a.out + (long long)(p.row0 + token) * a.ld_out + (p.block * a.group + my_head) * D;
             float* const part = a.parts + slot_row * D;
@@ -648,8 +648,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk(const __grid_co
     wait_for_previous_kernel();
     let_next_kernel_launch();
     Walk<kShift> w;
-    long long total;
-    const int workers = plan<kShift, kChunkThreads>(a, reinterpret_cast<PlanScratch<kChunkThreads>*>(smem), worker, 1, w, total);
+    const Shares shares = plan<kShift, kChunkThreads>(a, reinterpret_cast<PlanScratch<kChunkThreads>*>(smem), worker, 1, w);
     if (threadIdx.x == 0) a.joins[worker] = make_int4(0, 0, 0, 0);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");              // (copies go where the plan's sums were)
     tc_fence_before();
@@ -657,7 +656,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk(const __grid_co
     tc_fence_after();
     const uint32_t tmem = *(volatile uint32_t*)&sy.tmem;
     if (warp < 8) {
-        softmax_role<DT, D>(a, &sy, w, tmem, worker, max(workers, 1), total);
+        softmax_role<DT, D>(a, &sy, w, tmem, worker, shares);
     } else {
         if (warp == 8) load_role<D>(a, m, smem, &sy, w);
         else if (warp == 9) product_role<DT, D>(a, smem, &sy, w, tmem);

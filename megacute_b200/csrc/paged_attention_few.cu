@@ -21,8 +21,9 @@ constexpr int kLeastUnits = 2;                        // units that a worker has
 
 struct Piece {                                        // a part that a warp has of an item (rows 0: none)
     int rows, row0, block;
+    int last;                                         // of one that begins the item and does not end it: the worker that does
     bool ends;                                        // it ends the item
-    int last;                                         // else, of one that begins it: the worker that does
+    bool far;                                         // its products are in the workspace, not in the warp's ring
 };
 
 template <int D> constexpr int unit_shift = D == 128 ? 4 : 5;
@@ -44,7 +45,7 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
 }
 
 template <int DT, int D>
-__global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_constant__ AttnArgs a, const __grid_constant__ FewParts own) {
+__global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_constant__ AttnArgs a, float* own) {
     constexpr int SHIFT = unit_shift<D>, U = 1 << SHIFT, NT = U / 8, KS = U / 16, DK = D / 16, DN = D / 8;
     constexpr int CH = D / 8, ROWS_PER_COPY = 32 / CH;          // 16-byte pieces of a row; rows that 32 lanes copy
     constexpr float NEG_INF = -__builtin_huge_valf();
@@ -54,15 +55,15 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
     let_next_kernel_launch();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, worker = blockIdx.x * kFewWarps + warp;
     Walk<SHIFT> w;
-    long long total;
-    const int workers = plan<SHIFT, kFewWarps * 32>(a, &scratch, worker, kLeastUnits, w, total);
+    const Shares shares = plan<SHIFT, kFewWarps * 32>(a, &scratch, worker, kLeastUnits, w);
     if (threadIdx.x == 0) a.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
     __shared__ Piece pieces[kFewWarps][2];
+    __shared__ float2 stats[kFewWarps][2][kFewRows];
     if (lane < 2) pieces[warp][lane].rows = 0;
+    float* const near = reinterpret_cast<float*>(smem + warp * (kStagesFew * kUnitBytes));
     __syncwarp();
     const uint32_t ring = smem_u32(smem) + warp * (kStagesFew * kUnitBytes);
     const int quad = lane >> 2, pair = (lane & 3) * 2;           // this thread's rows quad, quad + 8; columns pair, pair + 1 of each 8
-    const long long end = (long long)(worker + 1) * total / max(workers, 1);
 
     while (w.left > 0) {
         const int tokens = w.item_tokens(a), rows = tokens * a.group, u0 = w.unit;
@@ -70,25 +71,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
         const Item it = w.item;
         const long long p0 = w.p + w.t;
         const int first_key = (it.first + u0) << SHIFT;
-        // ---- Q fragments
-        uint32_t q[DK][4];
-        long long row_at[2];                                     // element offset of this thread's two rows, -1: none
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int row = quad + 8 * i, tok = row / a.group;
-            row_at[i] = row < rows ? (long long)(base_row + tok) : -1;
-            const uint16_t* src = a.q + row_at[i] * a.ld_q + (kv * a.group + row - tok * a.group) * D + pair;
-#pragma unroll
-            for (int k = 0; k < DK; ++k) {
-                q[k][i] = row < rows ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16)) : 0u;
-                q[k][i + 2] = row < rows ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16 + 8)) : 0u;
-            }
-        }
         // keys that this thread's rows see
         int lo_r[2], hi_r[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const long long p = p0 + (quad + 8 * i) / a.group;
+            const long long p = p0 + a.token_of(quad + 8 * i);
             hi_r[i] = (int)min(max(p, -1ll), (long long)it.hi);
             lo_r[i] = a.window > 0 ? (int)min(max(p + 1 - a.window, 0ll), 0x7fffffffll) : 0;
         }
@@ -107,6 +94,20 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
             }
         };
         hold(block0);
+        // ---- Q fragments
+        uint32_t q[DK][4];
+        long long row_at[2];                                     // element offset of this thread's two rows, -1: none
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = quad + 8 * i, tok = a.token_of(row);
+            row_at[i] = row < rows ? (long long)(base_row + tok) : -1;
+            const uint16_t* src = a.q + row_at[i] * a.ld_q + (kv * a.group + row - tok * a.group) * D + pair;
+#pragma unroll
+            for (int k = 0; k < DK; ++k) {
+                q[k][i] = row < rows ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16)) : 0u;
+                q[k][i + 2] = row < rows ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16 + 8)) : 0u;
+            }
+        }
         uint32_t absent = 0;                                     // two bits of unit u from bit 2 (u % 16): blocks that are not there
         const uint16_t* kp = a.k + kv / a.shared * D + (lane % CH) * 8;
         const uint16_t* vp = a.v + kv / a.shared * D + (lane % CH) * 8;
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
                         const long long at = p0 + t;
                         const int hi = (int)min(max(at, -1ll), (long long)it.hi);
                         const int lo = a.window > 0 ? (int)min(max(at + 1 - a.window, 0ll), 0x7fffffffll) : 0;
-                        const bool r0 = quad / a.group == t, r1 = (quad + 8) / a.group == t;
+                        const bool r0 = a.token_of(quad) == t, r1 = a.token_of(quad + 8) == t;
                         uint32_t bt[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
@@ -265,12 +266,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
         }
         // ---- results, or this part's statistics and products
         const bool whole = u0 == 0 && count == it.units;
-        const int slot = worker * 2 + (u0 == 0 ? 1 : 0);
+        // (the worker's last part has the ring to itself; one in front of others, of which there is one at most, goes to the workspace)
+        const bool far = w.left > count;
         if (!whole && lane == 0) {
             // (an item that is begun and not finished is the worker's last)
             const bool ends = u0 + count == it.units;
-            const int last = ends || u0 > 0 ? 0 : worker_before(end + (it.units - count), total, workers);
-            pieces[warp][u0 == 0 ? 1 : 0] = Piece{rows, base_row, kv, ends, last};
+            const int last = ends || u0 > 0 ? 0 : shares.worker_of(shares.begin(worker + 1) + (it.units - count) - 1);
+            pieces[warp][u0 == 0 ? 1 : 0] = Piece{rows, base_row, kv, last, ends, far};
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -278,47 +280,69 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
             if (row >= rows) continue;
             if (whole) {
                 const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
-                uint16_t* to = a.out + row_at[i] * a.ld_out + (kv * a.group + row % a.group) * D + pair;
+                uint16_t* to = a.out + row_at[i] * a.ld_out + (kv * a.group + row - a.token_of(row) * a.group) * D + pair;
 #pragma unroll
                 for (int n = 0; n < DN; ++n) *reinterpret_cast<uint32_t*>(to + n * 8) = pack16<DT>(o[n][2 * i] * inv, o[n][2 * i + 1] * inv);
             } else {
-                const long long at = (long long)slot * kFewRows + row;
                 // (no score but NaN, which no maximum shows: a finite one, so that the part counts)
-                if ((lane & 3) == 0) own.stats[at] = make_float2(l[i] != l[i] && m[i] == NEG_INF ? 0.f : m[i], l[i]);
+                if ((lane & 3) == 0) stats[warp][u0 == 0 ? 1 : 0][row] = make_float2(l[i] != l[i] && m[i] == NEG_INF ? 0.f : m[i], l[i]);
+                float* const to = (far ? own + (long long)worker * kFewRows * D : near) + row * D + pair;
 #pragma unroll
-                for (int n = 0; n < DN; ++n) *reinterpret_cast<float2*>(own.parts + at * D + n * 8 + pair) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+                for (int n = 0; n < DN; ++n) *reinterpret_cast<float2*>(to + n * 8) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
             }
         }
         w.next(a, count);
     }
-    // ---- the warps' parts of an item: results where the block has all of them, else a part of the block
-    __shared__ Join<D, kFewRows, kFewWarps * 32> join;
+    // ---- the warps' parts of an item: results where the block has all of them, else a part of the block.
+    // A run of parts is one, and slot 0 of the warps behind up to one that ends the item.  Its rows are dealt out to the warps, a quarter or half
+    // a row's columns to a thread: l = sum_i 2^(m_i - M) l_i and the like for o, in the order of the warps.
     __syncthreads();
-    for (int at = 0; at < 2 * kFewWarps; ++at) {
-        const int from = at >> 1, slot0 = at & 1;                 // a run of parts: this one and slot 0 of the warps behind, up to one that ends the item
-        const Piece head = pieces[from][slot0];
-        if (head.rows == 0 || (slot0 == 0 && from > 0)) continue;              // (slot 0 of a later warp continues a run)
-        int count = 1;
-        bool ends = head.ends;
+    const int from = (lane >> 1) & (kFewWarps - 1), slot = lane & 1;
+    int count = 0;
+    bool ends = false;
+    if (lane < 2 * kFewWarps && pieces[from][slot].rows > 0 && (slot || from == 0)) {      // (slot 0 of a later warp continues a run)
+        count = 1;
+        ends = pieces[from][slot].ends;
         while (!ends && from + count < kFewWarps && pieces[from + count][0].rows > 0) ends = pieces[from + count++][0].ends;
-        const int w0 = blockIdx.x * kFewWarps + from;
-        const long long to = blockIdx.x * 2 + slot0;
-        if (slot0 && !ends && threadIdx.x == 0)
+    }
+    constexpr int LANES = D / 4, ROWS = 32 / LANES;               // threads of a row; rows of a warp at a time
+    int turn = 0;
+    for (uint32_t runs = __ballot_sync(0xffffffffu, count > 0); runs; runs &= runs - 1) {
+        const int at = __ffs(runs) - 1, n = __shfl_sync(0xffffffffu, count, at), first = at >> 1, begins = at & 1;
+        const bool done = __shfl_sync(0xffffffffu, ends, at) && begins;
+        const Piece head = pieces[first][begins];
+        const long long to = blockIdx.x * 2 + begins;
+        if (begins && !done && threadIdx.x == 0)
             a.joins[blockIdx.x] = make_int4(head.last / kFewWarps - (int)blockIdx.x + 1, head.row0, head.rows, head.block);
-        join.run(a, own.stats, own.parts, count, 0, head.rows, [&](int i) { return (long long)(i == 0 ? 2 * w0 + slot0 : 2 * (w0 + i)); },
-                 [&](int row, int col, float m, float l, const float4& o) {
-                     if (slot0 && ends) {
-                         write_result<DT, D>(a, head.row0, head.block, row, col, l, o);
-                     } else {
-                         if (col == 0) a.stats[to * kFewRows + row] = make_float2(m, l);
-                         *reinterpret_cast<float4*>(a.parts + (to * kFewRows + row) * D + col) = o;
-                     }
-                 });
+        for (int r = 0; r < head.rows; r += ROWS, ++turn) {
+            const int row = r + lane / LANES, col = lane % LANES * 4;
+            if ((turn & (kFewWarps - 1)) != warp || row >= head.rows) continue;
+            float m = NEG_INF, l = 0.f;
+            for (int i = 0; i < n; ++i) m = fmaxf(m, stats[first + i][i ? 0 : begins][row].x);
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < n; ++i) {
+                const int k = first + i, sl = i ? 0 : begins;
+                const float2 st = stats[k][sl][row];
+                if (st.x == NEG_INF) continue;                   // (it saw no key)
+                const float f = st.x == m ? 1.f : ex2(st.x - m);
+                const float* const src = pieces[k][sl].far ? own + (long long)(blockIdx.x * kFewWarps + k) * kFewRows * D
+                                                           : reinterpret_cast<const float*>(smem + k * (kStagesFew * kUnitBytes));
+                const float4 v = *reinterpret_cast<const float4*>(src + row * D + col);
+                l += f * st.y;
+                o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
+            }
+            if (done) {
+                write_result<DT, D>(a, head.row0, head.block, row, col, l, o);
+            } else {
+                if (col == 0) a.stats[to * kFewRows + row] = make_float2(m, l);
+                *reinterpret_cast<float4*>(a.parts + (to * kFewRows + row) * D + col) = o;
+            }
+        }
     }
 }
 
 template <int DT, int D>
-cudaError_t launch(const AttnArgs& a, const FewParts& own, int blocks, cudaStream_t stream) {
+cudaError_t launch(const AttnArgs& a, float* own, int blocks, cudaStream_t stream) {
     constexpr int bytes = kFewWarps * kStagesFew * kUnitBytes;
     const cudaError_t e = cudaFuncSetAttribute(attend_few<DT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
@@ -337,7 +361,7 @@ cudaError_t launch(const AttnArgs& a, const FewParts& own, int blocks, cudaStrea
 
 }  // namespace
 
-cudaError_t launch_few(const AttnArgs& a, const FewParts& own, int head_dim, int dtype, int blocks, cudaStream_t stream) {
+cudaError_t launch_few(const AttnArgs& a, float* own, int head_dim, int dtype, int blocks, cudaStream_t stream) {
     if (dtype == DT_F16) return head_dim == 64 ? launch<DT_F16, 64>(a, own, blocks, stream) : launch<DT_F16, 128>(a, own, blocks, stream);
     return head_dim == 64 ? launch<DT_BF16, 64>(a, own, blocks, stream) : launch<DT_BF16, 128>(a, own, blocks, stream);
 }
