@@ -99,7 +99,7 @@ SYMBOLS = {
     "mk_rotary": (ctypes.c_int, [ctypes.c_int, _BATCH, _ROTATION, _P, ctypes.c_int64, _P, ctypes.c_int64, ctypes.c_int, ctypes.c_int,
                                  ctypes.c_int, _P]),
     "mk_paged_append": (ctypes.c_int, [ctypes.c_int, _BATCH, _ROTATION, _CACHE, _P, ctypes.c_int64, _P, ctypes.c_int64, ctypes.c_int, _P]),
-    "mk_paged_attention_workspace": (ctypes.c_longlong, [ctypes.c_int, ctypes.c_int, _CACHE, ctypes.c_int]),
+    "mk_paged_attention_workspace": (ctypes.c_longlong, [ctypes.c_int] * 5),
     "mk_paged_attention": (ctypes.c_int, [ctypes.c_int, _BATCH, _CACHE, _P, ctypes.c_int64, _P, ctypes.c_int64, ctypes.c_int, ctypes.c_float,
                                           ctypes.c_int, ctypes.c_int, _P, ctypes.c_size_t, _P]),
     "mk_paged_attention_status": (ctypes.c_int, [ctypes.c_int, _P]),

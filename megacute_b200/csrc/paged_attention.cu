@@ -21,11 +21,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_parts(const __grid_constant
              [&](int row, int col, float, float l, const float4& o) { write_result<DT, D>(a, j.y, j.w, row, col, l, o); });
 }
 
-const char* shape_error(const mk_paged_cache* cache, int heads) {
-    const char* why = cache_error(cache);
-    if (!why && cache->head_dim != 64 && cache->head_dim != 128) why = "paged attention: head_dim is 64 or 128";
-    if (!why && (heads <= 0 || heads % cache->kv_heads)) why = "paged attention: heads is a multiple of kv_heads";
-    return why;
+const char* shape_error(int heads, int kv_heads, int head_dim) {
+    if (head_dim != 64 && head_dim != 128) return "paged attention: head_dim is 64 or 128";
+    if (heads <= 0 || kv_heads <= 0 || heads % kv_heads) return "paged attention: heads is a multiple of kv_heads";
+    return nullptr;
 }
 
 int sm_count(int device) {
@@ -89,21 +88,22 @@ cudaError_t launch_join(const AttnArgs& a, int blocks, cudaStream_t stream) {
 
 using namespace mk;
 
-extern "C" long long mk_paged_attention_workspace(int device, int heads, const mk_paged_cache* cache, int max_new) {
-    const char* why = shape_error(cache, heads);
+extern "C" long long mk_paged_attention_workspace(int device, int heads, int kv_heads, int head_dim, int max_new) {
+    const char* why = shape_error(heads, kv_heads, head_dim);
     if (why) return report(MK_E_ARG, why);
     const int sms = sm_count(device);
     if (!sms) return report(MK_E_CUDA, "no such device");
-    const size_t few = layout_of(sms, cache->head_dim, true).bytes, chunk = layout_of(sms, cache->head_dim, false).bytes;
+    const size_t few = layout_of(sms, head_dim, true).bytes, chunk = layout_of(sms, head_dim, false).bytes;
     // (a scale that is not positive is for the kernel for few rows, whatever max_new)
-    return (long long)(few_rows(heads / cache->kv_heads, max_new) || few > chunk ? few : chunk);
+    return (long long)(few_rows(heads / kv_heads, max_new) || few > chunk ? few : chunk);
 }
 
 extern "C" int mk_paged_attention(int device, const mk_batch* batch, const mk_paged_cache* cache, const void* q, int64_t ld_q, void* out,
                                   int64_t ld_out, int heads, float scale, int window, int max_new, void* workspace, size_t workspace_bytes,
                                   void* stream) {
     const char* why = batch_error(batch);
-    if (!why) why = shape_error(cache, heads);
+    if (!why) why = cache_error(cache);
+    if (!why) why = shape_error(heads, cache->kv_heads, cache->head_dim);
     if (!why && window < 0) why = "paged attention: window is a number of rows (0: the whole context)";
     if (why) return report(MK_E_ARG, why);
     if (batch->rows == 0 || batch->seqs == 0) return MK_OK;

@@ -9,6 +9,8 @@
 // part in the workspace (slot 0: a part that does not begin the item; slot 1: one that begins it); a block joins the parts that its
 // own workers have of an item, and a second kernel (paged_attention.cu) those of several blocks, always in the same order.
 #pragma once
+#include <atomic>
+
 #include "paged.cuh"
 
 namespace mk {
@@ -262,6 +264,20 @@ cudaError_t launch_few(const AttnArgs& a, float* own /* [worker][kFewRows][head_
 constexpr int kChunkTile = 128;
 cudaError_t launch_chunk(const AttnArgs& a, const mk_paged_cache* cache, int heads, cudaStream_t stream);
 cudaError_t chunk_status(int* failed, cudaStream_t stream);
+
+// A kernel's shared memory beyond 48 KB, asked for once per device.
+struct SharedMemory {
+    std::atomic<unsigned long long> devices{0};
+    cudaError_t allow(const void* kernel, int bytes) {
+        int device = 0;
+        cudaError_t e = cudaGetDevice(&device);
+        const unsigned long long bit = 1ull << (device & 63);
+        if (e != cudaSuccess || (device < 64 && (devices.load(std::memory_order_relaxed) & bit))) return e;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess && device < 64) devices.fetch_or(bit, std::memory_order_relaxed);
+        return e;
+    }
+};
 
 __device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_kernel_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

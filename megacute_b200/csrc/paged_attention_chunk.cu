@@ -696,7 +696,8 @@ template <int DT, int D>
 cudaError_t launch(const AttnArgs& a, const Maps& m, cudaStream_t stream) {
     constexpr int bytes = Map<D>::kBytes + sizeof(Sync);
     static_assert(bytes <= 232448, "shared memory of a block");
-    const cudaError_t e = cudaFuncSetAttribute(attend_chunk<DT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    static SharedMemory allowed;
+    const cudaError_t e = allowed.allow((const void*)attend_chunk<DT, D>, bytes);
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute pdl;
     pdl.id = cudaLaunchAttributeProgrammaticStreamSerialization;

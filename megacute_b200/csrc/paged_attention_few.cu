@@ -344,7 +344,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
 template <int DT, int D>
 cudaError_t launch(const AttnArgs& a, float* own, int blocks, cudaStream_t stream) {
     constexpr int bytes = kFewWarps * kStagesFew * kUnitBytes;
-    const cudaError_t e = cudaFuncSetAttribute(attend_few<DT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    static SharedMemory allowed;
+    const cudaError_t e = allowed.allow((const void*)attend_few<DT, D>, bytes);
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute pdl;
     pdl.id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -26,7 +26,7 @@ or is skipped, as each function says.
 
 from __future__ import annotations
 
-import ctypes
+import functools
 import math
 
 import torch
@@ -90,118 +90,124 @@ def rotary_tables(max_pos: int, rotary_dim: int, theta: float = 10000.0, scaling
     return (ang.cos() * factor).to(dtype), (ang.sin() * factor).to(dtype)
 
 
-# -- arguments
+# -- arguments: each tensor is looked at once, into a tuple of plain numbers
+_PTR, _LD, _ROWS, _COLS, _SIZE = range(5)
+
+
 def _rows(what, name, t, dtypes, device=None, cols=None):
-    """A (rows, cols) tensor whose rows start on 16-byte boundaries."""
-    if t.dim() != 2:
-        raise ValueError(f"{what}: {name} is 2-D")
+    """(address, elements between rows, rows, columns, element size) of a 2-D tensor whose rows start on 16-byte boundaries."""
     if t.dtype not in dtypes:
         raise TypeError(f"{what}: {name} has unsupported dtype {t.dtype}")
+    shape = t.shape
+    if len(shape) != 2:
+        raise ValueError(f"{what}: {name} is 2-D")
     if device is not None and t.device != device:
         raise ValueError(f"{what}: {name} is on {t.device}, the others on {device}")
-    if cols is not None and t.shape[1] != cols:
-        raise ValueError(f"{what}: {name} has {t.shape[1]} columns, expected {cols}")
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]) or \
-            t.stride(0) * t.element_size() % 16 or t.data_ptr() % 16:
+    rows, width = shape
+    if cols is not None and width != cols:
+        raise ValueError(f"{what}: {name} has {width} columns, expected {cols}")
+    ld, inner = t.stride()
+    ptr, size = t.data_ptr(), t.itemsize
+    if (inner != 1 and width > 1) or (ld < width and rows > 1) or ld * size % 16 or ptr % 16:
         raise ValueError(f"{what}: {name} needs unit inner stride and rows that start on 16-byte boundaries")
-    return t
-
-
-def _row_stride(t) -> int:
-    """Elements between rows; a single row's stride says nothing."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    return ptr, ld if ld > width else width, rows, width, size          # (a single row's stride says nothing)
 
 
 def _ints(what, name, t, device, dim):
     if t.dtype != torch.int32:
         raise TypeError(f"{what}: {name} is int32")
-    if t.device != device or t.dim() != dim or t.stride(0) < 0 or (t.shape[dim - 1] > 1 and t.stride(dim - 1) != 1):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != dim or t.device != device or stride[0] < 0 or (stride[-1] != 1 and shape[-1] > 1):
         raise ValueError(f"{what}: {name} is a {dim}-D tensor on {device} with unit inner stride")
+    return t.data_ptr(), stride[0], shape
 
 
 def _batch(what, rows, pos, starts, device) -> _lib.Batch:
-    _ints(what, "pos", pos, device, 2)
-    seqs = pos.shape[0]
-    if pos.shape[1] != 1:
+    ptr, ld, shape = _ints(what, "pos", pos, device, 2)
+    seqs = shape[0]
+    if shape[1] != 1:
         raise ValueError(f"{what}: pos has one column, one row per sequence")
+    bounds = None
     if starts is not None:
-        _ints(what, "starts", starts, device, 1)
-        if starts.shape[0] != seqs + 1:
+        bounds, _, shape = _ints(what, "starts", starts, device, 1)
+        if shape[0] != seqs + 1:
             raise ValueError(f"{what}: starts has one entry more than there are sequences")
     elif (rows % seqs if seqs else rows):
         raise ValueError(f"{what}: {rows} rows for {seqs} sequences: without starts every sequence has the same number")
-    return _lib.Batch(pos.data_ptr(), None if starts is None else starts.data_ptr(), pos.stride(0), rows, seqs)
+    return _lib.Batch(ptr, bounds, ld, rows, seqs)
 
 
 def _rotation(what, cos, sin, interleaved, head_dim, device) -> _lib.Rotation:
-    for name, t in (("cos", cos), ("sin", sin)):
-        _rows(what, name, t, _FLOATS, device)
-    if cos.shape != sin.shape or cos.dtype != sin.dtype:
+    c, s = _rows(what, "cos", cos, _FLOATS, device), _rows(what, "sin", sin, _FLOATS, device)
+    if c[_ROWS:] != s[_ROWS:] or cos.dtype != sin.dtype:
         raise ValueError(f"{what}: cos and sin have one shape and dtype")
-    n = cos.shape[1]
+    rows, n = c[_ROWS], c[_COLS]
     if n % 8 or n == 0 or 2 * n > head_dim:
         raise ValueError(f"{what}: cos has {n} columns: half the rotated part of a head of {head_dim}, a multiple of 8")
-    if cos.shape[0] == 0:
+    if rows == 0:
         raise ValueError(f"{what}: empty tables")
-    return _lib.Rotation(cos.data_ptr(), sin.data_ptr(), _row_stride(cos), _row_stride(sin), cos.shape[0], n, DTYPE_CODE[cos.dtype],
-                         1 if interleaved else 0)
+    return _lib.Rotation(c[_PTR], s[_PTR], c[_LD], s[_LD], rows, n, DTYPE_CODE[cos.dtype], 1 if interleaved else 0)
 
 
-def _cache(what, k_cache, v_cache, pages, seqs, kv_heads, head_dim, page_size, dtype, device) -> _lib.PagedCache:
+def _cache(what, k_cache, v_cache, pages, seqs, kv_heads, head_dim, page_size, dtype, device):
+    """mk_paged_cache and what _rows says of k_cache and v_cache"""
     if kv_heads <= 0:
         raise ValueError(f"{what}: kv_heads is positive")
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        _rows(what, name, t, _HALVES, device, kv_heads * head_dim)
-        if t.dtype != dtype:
-            raise TypeError(f"{what}: {name} is {t.dtype}, the activations {dtype}")
+    k = _rows(what, "k_cache", k_cache, _HALVES, device, kv_heads * head_dim)
+    v = _rows(what, "v_cache", v_cache, _HALVES, device, kv_heads * head_dim)
+    if k_cache.dtype != dtype or v_cache.dtype != dtype:
+        raise TypeError(f"{what}: k_cache is {k_cache.dtype}, v_cache {v_cache.dtype}, the activations {dtype}")
     if page_size < 16 or page_size & (page_size - 1):
         raise ValueError(f"{what}: page_size is a power of two from 16 up")
-    if k_cache.shape != v_cache.shape or k_cache.shape[0] % page_size:
+    rows = k[_ROWS]
+    if rows != v[_ROWS] or rows % page_size:
         raise ValueError(f"{what}: k_cache and v_cache have one shape, whole pages of {page_size} rows")
-    _ints(what, "pages", pages, device, 2)
-    if pages.shape[0] != seqs:
-        raise ValueError(f"{what}: pages has {pages.shape[0]} rows, pos {seqs}")
-    if max(k_cache.shape[0], pages.shape[1] * page_size) > 2 ** 31 - 1:
+    table, table_ld, shape = _ints(what, "pages", pages, device, 2)
+    if shape[0] != seqs:
+        raise ValueError(f"{what}: pages has {shape[0]} rows, pos {seqs}")
+    if rows > 2 ** 31 - 1 or shape[1] * page_size > 2 ** 31 - 1:
         raise ValueError(f"{what}: at most 2^31 - 1 rows in the cache and of a sequence")
-    return _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), pages.data_ptr(), _row_stride(k_cache), _row_stride(v_cache),
-                           pages.stride(0), k_cache.shape[0] // page_size, page_size, pages.shape[1], kv_heads, head_dim, DTYPE_CODE[dtype])
+    return _lib.PagedCache(k[_PTR], v[_PTR], table, k[_LD], v[_LD], table_ld, rows // page_size, page_size, shape[1], kv_heads, head_dim,
+                           DTYPE_CODE[dtype]), k, v
 
 
-def _out(what, out, like, cols):
+def _out(what, out, like, device, dtype, rows, cols):
+    """The result tensor, what _rows says of it, and whether it is the caller's."""
     if out is None:
-        return torch.empty(like.shape[0], cols, dtype=like.dtype, device=like.device)
-    _rows(what, "out", out, (like.dtype,), like.device, cols)
-    if out.shape[0] != like.shape[0]:
-        raise ValueError(f"{what}: out has {like.shape[0]} rows")
-    return out
+        out = torch.empty((rows, cols), dtype=dtype, device=device)
+        return out, (out.data_ptr(), cols, rows, cols, like[_SIZE]), False
+    o = _rows(what, "out", out, (dtype,), device, cols)
+    if o[_ROWS] != rows:
+        raise ValueError(f"{what}: out has {rows} rows")
+    return out, o, True
 
 
-def _span(t) -> tuple[int, int]:
-    """First and last byte address of a (rows, cols) tensor."""
-    if t.numel() == 0:
-        return (0, -1)
-    return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size() - 1
+def _apart(what, name, a, b):
+    """Refuse a result that shares memory with what the call reads (column ranges of one tensor are apart)."""
+    a0, b0 = a[_PTR], b[_PTR]
+    if a[_ROWS] == 0 or b[_ROWS] == 0 or a0 >= b0 + ((b[_ROWS] - 1) * b[_LD] + b[_COLS]) * b[_SIZE] or \
+            b0 >= a0 + ((a[_ROWS] - 1) * a[_LD] + a[_COLS]) * a[_SIZE]:
+        return
+    pitch = a[_LD] * a[_SIZE]
+    if pitch == b[_LD] * b[_SIZE]:                   # both in one grid of rows: compare the column ranges
+        at = (b0 - a0) % pitch
+        if at >= a[_COLS] * a[_SIZE] and at + b[_COLS] * b[_SIZE] <= pitch:
+            return
+    raise ValueError(f"{what}: {name} shares memory with an operand")
 
 
-def _apart(what, name, written, *read):
-    """Refuse outputs that share memory with what the call reads (column ranges of one tensor are apart)."""
-    a0, a1 = _span(written)
-    for t in read:
-        b0, b1 = _span(t)
-        if a0 > b1 or b0 > a1:
-            continue
-        pitch = written.stride(0) * written.element_size()
-        if pitch and pitch == t.stride(0) * t.element_size():        # both in one grid of rows: compare the column ranges
-            at, wa, wb = (b0 - a0) % pitch, written.shape[1] * written.element_size(), t.shape[1] * t.element_size()
-            if at >= wa and at + wb <= pitch:
-                continue
-        raise ValueError(f"{what}: {name} shares memory with an operand")
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(device_index, heads, kv_heads, head_dim, max_new) -> int:
+    nbytes = _lib.load().mk_paged_attention_workspace(device_index, heads, kv_heads, head_dim, max_new)
+    if nbytes < 0:
+        _lib.check(int(nbytes), "mk_paged_attention_workspace")
+    return nbytes
 
 
 def _stream(what, device):
     if device.type != "cuda":
         raise ValueError(f"{what}: expected CUDA tensors")
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch.cuda.current_stream(device.index).cuda_stream
 
 
 def _heads(what, heads, head_dim):
@@ -220,17 +226,17 @@ def rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Ten
     becomes zeros.  ``out`` may be x itself."""
     what = "rotary"
     _heads(what, heads, head_dim)
-    _rows(what, "x", x, _FLOATS, None, heads * head_dim)
-    rot = _rotation(what, cos, sin, interleaved, head_dim, x.device)
-    batch = _batch(what, x.shape[0], pos, starts, x.device)
-    out = _out(what, out, x, heads * head_dim)
-    if out.data_ptr() != x.data_ptr() or _row_stride(out) != _row_stride(x):
-        _apart(what, "out", out, x)
-    stream = _stream(what, x.device)
-    if batch.rows == 0:
-        return out
-    _lib.check(_lib.load().mk_rotary(x.device.index, batch, rot, x.data_ptr(), _row_stride(x), out.data_ptr(), _row_stride(out),
-                                     DTYPE_CODE[x.dtype], heads, head_dim, stream), "mk_rotary")
+    src = _rows(what, "x", x, _FLOATS, None, heads * head_dim)
+    device, dtype, rows = x.device, x.dtype, src[_ROWS]
+    rot = _rotation(what, cos, sin, interleaved, head_dim, device)
+    batch = _batch(what, rows, pos, starts, device)
+    out, dst, given = _out(what, out, src, device, dtype, rows, heads * head_dim)
+    if given and dst != src:
+        _apart(what, "out", dst, src)
+    stream = _stream(what, device)
+    if rows:
+        _lib.check(_lib.load().mk_rotary(device.index, batch, rot, src[_PTR], src[_LD], dst[_PTR], dst[_LD], DTYPE_CODE[dtype], heads,
+                                         head_dim, stream), "mk_rotary")
     return out
 
 
@@ -245,18 +251,22 @@ def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: t
     row: pages that sequences share lie below their positions."""
     what = "paged_append"
     _heads(what, heads, head_dim)
-    _rows(what, "qkv", qkv, _HALVES, None, (heads + 2 * kv_heads) * head_dim)
-    rot = _rotation(what, cos, sin, interleaved, head_dim, qkv.device)
-    batch = _batch(what, qkv.shape[0], pos, starts, qkv.device)
-    cache = _cache(what, k_cache, v_cache, pages, batch.seqs, kv_heads, head_dim, page_size, qkv.dtype, qkv.device)
-    out = _out(what, out, qkv, heads * head_dim)
-    for name, t, others in (("out", out, (qkv, k_cache, v_cache)), ("k_cache", k_cache, (qkv, v_cache)), ("v_cache", v_cache, (qkv,))):
-        _apart(what, name, t, *others)
-    stream = _stream(what, qkv.device)
-    if batch.rows == 0:
-        return out
-    _lib.check(_lib.load().mk_paged_append(qkv.device.index, batch, rot, cache, qkv.data_ptr(), _row_stride(qkv), out.data_ptr(),
-                                           _row_stride(out), heads, stream), "mk_paged_append")
+    src = _rows(what, "qkv", qkv, _HALVES, None, (heads + 2 * kv_heads) * head_dim)
+    device, dtype, rows = qkv.device, qkv.dtype, src[_ROWS]
+    rot = _rotation(what, cos, sin, interleaved, head_dim, device)
+    batch = _batch(what, rows, pos, starts, device)
+    cache, k, v = _cache(what, k_cache, v_cache, pages, batch.seqs, kv_heads, head_dim, page_size, dtype, device)
+    out, dst, given = _out(what, out, src, device, dtype, rows, heads * head_dim)
+    if given:
+        for t in (src, k, v):
+            _apart(what, "out", dst, t)
+    _apart(what, "k_cache", k, src)
+    _apart(what, "v_cache", v, src)
+    _apart(what, "k_cache", k, v)
+    stream = _stream(what, device)
+    if rows:
+        _lib.check(_lib.load().mk_paged_append(device.index, batch, rot, cache, src[_PTR], src[_LD], dst[_PTR], dst[_LD], heads, stream),
+                   "mk_paged_append")
     return out
 
 
@@ -282,23 +292,25 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     window = int(window or 0)
     if window < 0 or window > 2 ** 31 - 1:
         raise ValueError(f"{what}: window is a number of tokens (0 or None: the whole context)")
-    _rows(what, "q", q, _HALVES, None, heads * head_dim)
-    device = q.device
-    batch = _batch(what, q.shape[0], pos, starts, device)
-    cache = _cache(what, k_cache, v_cache, pages, batch.seqs, kv_heads, head_dim, page_size, q.dtype, device)
-    out = _out(what, out, q, heads * head_dim)
-    _apart(what, "out", out, q, k_cache, v_cache)
-    if max_new is None or starts is None:
-        max_new = batch.rows if starts is not None else batch.rows // max(batch.seqs, 1)
+    src = _rows(what, "q", q, _HALVES, None, heads * head_dim)
+    device, dtype, rows = q.device, q.dtype, src[_ROWS]
+    batch = _batch(what, rows, pos, starts, device)
+    seqs = batch.seqs
+    cache, k, v = _cache(what, k_cache, v_cache, pages, seqs, kv_heads, head_dim, page_size, dtype, device)
+    out, dst, given = _out(what, out, src, device, dtype, rows, heads * head_dim)
+    if given:
+        for t in (src, k, v):
+            _apart(what, "out", dst, t)
     stream = _stream(what, device)
-    if batch.rows == 0:
+    if rows == 0 or seqs == 0:
         return out
-    lib = _lib.load()
-    nbytes = lib.mk_paged_attention_workspace(device.index, heads, cache, max_new)
-    if nbytes < 0:
-        _lib.check(int(nbytes), "mk_paged_attention_workspace")
+    if starts is None:
+        max_new = rows // seqs
+    elif max_new is None:
+        max_new = rows
+    nbytes = _workspace_bytes(device.index, heads, kv_heads, head_dim, max_new)
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _lib.check(lib.mk_paged_attention(device.index, batch, cache, q.data_ptr(), _row_stride(q), out.data_ptr(), _row_stride(out), heads,
-                                      head_dim ** -0.5 if scale is None else scale, window, max_new, workspace.data_ptr(), nbytes,
-                                      stream), "mk_paged_attention")
+    _lib.check(_lib.load().mk_paged_attention(device.index, batch, cache, src[_PTR], src[_LD], dst[_PTR], dst[_LD], heads,
+                                      head_dim ** -0.5 if scale is None else scale, window, max_new, workspace.data_ptr(), nbytes, stream),
+               "mk_paged_attention")
     return out

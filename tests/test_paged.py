@@ -688,11 +688,11 @@ def test_abi_refusals():
     for bad in (R(cos=None), R(rows=0), R(columns=12), R(columns=40), R(dtype=3), R(ld_sin=30), R(sin=4100)):
         assert append(r=bad) == rotary(r=bad) == E
     assert attention(c=C(head_dim=32)) == attention(heads=3) == attention(window=-1) == attention(q=None) == attention(ld_q=252) == attention(out=8200) == E
-    assert attention(nbytes=1) == attention(ws=None) == attention(ws=4100) == E
+    assert attention(ws=None) == attention(ws=4100) == E and attention(nbytes=1) < 0
     assert append(ld=504) == append(ld_q=128) == append(qkv=4104) == append(heads=0) == E
     assert rotary(dtype=3) == rotary(head_dim=60) == rotary(out=None) == rotary(ld=128) == E
     assert b"16-byte" in lib.mk_last_cuda_error() or lib.mk_last_cuda_error()
-    assert lib.mk_paged_attention_workspace(0, 3, C(), 1) == E
+    assert lib.mk_paged_attention_workspace(0, 3, 2, 64, 1) == lib.mk_paged_attention_workspace(0, 4, 2, 96, 1) == E
     # nothing to do: nothing is launched
     none = B(rows=0)
     assert attention(none) == append(none) == rotary(none) == 0
