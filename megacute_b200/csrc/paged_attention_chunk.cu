@@ -61,23 +61,28 @@ struct Sync {
     int odd_any[kOddItems][2];
 };
 
-__device__ __forceinline__ bool wait_bar(Sync* s, unsigned long long* bar, uint32_t parity) {
-    for (int i = 0; i < 64; ++i)
-        if (mbar_test_wait(bar, parity)) return true;
-    const unsigned long long t0 = globaltimer();
-    while (!mbar_try_wait(bar, parity)) {
-        if (*(volatile int*)&s->abort) return false;
-        if (globaltimer() - t0 > kWaitNs) {
-            *(volatile int*)&s->abort = 1;
-            atomicExch(&g_paged_failed, 1);
-            return false;
+// All lanes of a warp wait for one phase.  Asked once in line; the rest, with the limit, is a call, so that the roles' loops stay short.
+__device__ __noinline__ bool wait_longer(Sync* s, uint32_t bar, uint32_t parity) {
+    auto* const at = reinterpret_cast<unsigned long long*>(__cvta_shared_to_generic(bar));
+    bool ok = false;
+    for (int i = 0; i < 64 && !ok; ++i) ok = mbar_test_wait(at, parity);
+    if (!ok) {
+        const unsigned long long t0 = globaltimer();
+        for (;;) {
+            ok = mbar_try_wait(at, parity);
+            if (ok || *(volatile int*)&s->abort) break;
+            if (globaltimer() - t0 > kWaitNs) {
+                *(volatile int*)&s->abort = 1;
+                atomicExch(&g_paged_failed, 1);
+                break;
+            }
         }
     }
-    return true;
+    return __all_sync(0xffffffffu, ok);
 }
 __device__ __forceinline__ bool warp_wait(Sync* s, unsigned long long* bar, uint32_t parity) {
     if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
-    return __all_sync(0xffffffffu, wait_bar(s, bar, parity));
+    return wait_longer(s, smem_u32(bar), parity);
 }
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* m, int x, int y, unsigned long long* bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(m),
@@ -273,77 +278,140 @@ __device__ __forceinline__ void load_role(const AttnArgs& a, const Maps& m, uint
 }
 
 // ---- products -----------------------------------------------------------------------------------------------------------------
+// One warp issues all of a block's products, and what it executes between two of them is time the tensor cores stand still: positions in the rings
+// are counted on, not computed, and the two tiles are written out.
+__device__ __forceinline__ uint64_t desc_at(uint32_t lo, uint32_t hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+    return d;
+}
+template <int DT, int D>
+struct Products {
+    using M = Map<D>;
+    static constexpr uint32_t kFmt = DT == DT_F16 ? 0u : 1u;
+    // fp32 accumulator, M = 128; S: N = 128, both operands K-major; O: N = D, B MN-major
+    static constexpr uint32_t kBasic = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((128u >> 4) << 24);
+    static constexpr uint32_t kIdescS = kBasic | ((128u >> 3) << 17), kIdescO = kBasic | (1u << 16) | (((uint32_t)D >> 3) << 17);
+    Sync* sy;
+    uint32_t tmem;
+    uint32_t lo, hi, vlo;                             // halves of the descriptor of shared memory's first byte, as K-major and as MN-major operand
+    bool leader;
+    uint32_t kt = 0, vt = 0, kslot = 0, vslot = 1;    // key tiles whose scores (of the first tile), whose P V came last; their slots
+    uint32_t sbuf = 0, pbuf = 0;                      // columns of the next scores, of the next P
+    uint32_t sdone[2] = {0, 0}, pdone[2] = {0, 0};    // blocks of scores, of P V of each tile
+    uint32_t items = 0, outs[2] = {0, 0};
+
+    __device__ __forceinline__ bool key_tile() { return warp_wait(sy, &sy->k_full[kt & (kRingBars - 1)], (kt / kRingBars) & 1u); }
+    // S of tile T from the key tile in slot kslot; the last tile of an item moves on to the next key tile
+    template <int T, bool LAST>
+    __device__ __forceinline__ void scores(bool item_ends) {
+        const uint32_t q = lo + ((M::kQ + T * M::kTile) >> 4), k0 = lo + (M::kRing >> 4) + kslot * (M::kTile >> 4);
+        if (leader) {
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                const uint32_t off = (k & 3) * 2 + (k >> 2) * (kSubBytes >> 4);
+                tc_mma(tmem + sbuf, desc_at(q + off, hi), desc_at(k0 + off, hi), kIdescS, k ? 1u : 0u);
+            }
+            tc_commit(&sy->s_full[T][sdone[T] & 3u]);
+            if (LAST) tc_commit(&sy->slot_free[kslot]);
+            if (LAST && item_ends) tc_commit(&sy->q_free);
+        }
+        __syncwarp();
+        ++sdone[T];
+        sbuf = sbuf + 128 == M::kScores * 128 ? 0 : sbuf + 128;
+        if (LAST) {
+            ++kt;
+            kslot = kslot + 2 >= M::kSlots ? kslot + 2 - M::kSlots : kslot + 2;
+        }
+    }
+    // O += P V of tile T, the value tile in slot vslot
+    template <int T, bool LAST>
+    __device__ __forceinline__ bool values(bool first) {
+        if (first && !warp_wait(sy, &sy->o_free[T], (outs[T] & 1u) ^ 1u)) return false;       // (the item before has been read)
+        if (!warp_wait(sy, &sy->p_full[T][pdone[T] & 3u], (pdone[T] >> 2) & 1u)) return false;
+        tc_fence_after();
+        const uint32_t v = vlo + (M::kRing >> 4) + vslot * (M::kTile >> 4);
+        const uint32_t keep = first ? 0u : 1u;
+        if (leader) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)                // 16 keys: 8 columns of P, 2048 bytes of V
+                mma_ta(tmem + M::kO + D * T, tmem + pbuf + 8 * k, desc_at(v + 128 * k, hi), kIdescO, k ? 1u : keep);
+            tc_commit(&sy->pv_done[T][pdone[T] & 3u]);
+            if (LAST) tc_commit(&sy->slot_free[vslot]);
+        }
+        __syncwarp();
+        ++pdone[T];
+        pbuf = pbuf + 128 == M::kScores * 128 ? 0 : pbuf + 128;
+        if (LAST) {
+            ++vt;
+            vslot = vslot + 2 >= M::kSlots ? vslot + 2 - M::kSlots : vslot + 2;
+        }
+        return true;
+    }
+    __device__ __forceinline__ bool value_tile() { return warp_wait(sy, &sy->v_ready[vt & (kRingBars - 1)], (vt / kRingBars) & 1u); }
+
+    // An item of two tiles: the scores of block n + kScores (blocks of both tiles in turns) right behind P V of block n, into the same columns.
+    __device__ __forceinline__ bool two(int units) {
+        if (!key_tile()) return false;
+        tc_fence_after();
+        scores<0, false>(false);
+        scores<1, true>(units == 1);
+        if (M::kScores == 3 && units > 1) {
+            if (!key_tile()) return false;
+            scores<0, false>(false);
+        }
+        for (int j = 0; j < units; ++j) {
+            if (!value_tile()) return false;
+            if (M::kScores == 3) {
+                if (!values<0, false>(j == 0)) return false;
+                if (j + 1 < units) scores<1, true>(j + 2 == units);
+                if (j + 2 < units && !key_tile()) return false;
+                if (!values<1, true>(j == 0)) return false;
+                if (j + 2 < units) scores<0, false>(false);
+            } else {
+                if (j + 1 < units && !key_tile()) return false;
+                if (!values<0, false>(j == 0)) return false;
+                if (j + 1 < units) scores<0, false>(false);
+                if (!values<1, true>(j == 0)) return false;
+                if (j + 1 < units) scores<1, true>(j + 2 == units);
+            }
+        }
+        return true;
+    }
+    __device__ __forceinline__ bool one(int units) {
+        for (int j = 0; j < M::kScores && j < units; ++j) {
+            if (!key_tile()) return false;
+            tc_fence_after();
+            scores<0, true>(j + 1 == units);
+        }
+        for (int j = 0; j < units; ++j) {
+            const bool more = j + M::kScores < units;
+            if (!value_tile() || (more && !key_tile()) || !values<0, true>(j == 0)) return false;
+            if (more) scores<0, true>(j + M::kScores + 1 == units);
+        }
+        return true;
+    }
+};
 template <int DT, int D>
 __device__ __forceinline__ void product_role(const AttnArgs& a, uint8_t* smem, Sync* sy, Walk<kShift> w, uint32_t tmem) {
-    using M = Map<D>;
-    const uint32_t fmt = DT == DT_F16 ? 0u : 1u;
-    // fp32 accumulator, M = 128; S: N = 128, both operands K-major; O: N = D, B MN-major
-    const uint32_t basic = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 4) << 24);
-    const uint32_t idesc_s = basic | ((128u >> 3) << 17), idesc_o = basic | (1u << 16) | (((uint32_t)D >> 3) << 17);
     const uint64_t d0 = tc_smem_desc(smem_u32(smem));
+    Products<DT, D> p;
+    p.sy = sy;
+    p.tmem = __shfl_sync(0xffffffffu, tmem, 0);       // (the same in all lanes, told so to the compiler: operands in uniform registers)
+    p.lo = (uint32_t)d0;
+    p.hi = (uint32_t)(d0 >> 32);
     // MN-major: 8-key groups 1024 bytes apart (the descriptor's stride), sub-tiles of 64 columns 16 KB apart (its leading offset)
-    const uint64_t v0 = D == 64 ? d0 : d0 - (1ull << 16) + ((uint64_t)(kSubBytes >> 4) << 16);
-    uint32_t c = 0, items = 0, scores_done = 0, blocks[2] = {0, 0}, outs[2] = {0, 0};
-    for (; w.left > 0; ++items) {
-        const Part p = part_of(a, w);
-        const int total = p.units * p.tiles;
-        int done[2] = {0, 0};                         // blocks of this item whose P V has been issued (`blocks`: of all)
-        const uint32_t first = scores_done;
-        // K of the n-th block has landed (asked for ahead of its product, and for the first of two tiles only)
-        auto landed = [&](int n) {
-            const int t = p.tiles == 2 ? n & 1 : 0;
-            const uint32_t kt = c + (uint32_t)(p.tiles == 2 ? n >> 1 : n);
-            return t != 0 || warp_wait(sy, &sy->k_full[kt % kRingBars], (kt / kRingBars) & 1u);
-        };
-        auto scores = [&](int n) {
-            const int t = p.tiles == 2 ? n & 1 : 0, j = p.tiles == 2 ? n >> 1 : n;
-            const uint32_t slot = 2 * (c + (uint32_t)j) % M::kSlots, buf = scores_done % M::kScores;
-            const uint64_t qd = d0 + (uint32_t)((M::kQ + t * M::kTile) >> 4), kd = d0 + (uint32_t)((M::kRing + slot * M::kTile) >> 4);
-            if (elect_one()) {
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t off = (k & 3) * 2 + (k >> 2) * (kSubBytes >> 4);
-                    tc_mma(tmem + 128 * buf, qd + off, kd + off, idesc_s, k ? 1u : 0u);
-                }
-                tc_commit(&sy->s_full[t][(blocks[t] + (uint32_t)(j - done[t])) & 3u]);
-                if (t == p.tiles - 1) tc_commit(&sy->slot_free[slot]);
-                if (n == total - 1) tc_commit(&sy->q_free);
-            }
-            __syncwarp();
-            ++scores_done;
-        };
-        if (!warp_wait(sy, &sy->q_full, items & 1u)) return;
-        for (int n = 0; n < M::kScores && n < total; ++n) {
-            if (!landed(n)) return;
-            tc_fence_after();
-            scores(n);
-        }
-        for (int n = 0; n < total; ++n) {
-            const int t = p.tiles == 2 ? n & 1 : 0, j = p.tiles == 2 ? n >> 1 : n;
-            const uint32_t kt = c + (uint32_t)j, slot = (2 * kt + 1) % M::kSlots, buf = (first + (uint32_t)n) % M::kScores;
-            const bool more = n + M::kScores < total;
-            if (t == 0 && !warp_wait(sy, &sy->v_ready[kt % kRingBars], (kt / kRingBars) & 1u)) return;
-            if (more && !landed(n + M::kScores)) return;
-            // (the first product of an item overwrites O: the one before has been read)
-            if (j == 0 && !warp_wait(sy, &sy->o_free[t], (outs[t] & 1u) ^ 1u)) return;
-            if (!warp_wait(sy, &sy->p_full[t][blocks[t] & 3u], (blocks[t] >> 2) & 1u)) return;
-            tc_fence_after();
-            const uint64_t vd = v0 + (uint32_t)((M::kRing + slot * M::kTile) >> 4);
-            if (elect_one()) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k)            // 16 keys: 8 columns of P, 2048 bytes of V
-                    mma_ta(tmem + M::kO + D * t, tmem + 128 * buf + 8 * k, vd + 128 * k, idesc_o, j > 0 || k > 0 ? 1u : 0u);
-                tc_commit(&sy->pv_done[t][blocks[t] & 3u]);
-                if (t == p.tiles - 1) tc_commit(&sy->slot_free[slot]);
-            }
-            __syncwarp();
-            ++blocks[t];
-            ++done[t];
-            if (more) scores(n + M::kScores);
-        }
-        c += (uint32_t)p.units;
-        for (int t = 0; t < p.tiles; ++t) ++outs[t];
-        w.next(a, p.units);
+    p.vlo = D == 64 ? p.lo : p.lo - (1u << 16) + ((uint32_t)(kSubBytes >> 4) << 16);
+    p.leader = elect_one();
+    while (w.left > 0) {
+        const Part part = part_of(a, w);
+        const int units = __shfl_sync(0xffffffffu, part.units, 0), tiles = __shfl_sync(0xffffffffu, part.tiles, 0);
+        if (!warp_wait(sy, &sy->q_full, p.items & 1u)) return;
+        if (!(tiles == 2 ? p.two(units) : p.one(units))) return;
+        ++p.items;
+        ++p.outs[0];
+        if (tiles == 2) ++p.outs[1];
+        w.next(a, part.units);
     }
 }
 
