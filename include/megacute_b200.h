@@ -268,7 +268,7 @@ int mk_paged_append(int device, const mk_batch* batch, const mk_rotation* rot, c
 /* out[r, h] = softmax(scale * q[r, h] K^T) V over the cache rows [max(0, p + 1 - window), p] of the row's sequence (p: the row's
  * position; window 0: from row 0), those of absent pages left out; a row that sees none becomes zeros.  max_new: the largest number of
  * rows of a sequence, which the choice of kernel goes by; results are right whatever it is.  `workspace`: device memory of at least
- * mk_paged_attention_workspace() bytes, 16-byte aligned, used by this call alone until it has run. */
+ * mk_paged_attention_workspace() bytes, 256-byte aligned, used by this call alone until it has run. */
 long long mk_paged_attention_workspace(int device, int heads, int kv_heads, int head_dim, int max_new);
 int mk_paged_attention(int device, const mk_batch* batch, const mk_paged_cache* cache, const void* q, int64_t ld_q, void* out, int64_t ld_out,
                        int heads, float scale, int window, int max_new, void* workspace, size_t workspace_bytes, void* stream);

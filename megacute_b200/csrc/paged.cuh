@@ -65,21 +65,21 @@ struct Batch {
     const int* pos;
     const int* starts;
     long long pos_ld;
-    int rows, seqs;
+    int rows, seqs, each;                             // each: rows of a sequence where there are no starts
     // first row and number of rows of sequence s, inside the packed batch whatever `starts` holds
     __device__ __forceinline__ int first(int s) const {
-        return starts ? min(max(__ldg(starts + s), 0), rows) : s * (rows / seqs);
+        return starts ? min(max(__ldg(starts + s), 0), rows) : s * each;
     }
     __device__ __forceinline__ int count(int s, int r0) const {
-        return starts ? min(max(__ldg(starts + s + 1), r0), rows) - r0 : rows / seqs;
+        return starts ? min(max(__ldg(starts + s + 1), r0), rows) - r0 : each;
     }
     __device__ __forceinline__ int position(int s) const { return __ldg(pos + s * pos_ld); }
 };
-inline Batch batch_of(const mk_batch* b) { return Batch{b->pos, b->starts, (long long)b->pos_ld, b->rows, b->seqs}; }
+inline Batch batch_of(const mk_batch* b) { return Batch{b->pos, b->starts, (long long)b->pos_ld, b->rows, b->seqs, b->rows / b->seqs}; }
 
 // The sequence of row r, -1 if it has none: a whole warp asks for one row, 32 entries of `starts` at a time.
 __device__ __forceinline__ int sequence_of_row(const Batch& b, int r) {
-    if (!b.starts) return r / (b.rows / b.seqs);
+    if (!b.starts) return r / b.each;
     const int lane = threadIdx.x & 31;
     int lo = 0, n = b.seqs + 1;                       // entries [lo, lo + n) hold the border; those in front are <= r
     while (n > 0) {

@@ -17,8 +17,11 @@ __global__ void __launch_bounds__(kJoinThreads) join_parts(const __grid_constant
     const int w = blockIdx.x, first = blockIdx.y * ROWS;
     const int4 j = __ldcg(a.joins + w);
     if (j.x == 0 || first >= j.z) return;
-    join.run(a, a.stats, a.parts, j.x, first, min(first + ROWS, j.z), [&](int i) { return (long long)(i == 0 ? 2 * w + 1 : 2 * (w + i)); },
-             [&](int row, int col, float, float l, const float4& o) { write_result<DT, D>(a, j.y, j.w, row, col, l, o); });
+    join.run(a, j.x, first, min(first + ROWS, j.z), [&](int i) { return (long long)(i == 0 ? 2 * w + 1 : 2 * (w + i)); },
+             [&](int row, int col, float l, const float4& x, const float4& y) {
+                 write_result<DT, D>(a, j.y, j.w, row, col, l, x);
+                 write_result<DT, D>(a, j.y, j.w, row, col + 4, l, y);
+             });
 }
 
 const char* shape_error(int heads, int kv_heads, int head_dim) {
@@ -62,7 +65,7 @@ Layout layout_of(int sms, int head_dim, bool few) {
     l.workers = few ? sms * kFewWarps : sms;
     l.part_rows = few ? kFewRows : 2 * kChunkTile;
     const size_t rows = (size_t)sms * 2 * l.part_rows;
-    l.stats = (size_t)sms * sizeof(int4);
+    l.stats = ((size_t)sms * sizeof(int4) + 255) / 256 * 256;
     l.parts = l.stats + rows * sizeof(float2);
     l.own = l.parts + rows * head_dim * sizeof(float);
     l.bytes = l.own + (few ? (size_t)l.workers * kFewRows * head_dim * sizeof(float) : 0);
@@ -111,7 +114,7 @@ extern "C" int mk_paged_attention(int device, const mk_batch* batch, const mk_pa
     const long long width = (long long)heads * D;
     if (!q || !out || ld_q < width || ld_out < width || !aligned16(q, ld_q, 2) || !aligned16(out, ld_out, 2))
         return report(MK_E_ARG, "paged attention: rows hold all heads and start on 16-byte boundaries");
-    if (!workspace || ((uintptr_t)workspace & 15)) return report(MK_E_ARG, "paged attention: workspace of 16-byte aligned device memory");
+    if (!workspace || ((uintptr_t)workspace & 255)) return report(MK_E_ARG, "paged attention: workspace of 256-byte aligned device memory");
     const int sms = sm_count(device);
     if (!sms) return report(MK_E_CUDA, "no such device");
     const bool few = few_rows(group, max_new) || !(scale > 0.f) || scale > 1e30f;

@@ -32,7 +32,10 @@ struct AttnArgs {
     int4* joins;                                      // of each block: parts of the item that it begins and does not end (0: none), its first
                                                       // row, its rows, its block of heads
     float2* stats;                                    // [block][2][part_rows]: maximum (log2 domain) and sum
-    float* parts;                                     // [block][2][part_rows][head_dim]
+    float* parts;                                     // [block][2][head_dim / 8][part_rows][8]: rows side by side, for those who have one each
+    __device__ __forceinline__ float* part(long long slot, int head_dim, int row, int col) const {
+        return parts + ((slot * (head_dim / 8) + (col >> 3)) * part_rows + row) * 8 + (col & 7);
+    }
 };
 
 struct Item {
@@ -145,6 +148,43 @@ struct PlanScratch {
 template <int SHIFT, int THREADS>
 __device__ __forceinline__ Shares plan(const AttnArgs& a, PlanScratch<THREADS>* sc, int worker, int least, Walk<SHIFT>& walk) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    if (a.batch.seqs <= 128) {                        // a few sequences a lane: every warp by itself, in 32 bits
+        const int each = (a.batch.seqs + 31) / 32;
+        int units[4], run = 0;
+        bool big = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int s = lane * each + k;
+            long long u = k < each && s < a.batch.seqs ? sequence_units<SHIFT>(a, s) : 0;
+            big |= u > (1 << 23) / a.blocks;          // (128 of them stay below 2^30)
+            units[k] = (int)u * a.blocks;
+            run += units[k];
+        }
+        if (!__any_sync(0xffffffffu, big)) {
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, run, d);
+                if (lane >= d) run += up;
+            }
+            const Shares shares(__shfl_sync(0xffffffffu, run, 31), a.workers, least);
+            const int begin = worker < shares.workers ? (int)shares.begin(worker) : (int)shares.total;
+            walk.left = worker < shares.workers ? shares.begin(worker + 1) - begin : 0;
+            if (walk.left > 0) {
+                const int in = __popc(__ballot_sync(0xffffffffu, run <= begin));       // the lane that has it
+                int at = begin - (in > 0 ? __shfl_sync(0xffffffffu, run, in - 1) : 0), k = 0, n = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int u = __shfl_sync(0xffffffffu, units[i], in);
+                    if (k == i) {
+                        n = u;
+                        if (at >= u) { at -= u; ++k; }
+                    }
+                }
+                walk.start(a, in * each + k, at, n / a.blocks);
+            }
+            return shares;
+        }
+    }
     const int rounds = (a.batch.seqs + THREADS - 1) / THREADS;
     long long mine = 0, sum = 0;
     for (int r = 0; r < rounds; ++r) {
@@ -193,56 +233,54 @@ __device__ __forceinline__ Shares plan(const AttnArgs& a, PlanScratch<THREADS>* 
     return shares;
 }
 
-// Joins `count` parts of rows [row_begin, row_end) of an item, ROWS of them: part i has `slot(i)`.  With M the largest of their maxima m_i
+// Joins `count` parts of rows [row_begin, row_end) of an item, ROWS of them: part i has slot(i).  With M the largest of their maxima m_i
 //   l = sum_i 2^(m_i - M) l_i,   o = sum_i 2^(m_i - M) o_i,   in the order of i.
-// A thread has four columns of a row; where that leaves threads over they share a row's parts and add through shared memory.  All threads of the block
-// call it.  `write(row, column, M, l, o)` takes four columns.
+// A thread has eight columns of a row; where that leaves threads over they share a row's parts and add through shared memory.  All threads of the block
+// call it.  write(row, column, l, o) takes eight columns.
 template <int D, int ROWS, int THREADS>
 struct Join {
-    static constexpr int kLanes = D / 4, kTasks = ROWS * kLanes, kSplits = kTasks < THREADS ? THREADS / kTasks : 1;
-    static constexpr int kTurns = kTasks > THREADS ? kTasks / THREADS : 1;
-    float4 o[kSplits > 1 ? THREADS : 1];
+    static constexpr int kTasks = ROWS * (D / 8), kSplits = THREADS / kTasks;
+    static_assert(kSplits * kTasks == THREADS, "threads of a join");
+    float4 o[kSplits > 1 ? 2 * THREADS : 1];
     float l[kSplits > 1 ? THREADS : 1];
 
     template <class Slot, class Write>
-    __device__ __forceinline__ void run(const AttnArgs& a, const float2* stats, const float* parts, int count, int row_begin, int row_end, Slot slot,
-                                        Write write) {
-        const int t = threadIdx.x, lane = t % kLanes, split = kSplits > 1 ? t / kTasks : 0;
-#pragma unroll
-        for (int turn = 0; turn < kTurns; ++turn) {
-            const int row = row_begin + (t % kTasks) / kLanes + turn * (THREADS / kLanes);
-            const bool mine = row < row_end;
-            float m = -__builtin_huge_valf(), sum = 0.f;
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (mine) {
+    __device__ __forceinline__ void run(const AttnArgs& a, int count, int row_begin, int row_end, Slot slot, Write write) {
+        const int t = threadIdx.x, split = t / kTasks, row = row_begin + t % ROWS, col = t % kTasks / ROWS * 8;
+        const bool mine = row < row_end;
+        float m = -__builtin_huge_valf(), sum = 0.f;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+        if (mine) {
 #pragma unroll 8
-                for (int i = 0; i < count; ++i) m = fmaxf(m, __ldcg(&stats[slot(i) * a.part_rows + row].x));
-#pragma unroll 8
-                for (int i = split; i < count; i += kSplits) {
-                    const long long at = slot(i) * a.part_rows + row;
-                    const float2 st = __ldcg(&stats[at]);
-                    const float4 v = __ldcg(reinterpret_cast<const float4*>(parts + at * D) + lane);
-                    const float f = st.x == m ? 1.f : ex2(st.x - m);
-                    if (st.x != -__builtin_huge_valf()) {                      // (a part that saw no key has nothing to add)
-                        sum += f * st.y;
-                        x.x += f * v.x; x.y += f * v.y; x.z += f * v.z; x.w += f * v.w;
-                    }
+            for (int i = 0; i < count; ++i) m = fmaxf(m, __ldcg(&a.stats[slot(i) * a.part_rows + row].x));
+#pragma unroll 4
+            for (int i = split; i < count; i += kSplits) {
+                const long long at = slot(i);
+                const float2 st = __ldcg(&a.stats[at * a.part_rows + row]);
+                const float4* const src = reinterpret_cast<const float4*>(a.part(at, D, row, col));
+                const float4 v = __ldcg(src), w = __ldcg(src + 1);
+                const float f = st.x == m ? 1.f : ex2(st.x - m);
+                if (st.x != -__builtin_huge_valf()) {                          // (a part that saw no key has nothing to add)
+                    sum += f * st.y;
+                    x.x += f * v.x; x.y += f * v.y; x.z += f * v.z; x.w += f * v.w;
+                    y.x += f * w.x; y.y += f * w.y; y.z += f * w.z; y.w += f * w.w;
                 }
             }
-            if (kSplits > 1) {
-                __syncthreads();                      // (what a call before this one left has been read)
-                o[t] = x;
-                l[t] = sum;
-                __syncthreads();
-                if (split > 0) continue;
-                for (int k = 1; k < kSplits; ++k) {
-                    const float4 v = o[t + k * kTasks];
-                    sum += l[t + k * kTasks];
-                    x.x += v.x; x.y += v.y; x.z += v.z; x.w += v.w;
-                }
-            }
-            if (mine) write(row, lane * 4, m, sum, x);
         }
+        if (kSplits > 1) {
+            o[t] = x;
+            o[THREADS + t] = y;
+            l[t] = sum;
+            __syncthreads();
+            if (split > 0) return;
+            for (int k = 1; k < kSplits; ++k) {
+                const float4 v = o[t + k * kTasks], w = o[THREADS + t + k * kTasks];
+                sum += l[t + k * kTasks];
+                x.x += v.x; x.y += v.y; x.z += v.z; x.w += v.w;
+                y.x += w.x; y.y += w.y; y.z += w.z; y.w += w.w;
+            }
+        }
+        if (mine) write(row, col, sum, x, y);
     }
 };
 

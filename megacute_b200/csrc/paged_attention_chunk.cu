@@ -452,16 +452,20 @@ __device__ __forceinline__ void value_role(const AttnArgs& a, uint8_t* smem, Syn
 #pragma unroll
                 for (int sub = 0; sub < M::kSubs; ++sub) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const uint32_t at = tile + sub * kSubBytes + i * 512;
-                        if ((none >> i) & 1u) {
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
-                        } else if ((part >> i) & 1u) {
-                            uint32_t x[4];
-                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
+                    for (int i = 0; i < 16; ++i)
+                        asm volatile("{ .reg .pred p; setp.ne.u32 p, %2, 0; @p st.shared.v4.b32 [%0], {%1, %1, %1, %1}; }" ::"r"(tile + sub * kSubBytes + i * 512),
+                                     "r"(0), "r"(none & (1u << i))
+                                     : "memory");
+                    if (!__any_sync(0xffffffffu, part)) continue;
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) odd |= (x[e] & E) + ONE;
-                        }
+                    for (int i = 0; i < 16; ++i) {
+                        uint32_t x[4] = {};
+                        asm volatile("{ .reg .pred p; setp.ne.u32 p, %5, 0; @p ld.shared.v4.b32 {%0, %1, %2, %3}, [%4]; }"
+                                     : "+r"(x[0]), "+r"(x[1]), "+r"(x[2]), "+r"(x[3])
+                                     : "r"(tile + sub * kSubBytes + i * 512), "r"(part & (1u << i))
+                                     : "memory");
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) odd |= (x[e] & E) + ONE;
                     }
                 }
                 if (__any_sync(0xffffffffu, odd & 0x80008000u) && partial < kOddTiles) {
@@ -511,9 +515,12 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
         if (t < p.tiles) {
             const int token = t * tile_tokens + my_token;
             const bool mine = my_token < tile_tokens && token < p.tokens;
-            int lo, hi, lo_all, hi_all;
+            int lo, hi, lo_all, hi_all, lo_any, hi_any, unused;               // keys that this row, every row, some row of the tile sees
             seen_by(a, p, min(token, p.tokens - 1), lo, hi);
-            seen_by_all(a, p, t * tile_tokens, min(p.tokens, (t + 1) * tile_tokens), lo_all, hi_all);
+            const int last = min(p.tokens, (t + 1) * tile_tokens);
+            seen_by_all(a, p, t * tile_tokens, last, lo_all, hi_all);
+            seen_by(a, p, t * tile_tokens, lo_any, unused);
+            seen_by(a, p, last - 1, unused, hi_any);
             float m = NEG_INF, l = 0.f;
             for (int u = 0; u < p.units; ++u) {
                 const uint32_t n = seq0 + (uint32_t)(u * p.tiles + t), buf = n % M::kScores;
@@ -522,10 +529,13 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
                 tc_fence_after();
                 const int key0 = p.key0 + (u << kShift);
                 const uint32_t there = *(volatile uint32_t*)&sy->there[(c + (uint32_t)u) % kSeen];
-                const bool edge = key0 < lo_all || key0 + 127 > hi_all || there != 0xffu;      // keys that this row does not see
+                const bool edge = key0 < lo_all || key0 + 127 > hi_all || there != 0xffu;      // keys that some row does not see
                 const int from = lo - key0, to = hi - key0;
                 float va[32], vb[32];
-                auto hide = [&](int ch, float* v) {                            // columns [32 ch, 32 ch + 32): those in [from, to], of blocks that are there
+                // of 32 columns from 32 ch on, the same for all rows: none is seen; every one is
+                auto nobody = [&](int ch) { return key0 + ch * 32 > hi_any || key0 + ch * 32 + 31 < lo_any || !((there >> 2 * ch) & 3u); };
+                auto hide = [&](int ch, float* v) {                            // those in [from, to], of blocks that are there
+                    if (key0 + ch * 32 >= lo_all && key0 + ch * 32 + 31 <= hi_all && ((there >> 2 * ch) & 3u) == 3u) return;
                     const int f = min(max(from - ch * 32, 0), 32), n = min(max(to + 1 - ch * 32, 0), 32);
                     const uint32_t below = n == 32 ? 0xffffffffu : (1u << n) - 1u, front = f == 32 ? 0xffffffffu : (1u << f) - 1u;
                     const uint32_t two = there >> 2 * ch, w = below & ~front & ((two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u));
@@ -533,24 +543,36 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
                     for (int e = 0; e < 32; ++e) v[e] = w & (1u << e) ? v[e] : NEG_INF;
                 };
                 float m4[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+                if (!edge) {
 #pragma unroll 1
-                for (int ch = 0; ch < 4; ch += 2) {
-                    tmem_ld32(scol + ch * 32, va);
-                    tmem_ld32(scol + ch * 32 + 32, vb);
-                    tmem_wait_ld();
-                    use32(va);
-                    use32(vb);
-                    if (edge) {
-                        hide(ch, va);
-                        hide(ch + 1, vb);
-                    }
+                    for (int ch = 0; ch < 4; ch += 2) {
+                        tmem_ld32(scol + ch * 32, va);
+                        tmem_ld32(scol + ch * 32 + 32, vb);
+                        tmem_wait_ld();
+                        use32(va);
+                        use32(vb);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        m4[0] = max_3(m4[0], va[e], va[e + 1]); m4[1] = max_3(m4[1], va[e + 2], va[e + 3]);
-                        m4[2] = max_3(m4[2], vb[e], vb[e + 1]); m4[3] = max_3(m4[3], vb[e + 2], vb[e + 3]);
+                        for (int e = 0; e < 32; e += 4) {
+                            m4[0] = max_3(m4[0], va[e], va[e + 1]); m4[1] = max_3(m4[1], va[e + 2], va[e + 3]);
+                            m4[2] = max_3(m4[2], vb[e], vb[e + 1]); m4[3] = max_3(m4[3], vb[e + 2], vb[e + 3]);
+                        }
+                    }
+                } else {
+#pragma unroll 1
+                    for (int ch = 0; ch < 4; ++ch) {
+                        if (nobody(ch)) continue;
+                        tmem_ld32(scol + ch * 32, va);
+                        tmem_wait_ld();
+                        use32(va);
+                        hide(ch, va);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            m4[0] = max_3(m4[0], va[e], va[e + 1]); m4[1] = max_3(m4[1], va[e + 2], va[e + 3]);
+                        }
+                        __syncwarp();
                     }
                 }
-                tmem_ld32(scol, va);                                           // (under way meanwhile)
+                if (!edge) tmem_ld32(scol, va);                                // (under way meanwhile)
                 const float mx = max_3(m4[0], m4[1], max_3(m4[2], m4[2], m4[3])) * a.scale2;
                 // (a row that sees NaN or an infinite score has no result; said here, since what follows may lose it)
                 if (!(mx < -NEG_INF)) l = __int_as_float(0x7fffffff);
@@ -591,19 +613,30 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
                     }
                     tmem_st16(scol + ch * 16, x);
                 };
-                auto weigh_all = [&](auto edges) {
+                if (!edge) {
 #pragma unroll 1
                     for (int ch = 0; ch < 4; ch += 2) {
                         tmem_wait_ld();
                         tmem_ld32(scol + ch * 32 + 32, vb);
-                        weigh(ch, va, edges);
+                        weigh(ch, va, Const<false>{});
                         tmem_wait_ld();
                         if (ch == 0) tmem_ld32(scol + 64, va);
-                        weigh(ch + 1, vb, edges);
+                        weigh(ch + 1, vb, Const<false>{});
                     }
-                };
-                if (edge) weigh_all(Const<true>{});
-                else weigh_all(Const<false>{});
+                } else {
+#pragma unroll 1
+                    for (int ch = 0; ch < 4; ++ch) {
+                        if (nobody(ch)) {
+                            uint32_t x[16] = {};
+                            tmem_st16(scol + ch * 16, x);
+                        } else {
+                            tmem_ld32(scol + ch * 32, va);
+                            tmem_wait_ld();
+                            weigh(ch, va, Const<true>{});
+                        }
+                        __syncwarp();
+                    }
+                }
                 l += ((l4[0].x + l4[0].y) + (l4[1].x + l4[1].y)) + ((l4[2].x + l4[2].y) + (l4[3].x + l4[3].y));
                 tmem_wait_st();
                 tc_fence_before();
@@ -615,17 +648,18 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
             if (!warp_wait(sy, &sy->pv_done[t][(blocks - 1u) & 3u], ((blocks - 1u) >> 2) & 1u)) return;
             tc_fence_after();
             const bool whole = p.begins && p.ends;
-            const long long slot_row = ((long long)worker * 2 + (p.begins ? 1 : 0)) * a.part_rows + token * a.group + my_head;
+            const int part_row = token * a.group + my_head;
+            const long long slot = (long long)worker * 2 + (p.begins ? 1 : 0);
             const float inv = l == 0.f ? 0.f : 1.f / l;
             if (p.begins && !p.ends && i == 0 && t == 0) {
                 const long long item_end = end + (w.item.units - p.units);     // (the item is not finished: the worker's last)
                 a.joins[worker] = make_int4(shares.worker_of(item_end - 1) - worker + 1, p.row0, p.tokens * a.group, p.block);
             }
             uint16_t* const to = a.out + (long long)(p.row0 + token) * a.ld_out + (p.block * a.group + my_head) * D;
-            float* const part = a.parts + slot_row * D;
+            const bool sectors = ((uintptr_t)a.out & 31) == 0 && a.ld_out % 16 == 0;       // rows of the result start on 32-byte boundaries
             const uint32_t mem = items % kOddItems;
             const bool odd = (*(volatile int*)&sy->odd_any[mem][0] | *(volatile int*)&sy->odd_any[mem][1]) != 0;
-            if (mine && !whole) a.stats[slot_row] = make_float2(l != l && m == NEG_INF ? 0.f : m, l);
+            if (mine && !whole) a.stats[slot * a.part_rows + part_row] = make_float2(l != l && m == NEG_INF ? 0.f : m, l);
 #pragma unroll 1
             for (int ch = 0; ch < D / 16; ++ch) {
                 float o[16];
@@ -660,12 +694,15 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
                     uint32_t x[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[e] = pack16<DT>(o[2 * e] * inv, o[2 * e + 1] * inv);
-                    reinterpret_cast<uint4*>(to + ch * 16)[0] = make_uint4(x[0], x[1], x[2], x[3]);
-                    reinterpret_cast<uint4*>(to + ch * 16)[1] = make_uint4(x[4], x[5], x[6], x[7]);
+                    st32B(reinterpret_cast<uint8_t*>(to + ch * 16), x, sectors);
                 } else if (mine) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        reinterpret_cast<float4*>(part + ch * 16)[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                    for (int e = 0; e < 2; ++e) {
+                        uint32_t x[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) x[k] = __float_as_uint(o[8 * e + k]);
+                        st32B(reinterpret_cast<uint8_t*>(a.part(slot, D, part_row, ch * 16 + 8 * e)), x, true);
+                    }
                 }
                 __syncwarp();
             }

@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
                 write_result<DT, D>(a, head.row0, head.block, row, col, l, o);
             } else {
                 if (col == 0) a.stats[to * kFewRows + row] = make_float2(m, l);
-                *reinterpret_cast<float4*>(a.parts + (to * kFewRows + row) * D + col) = o;
+                *reinterpret_cast<float4*>(a.part(to, D, row, col)) = o;
             }
         }
     }
