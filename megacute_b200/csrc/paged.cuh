@@ -93,6 +93,10 @@ __device__ __forceinline__ int sequence_of_row(const Batch& b, int r) {
     return lo > b.seqs ? -1 : lo - 1;                 // (lo: entries <= r)
 }
 
+// Kernels are launched with programmatic serialization: their blocks start when those of the kernel in front have ended, and touch no memory before
+// this, which waits until its writes can be seen.
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 struct Pages {
     const int* table;
     long long ld;

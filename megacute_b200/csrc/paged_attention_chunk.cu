@@ -28,7 +28,7 @@ namespace {
 
 constexpr int kChunkThreads = 384;
 constexpr float kLazy = 8.0f;
-constexpr uint32_t kFmaPairs = 0b01001001;            // of eight pairs of exponentials, those that the fp32 units take
+constexpr uint32_t kFmaPairs = 0b00010001;            // of eight pairs of exponentials, those that the fp32 units take
 template <bool V> struct Const { static constexpr bool value = V; };
 constexpr unsigned long long kWaitNs = 2000000000ull;
 constexpr int kTileRows = 128;
@@ -64,18 +64,14 @@ struct Sync {
 // All lanes of a warp wait for one phase.  Asked once in line; the rest, with the limit, is a call, so that the roles' loops stay short.
 __device__ __noinline__ bool wait_longer(Sync* s, uint32_t bar, uint32_t parity) {
     auto* const at = reinterpret_cast<unsigned long long*>(__cvta_shared_to_generic(bar));
-    bool ok = false;
-    for (int i = 0; i < 64 && !ok; ++i) ok = mbar_test_wait(at, parity);
-    if (!ok) {
-        const unsigned long long t0 = globaltimer();
-        for (;;) {
-            ok = mbar_try_wait(at, parity);
-            if (ok || *(volatile int*)&s->abort) break;
-            if (globaltimer() - t0 > kWaitNs) {
-                *(volatile int*)&s->abort = 1;
-                atomicExch(&g_paged_failed, 1);
-                break;
-            }
+    const unsigned long long t0 = globaltimer();
+    bool ok;
+    // (try_wait suspends the warp: what asks again and again takes issue slots from the softmax)
+    while (!(ok = mbar_try_wait(at, parity)) && !*(volatile int*)&s->abort) {
+        if (globaltimer() - t0 > kWaitNs) {
+            *(volatile int*)&s->abort = 1;
+            atomicExch(&g_paged_failed, 1);
+            break;
         }
     }
     return __all_sync(0xffffffffu, ok);
@@ -572,7 +568,7 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
                         __syncwarp();
                     }
                 }
-                if (!edge) tmem_ld32(scol, va);                                // (under way meanwhile)
+
                 const float mx = max_3(m4[0], m4[1], max_3(m4[2], m4[2], m4[3])) * a.scale2;
                 // (a row that sees NaN or an infinite score has no result; said here, since what follows may lose it)
                 if (!(mx < -NEG_INF)) l = __int_as_float(0x7fffffff);
@@ -615,13 +611,10 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
                 };
                 if (!edge) {
 #pragma unroll 1
-                    for (int ch = 0; ch < 4; ch += 2) {
+                    for (int ch = 0; ch < 4; ++ch) {
+                        tmem_ld32(scol + ch * 32, va);
                         tmem_wait_ld();
-                        tmem_ld32(scol + ch * 32 + 32, vb);
                         weigh(ch, va, Const<false>{});
-                        tmem_wait_ld();
-                        if (ch == 0) tmem_ld32(scol + 64, va);
-                        weigh(ch + 1, vb, Const<false>{});
                     }
                 } else {
 #pragma unroll 1

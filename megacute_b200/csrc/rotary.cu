@@ -6,7 +6,7 @@
 // in fp32, rounded once.  Bound by memory: every element is read and written once, a position's table row once per row.
 // A thread owns 16 elements of a head (8 pairs: two 16-byte accesses of a 16-bit type, the same 8 table columns in both layouts) and
 // takes them through up to kHeads heads of the row, so that its cosines and sines are fetched once and its loads of all those heads are
-// under way together.  A block has up to eight rows; one warp per row finds the row's sequence, position and cache row.
+// under way together.  A block has up to eight rows; one warp per row finds the row's sequence, position and cache row while the elements come.
 #include "paged.cuh"
 
 namespace mk {
@@ -90,8 +90,32 @@ template <int DT, bool INTER, bool APPEND>
 __global__ void __launch_bounds__(kRotThreads) rotate_rows(const __grid_constant__ RotArgs a) {
     constexpr int ES = DT == DT_F32 ? 4 : 2;
     __shared__ int s_state[kRotRows], s_pos[kRotRows], s_row[kRotRows];
+    wait_for_previous_kernel();
     const int row0 = blockIdx.x * a.block_rows, rows = min(a.block_rows, a.batch.rows - row0);
     const int warp = threadIdx.x >> 5;
+    const int slots = a.head_dim >> 4, heads = APPEND ? a.heads + 2 * a.kv_heads : a.heads;
+    const int per_row = slots * a.groups, turned = APPEND ? a.heads + a.kv_heads : a.heads;
+    // what thread u of the rows' does: a row, 16 elements of a head, every groups-th head from `group` on
+    int u = threadIdx.x, row, slot, group, e0, e1;
+    bool turn;
+    Sixteen<ES> v[kHeads];
+    auto request = [&] {                              // its elements: asked for before it is known where they go
+        row = u / per_row;
+        const int at = u - row * per_row;
+        slot = at % slots;
+        group = at / slots;
+        turn = slot < a.columns >> 3;
+        // the two vectors' first elements in a head
+        e0 = turn && !INTER ? slot * 8 : slot * 16;
+        e1 = turn && !INTER ? a.columns + slot * 8 : slot * 16 + 8;
+        const uint8_t* x = a.x + (row0 + row) * a.ld_x * ES;
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+            const int h = group + i * a.groups;
+            if (h < heads) load16(v[i], x + (h * a.head_dim + e0) * ES, x + (h * a.head_dim + e1) * ES);
+        }
+    };
+    if (u < rows * per_row) request();
     if (warp < rows) {
         const int r = row0 + warp, s = sequence_of_row(a.batch, r);
         int state = ROW_NONE, cache_row = -1;
@@ -114,23 +138,11 @@ __global__ void __launch_bounds__(kRotThreads) rotate_rows(const __grid_constant
         }
     }
     __syncthreads();
-    const int slots = a.head_dim >> 4, heads = APPEND ? a.heads + 2 * a.kv_heads : a.heads;
-    const int per_row = slots * a.groups, turned = APPEND ? a.heads + a.kv_heads : a.heads;
-    for (int u = threadIdx.x; u < rows * per_row; u += kRotThreads) {
-        const int row = u / per_row, at = u - row * per_row, slot = at % slots, group = at / slots;
+    for (; u < rows * per_row; u += kRotThreads) {
+        if (u >= kRotThreads) request();
         const int state = s_state[row];
         if (state == ROW_NONE) continue;
         const long long r = row0 + row;
-        const bool turn = slot < a.columns >> 3;
-        // the two vectors' first elements in a head
-        const int e0 = turn && !INTER ? slot * 8 : slot * 16, e1 = turn && !INTER ? a.columns + slot * 8 : slot * 16 + 8;
-        const uint8_t* x = a.x + r * a.ld_x * ES;
-        Sixteen<ES> v[kHeads];
-#pragma unroll
-        for (int i = 0; i < kHeads; ++i) {
-            const int h = group + i * a.groups;
-            if (h < heads) load16(v[i], x + (h * a.head_dim + e0) * ES, x + (h * a.head_dim + e1) * ES);
-        }
         float c[8], s[8];
         if (turn && state == ROW_TURN) {
             table8(a.cos, a.tdtype, s_pos[row] * a.ld_cos + slot * 8, c);
@@ -183,6 +195,11 @@ int launch(RotArgs& a, int dtype, bool inter, bool append, void* stream) {
     cfg.gridDim = dim3((unsigned)((a.batch.rows + a.block_rows - 1) / a.block_rows));
     cfg.blockDim = dim3(kRotThreads);
     cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute pdl;
+    pdl.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    pdl.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &pdl;
+    cfg.numAttrs = 1;
     cudaError_t e;
 #define MK_ROT(DT, APPEND) e = inter ? cudaLaunchKernelEx(&cfg, rotate_rows<DT, true, APPEND>, a) : cudaLaunchKernelEx(&cfg, rotate_rows<DT, false, APPEND>, a)
     if (append) {
