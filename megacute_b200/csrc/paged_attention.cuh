@@ -234,53 +234,82 @@ __device__ __forceinline__ Shares plan(const AttnArgs& a, PlanScratch<THREADS>* 
 }
 
 // Joins `count` parts of rows [row_begin, row_end) of an item, ROWS of them: part i has slot(i).  With M the largest of their maxima m_i
-//   l = sum_i 2^(m_i - M) l_i,   o = sum_i 2^(m_i - M) o_i,   in the order of i.
-// A thread has eight columns of a row; where that leaves threads over they share a row's parts and add through shared memory.  All threads of the block
-// call it.  write(row, column, l, o) takes eight columns.
+//   l = sum_i 2^(m_i - M) l_i,   o = sum_i 2^(m_i - M) o_i,   always in the same order.
+// A thread has eight columns of a row; where that leaves threads over they share a row's parts and add through shared memory.  What a thread waits for
+// is memory, so it asks for kAtOnce parts together.  All threads of the block call it.  write(row, column, l, o) takes eight columns.
 template <int D, int ROWS, int THREADS>
 struct Join {
-    static constexpr int kTasks = ROWS * (D / 8), kSplits = THREADS / kTasks;
+    static constexpr int kTasks = ROWS * (D / 8), kSplits = THREADS / kTasks, kAtOnce = 4;
     static_assert(kSplits * kTasks == THREADS, "threads of a join");
-    float4 o[kSplits > 1 ? 2 * THREADS : 1];
-    float l[kSplits > 1 ? THREADS : 1];
+    float o[kSplits > 1 ? 8 : 1][kSplits > 1 ? THREADS : 1];
+    float m[kSplits > 1 ? THREADS : 1], l[kSplits > 1 ? THREADS : 1];
+
+    static __device__ __forceinline__ float factor(float m, float to) { return m == to ? 1.f : ex2(m - to); }      // (-inf: 0, unless both are)
 
     template <class Slot, class Write>
     __device__ __forceinline__ void run(const AttnArgs& a, int count, int row_begin, int row_end, Slot slot, Write write) {
+        constexpr float NEG_INF = -__builtin_huge_valf();
         const int t = threadIdx.x, split = t / kTasks, row = row_begin + t % ROWS, col = t % kTasks / ROWS * 8;
         const bool mine = row < row_end;
-        float m = -__builtin_huge_valf(), sum = 0.f;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-        if (mine) {
-#pragma unroll 8
-            for (int i = 0; i < count; ++i) m = fmaxf(m, __ldcg(&a.stats[slot(i) * a.part_rows + row].x));
-#pragma unroll 4
-            for (int i = split; i < count; i += kSplits) {
-                const long long at = slot(i);
-                const float2 st = __ldcg(&a.stats[at * a.part_rows + row]);
-                const float4* const src = reinterpret_cast<const float4*>(a.part(at, D, row, col));
-                const float4 v = __ldcg(src), w = __ldcg(src + 1);
-                const float f = st.x == m ? 1.f : ex2(st.x - m);
-                if (st.x != -__builtin_huge_valf()) {                          // (a part that saw no key has nothing to add)
-                    sum += f * st.y;
-                    x.x += f * v.x; x.y += f * v.y; x.z += f * v.z; x.w += f * v.w;
-                    y.x += f * w.x; y.y += f * w.y; y.z += f * w.z; y.w += f * w.w;
+        float mx = NEG_INF, sum = 0.f, x[8] = {};
+        for (int i = split; mine && i < count; i += kSplits * kAtOnce) {
+            float2 st[kAtOnce];
+            float4 v[kAtOnce][2];
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                st[k] = make_float2(NEG_INF, 0.f);
+                v[k][0] = v[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i + k * kSplits < count) {
+                    const long long at = slot(i + k * kSplits);
+                    const float4* const src = reinterpret_cast<const float4*>(a.part(at, D, row, col));
+                    st[k] = __ldcg(&a.stats[at * a.part_rows + row]);
+                    v[k][0] = __ldcg(src);
+                    v[k][1] = __ldcg(src + 1);
                 }
+            }
+            float to = mx;
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) to = fmaxf(to, st[k].x);
+            if (to == NEG_INF) continue;              // (none of them saw a key)
+            const float f = factor(mx, to);
+            sum *= f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= f;
+            mx = to;
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                if (st[k].x == NEG_INF) continue;     // (nothing to add)
+                const float g = factor(st[k].x, to);
+                sum += g * st[k].y;
+                x[0] += g * v[k][0].x; x[1] += g * v[k][0].y; x[2] += g * v[k][0].z; x[3] += g * v[k][0].w;
+                x[4] += g * v[k][1].x; x[5] += g * v[k][1].y; x[6] += g * v[k][1].z; x[7] += g * v[k][1].w;
             }
         }
         if (kSplits > 1) {
-            o[t] = x;
-            o[THREADS + t] = y;
+            m[t] = mx;
             l[t] = sum;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e][t] = x[e];
             __syncthreads();
-            if (split > 0) return;
-            for (int k = 1; k < kSplits; ++k) {
-                const float4 v = o[t + k * kTasks], w = o[THREADS + t + k * kTasks];
-                sum += l[t + k * kTasks];
-                x.x += v.x; x.y += v.y; x.z += v.z; x.w += v.w;
-                y.x += w.x; y.y += w.y; y.z += w.z; y.w += w.w;
+            if (split > 0 || !mine) return;
+            float to = mx;
+            for (int k = 1; k < kSplits; ++k) to = fmaxf(to, m[t + k * kTasks]);
+            if (to != NEG_INF) {
+                const float f = factor(mx, to);
+                sum *= f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] *= f;
+                for (int k = 1; k < kSplits; ++k) {
+                    const int at = t + k * kTasks;
+                    if (m[at] == NEG_INF) continue;
+                    const float g = factor(m[at], to);
+                    sum += g * l[at];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] += g * o[e][at];
+                }
             }
         }
-        if (mine) write(row, col, sum, x, y);
+        if (mine) write(row, col, sum, make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]));
     }
 };
 

@@ -652,7 +652,7 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
             const bool sectors = ((uintptr_t)a.out & 31) == 0 && a.ld_out % 16 == 0;       // rows of the result start on 32-byte boundaries
             const uint32_t mem = items % kOddItems;
             const bool odd = (*(volatile int*)&sy->odd_any[mem][0] | *(volatile int*)&sy->odd_any[mem][1]) != 0;
-            if (mine && !whole) a.stats[slot * a.part_rows + part_row] = make_float2(l != l && m == NEG_INF ? 0.f : m, l);
+            if (mine && !whole) a.stats[slot * a.part_rows + part_row] = make_float2(l != l ? 0.f : m, l);       // (no result: a maximum that counts)
 #pragma unroll 1
             for (int ch = 0; ch < D / 16; ++ch) {
                 float o[16];

@@ -284,8 +284,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
 #pragma unroll
                 for (int n = 0; n < DN; ++n) *reinterpret_cast<uint32_t*>(to + n * 8) = pack16<DT>(o[n][2 * i] * inv, o[n][2 * i + 1] * inv);
             } else {
-                // (no score but NaN, which no maximum shows: a finite one, so that the part counts)
-                if ((lane & 3) == 0) stats[warp][u0 == 0 ? 1 : 0][row] = make_float2(l[i] != l[i] && m[i] == NEG_INF ? 0.f : m[i], l[i]);
+                // (no result: a maximum that counts)
+                if ((lane & 3) == 0) stats[warp][u0 == 0 ? 1 : 0][row] = make_float2(l[i] != l[i] ? 0.f : m[i], l[i]);
                 float* const to = (far ? own + (long long)worker * kFewRows * D : near) + row * D + pair;
 #pragma unroll
                 for (int n = 0; n < DN; ++n) *reinterpret_cast<float2*>(to + n * 8) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
