@@ -1,7 +1,7 @@
 // How attention over a paged cache is divided among workers, and what its kernels share.
 //
 // An item is up to `tokens` consecutive new tokens of one sequence and `group` query heads of one kv head: rows token * group + head of one
-// operand tile.  (Where more heads share a kv head than the tile has rows, `shared` such blocks of heads read it.)  Its keys are cut into units of 2^shift keys, aligned in the sequence.  All units of all items -- in the order
+// operand tile.  (Where more heads share a kv head than the tile has rows, `shared` such blocks of heads read it.)  Its keys are cut into units of 2^shift keys.  All units of all items -- in the order
 // sequence, block of heads, tokens -- make one list, which is dealt out evenly: each worker has the next N / W of them, the first N % W one
 // more.  Lengths are known on
 // the device only, so every block works out its part itself, and batches of the most unlike lengths load all SMs alike.
@@ -27,6 +27,7 @@ struct AttnArgs {
     int group_inverse;                                // 65536 / group + 1: row * group_inverse >> 16 is row / group for rows below 256
     float scale2;                                     // scale * log2(e)
     int tokens;                                       // new tokens of an item
+    int align;                                        // an item's first unit begins at a multiple of it, a power of two
     int workers, part_rows;                           // ... and rows of a part in the workspace
     __device__ __forceinline__ int token_of(int row) const { return row * group_inverse >> 16; }
     int4* joins;                                      // of each block: parts of the item that it begins and does not end (0: none), its first
@@ -40,7 +41,7 @@ struct AttnArgs {
 
 struct Item {
     int lo, hi;                                       // keys some token sees (lo > hi: none)
-    int first, units;                                 // units; at least one
+    int key0, units;                                  // first key of the first unit; units, at least one
 };
 
 // (the 64-bit division takes a few hundred cycles, and numbers above 2^32 are rare)
@@ -70,8 +71,8 @@ __device__ __forceinline__ Item item_at(const AttnArgs& a, long long p0, int tok
     Item it;
     it.hi = (int)min(max(p0 + tokens - 1, -1ll), cap - 1);
     it.lo = a.window > 0 ? (int)min(max(p0 + 1 - a.window, 0ll), cap) : 0;
-    it.first = it.hi < it.lo ? 0 : it.lo >> SHIFT;
-    it.units = it.hi < it.lo ? 1 : (it.hi >> SHIFT) - it.first + 1;
+    it.key0 = it.hi < it.lo ? 0 : it.lo & -a.align;
+    it.units = it.hi < it.lo ? 1 : ((it.hi - it.key0) >> SHIFT) + 1;
     return it;
 }
 

@@ -57,7 +57,7 @@ struct Sync {
     uint32_t tmem;
     int abort;
     uint32_t there[kSeen];                            // bit b: keys [16 b, 16 b + 16) of the tile are loaded
-    uint32_t odd[kOddItems][kOddTiles][4];            // keys of the item's n-th partial tile with values that are no numbers
+    uint32_t odd[kOddItems][2][kOddTiles][4];         // keys of the item's n-th partial tile with values that are no numbers, as either warp found them
     int odd_any[kOddItems][2];
 };
 
@@ -181,7 +181,7 @@ __device__ __forceinline__ Part part_of(const AttnArgs& a, const Walk<kShift>& w
     p.s = w.s;
     p.lo = w.item.lo;
     p.hi = w.item.hi;
-    p.key0 = (w.item.first + w.unit) << kShift;
+    p.key0 = w.item.key0 + (w.unit << kShift);
     p.units = (int)min((long long)(w.item.units - w.unit), w.left);
     p.tiles = p.tokens > a.tokens / 2 ? 2 : 1;
     p.begins = w.unit == 0;
@@ -423,7 +423,7 @@ __device__ __forceinline__ void value_role(const AttnArgs& a, uint8_t* smem, Syn
         seen_by_all(a, p, 0, p.tokens, lo_all, hi_all);
         const uint32_t mem = items % kOddItems;
         if (!warp_wait(sy, &sy->item_done[mem], ((items / kOddItems) & 1u) ^ 1u)) return;      // (the item that used it last has ended)
-        if (lane < kOddTiles * 2) sy->odd[mem][lane >> 1][half * 2 + (lane & 1)] = 0;
+        if (lane < kOddTiles * 4) sy->odd[mem][half][lane >> 2][lane & 3] = 0;
         if (lane == 0) sy->odd_any[mem][half] = 0;
         __syncwarp();
         for (int u = 0; u < p.units; ++u, ++c) {
@@ -433,41 +433,46 @@ __device__ __forceinline__ void value_role(const AttnArgs& a, uint8_t* smem, Syn
             const bool some = key0 < lo_all || key0 + 127 > hi_all;          // keys that some token does not see
             const uint32_t there = *(volatile uint32_t*)&sy->there[c % kSeen];
             if (some || there != 0xffu) {
-                const uint32_t tile = smem_u32(smem) + M::kRing + slot * M::kTile + half * 8192 + lane * 16;      // a warp has half of the rows
-                // rows 4 i + lane / 8 of the half: `none`: nobody sees them; `part`: some do
-                uint32_t none = 0, part = 0;
+                // a warp has every other four rows: 8 i + 4 half + lane / 8; the other lanes' pieces of 16 bytes
+                const int row0 = 4 * half + (lane >> 3);
+                const uint32_t tile = smem_u32(smem) + M::kRing + slot * M::kTile + row0 * 128 + (lane & 7) * 16;
+                uint32_t none = 0, part = 0;          // bit i: nobody sees the row; some do
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int row = half * 64 + 4 * i + (lane >> 3), key = key0 + row;
-                    const bool out = key < p.lo || key > p.hi || !((there >> (row >> 4)) & 1u);
+                    const int key = key0 + 8 * i + row0;
+                    const bool out = key < p.lo || key > p.hi || !((there >> (i >> 1)) & 1u);
                     none |= (uint32_t)out << i;
                     part |= (uint32_t)(!out && (key < lo_all || key > hi_all)) << i;
                 }
+                for (uint32_t rows = __reduce_or_sync(0xffffffffu, none); rows; rows &= rows - 1) {
+                    const int i = __ffs(rows) - 1;
+                    if ((none >> i) & 1u) {
+#pragma unroll
+                        for (int sub = 0; sub < M::kSubs; ++sub)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + sub * kSubBytes + i * 1024), "r"(0) : "memory");
+                    }
+                    __syncwarp();
+                }
                 uint32_t odd = 0;                     // top bit of each 16 bits: an exponent of all ones
                 constexpr uint32_t E = DT == DT_F16 ? 0x7c007c00u : 0x7f807f80u, ONE = DT == DT_F16 ? 0x04000400u : 0x00800080u;
+                for (uint32_t rows = __reduce_or_sync(0xffffffffu, part); rows; rows &= rows - 1) {
+                    const int i = __ffs(rows) - 1;
+                    if ((part >> i) & 1u) {
 #pragma unroll
-                for (int sub = 0; sub < M::kSubs; ++sub) {
+                        for (int sub = 0; sub < M::kSubs; ++sub) {
+                            uint32_t x[4];
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                                         : "r"(tile + sub * kSubBytes + i * 1024) : "memory");
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        asm volatile("{ .reg .pred p; setp.ne.u32 p, %2, 0; @p st.shared.v4.b32 [%0], {%1, %1, %1, %1}; }" ::"r"(tile + sub * kSubBytes + i * 512),
-                                     "r"(0), "r"(none & (1u << i))
-                                     : "memory");
-                    if (!__any_sync(0xffffffffu, part)) continue;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        uint32_t x[4] = {};
-                        asm volatile("{ .reg .pred p; setp.ne.u32 p, %5, 0; @p ld.shared.v4.b32 {%0, %1, %2, %3}, [%4]; }"
-                                     : "+r"(x[0]), "+r"(x[1]), "+r"(x[2]), "+r"(x[3])
-                                     : "r"(tile + sub * kSubBytes + i * 512), "r"(part & (1u << i))
-                                     : "memory");
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) odd |= (x[e] & E) + ONE;
+                            for (int e = 0; e < 4; ++e) odd |= (x[e] & E) + ONE;
+                        }
                     }
+                    __syncwarp();
                 }
                 if (__any_sync(0xffffffffu, odd & 0x80008000u) && partial < kOddTiles) {
                     for (int k = 0; k < 16 * M::kSubs; ++k) {
                         const int i = k & 15;
-                        const uint32_t at = tile + (k >> 4) * kSubBytes + i * 512;
+                        const uint32_t at = tile + (k >> 4) * kSubBytes + i * 1024;
                         if (!((part >> i) & 1u)) continue;
                         uint32_t x[4];
                         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
@@ -479,9 +484,9 @@ __device__ __forceinline__ void value_role(const AttnArgs& a, uint8_t* smem, Syn
                             x[e] &= (l ? 0u : 0xffffu) | (h ? 0u : 0xffff0000u);
                         }
                         if (any) {
-                            const int row = half * 64 + 4 * i + (lane >> 3);
+                            const int row = 8 * i + row0;
                             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
-                            atomicOr(&sy->odd[mem][partial][row >> 5], 1u << (row & 31));
+                            atomicOr(&sy->odd[mem][half][partial][row >> 5], 1u << (row & 31));
                             *(volatile int*)&sy->odd_any[mem][half] = 1;
                         }
                     }
@@ -654,15 +659,19 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
             const bool odd = (*(volatile int*)&sy->odd_any[mem][0] | *(volatile int*)&sy->odd_any[mem][1]) != 0;
             if (mine && !whole) a.stats[slot * a.part_rows + part_row] = make_float2(l != l ? 0.f : m, l);       // (no result: a maximum that counts)
 #pragma unroll 1
-            for (int ch = 0; ch < D / 16; ++ch) {
-                float o[16];
-                tc_ld16(ocol + ch * 16, o);
-                if (ch == D / 16 - 1) {
+            for (int ch = 0; ch < D; ch += 64) {
+                float o[64];
+                tmem_ld32(ocol + ch, o);
+                tmem_ld32(ocol + ch + 32, o + 32);
+                tmem_wait_ld();
+                use32(o);
+                use32(o + 32);
+                if (ch == D - 64) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sy->o_free[t]);
                 }
-                if (odd && mine) {                                                     // values that are no numbers, for the tokens that see them
+                if (odd && mine) {                                             // values that are no numbers, for the tokens that see them
                     int n = 0, alo, ahi;
                     seen_by_all(a, p, 0, p.tokens, alo, ahi);
                     for (int u = 0; u < p.units; ++u) {
@@ -670,12 +679,13 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
                         if (!(key0 < alo || key0 + 127 > ahi)) continue;
                         for (int r = 0; r < 128 && n < kOddTiles; ++r) {
                             const int key = key0 + r;
-                            if (!((*(volatile uint32_t*)&sy->odd[mem][n][r >> 5] >> (r & 31)) & 1u) || key < lo || key > hi) continue;
+                            const uint32_t bits = *(volatile uint32_t*)&sy->odd[mem][0][n][r >> 5] | *(volatile uint32_t*)&sy->odd[mem][1][n][r >> 5];
+                            if (!((bits >> (r & 31)) & 1u) || key < lo || key > hi) continue;
                             const int first = a.pages.page_row(p.s, key >> a.pages.shift);
                             if (first < 0) continue;
-                            const uint16_t* v = a.v + (long long)(first + (key & ((1 << a.pages.shift) - 1))) * a.ld_v + p.block / a.shared * D + ch * 16;
+                            const uint16_t* v = a.v + (long long)(first + (key & ((1 << a.pages.shift) - 1))) * a.ld_v + p.block / a.shared * D + ch;
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) {
+                            for (int e = 0; e < 64; ++e) {
                                 const uint32_t h = v[e];
                                 if (odd_value<DT>(h)) o[e] += unpack16<DT>(h).x;
                             }
@@ -684,17 +694,20 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
                     }
                 }
                 if (mine && whole) {
-                    uint32_t x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = pack16<DT>(o[2 * e] * inv, o[2 * e + 1] * inv);
-                    st32B(reinterpret_cast<uint8_t*>(to + ch * 16), x, sectors);
-                } else if (mine) {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
+                    for (int k = 0; k < 64; k += 16) {
                         uint32_t x[8];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) x[k] = __float_as_uint(o[8 * e + k]);
-                        st32B(reinterpret_cast<uint8_t*>(a.part(slot, D, part_row, ch * 16 + 8 * e)), x, true);
+                        for (int e = 0; e < 8; ++e) x[e] = pack16<DT>(o[k + 2 * e] * inv, o[k + 2 * e + 1] * inv);
+                        st32B(reinterpret_cast<uint8_t*>(to + ch + k), x, sectors);
+                    }
+                } else if (mine) {
+#pragma unroll
+                    for (int k = 0; k < 64; k += 8) {
+                        uint32_t x[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] = __float_as_uint(o[k + e]);
+                        st32B(reinterpret_cast<uint8_t*>(a.part(slot, D, part_row, ch + k)), x, true);
                     }
                 }
                 __syncwarp();

@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
         const int count = (int)min((long long)(w.item.units - u0), w.left), base_row = w.r0 + w.t, kv = w.kv, s = w.s;
         const Item it = w.item;
         const long long p0 = w.p + w.t;
-        const int first_key = (it.first + u0) << SHIFT;
+        const int first_key = it.key0 + (u0 << SHIFT);
         // keys that this thread's rows see
         int lo_r[2], hi_r[2];
 #pragma unroll
