@@ -146,6 +146,9 @@ extern "C" int mk_paged_attention(int device, const mk_batch* batch, const mk_pa
     a.parts = (float*)((uint8_t*)workspace + lay.parts);
     cudaStream_t st = (cudaStream_t)stream;
     a.tokens = few ? kFewRows / a.group : kChunkTile / a.group * 2;
+    a.begin_cost = few ? 0 : kChunkBegin;
+    a.unit_cost = few ? 1 : kChunkUnit;
+    a.half_cost = few ? 1 : kChunkHalf;
     a.align = few ? 16 : cache->page_size < kChunkTile ? cache->page_size : kChunkTile;
     float* const own = (float*)((uint8_t*)workspace + lay.own);
     cudaError_t e = few ? launch_few(a, own, D, cache->dtype, sms, st) : launch_chunk(a, cache, heads, st);

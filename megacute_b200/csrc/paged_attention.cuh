@@ -2,8 +2,8 @@
 //
 // An item is up to `tokens` consecutive new tokens of one sequence and `group` query heads of one kv head: rows token * group + head of one
 // operand tile.  (Where more heads share a kv head than the tile has rows, `shared` such blocks of heads read it.)  Its keys are cut into units of 2^shift keys.  All units of all items -- in the order
-// sequence, block of heads, tokens -- make one list, which is dealt out evenly: each worker has the next N / W of them, the first N % W one
-// more.  Lengths are known on
+// sequence, block of heads, tokens -- make one list, which is dealt out evenly by what they cost (Cost): each worker has the next N / W of the
+// list's whole cost N, the first N % W one more.  Lengths are known on
 // the device only, so every block works out its part itself, and batches of the most unlike lengths load all SMs alike.
 // A worker that has an item's units from the first to the last writes results.  Else it leaves the running maximum, the sum and the products of its
 // part in the workspace (slot 0: a part that does not begin the item; slot 1: one that begins it); a block joins the parts that its
@@ -27,6 +27,7 @@ struct AttnArgs {
     int group_inverse;                                // 65536 / group + 1: row * group_inverse >> 16 is row / group for rows below 256
     float scale2;                                     // scale * log2(e)
     int tokens;                                       // new tokens of an item
+    int begin_cost, unit_cost, half_cost;             // of an item: its beginning, a unit, a unit of an item of at most half as many tokens (Cost)
     int align;                                        // an item's first unit begins at a multiple of it, a power of two
     int workers, part_rows;                           // ... and rows of a part in the workspace
     __device__ __forceinline__ int token_of(int row) const { return row * group_inverse >> 16; }
@@ -48,20 +49,29 @@ struct Item {
 __device__ __forceinline__ long long divide(long long a, long long b) {
     return (unsigned long long)(a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
 }
-// Shares of the list of units.
+// Shares of the list's cost.
 struct Shares {
     long long total, per;
-    int workers, longer;                              // `longer` workers have per + 1 units, the others per
-    __device__ __forceinline__ Shares(long long units, int most, int least) {
-        total = units;
+    int workers, longer;                              // `longer` workers have per + 1, the others per
+    __device__ __forceinline__ Shares(long long cost, int most, int least) {
+        total = cost;
         workers = (int)min((long long)most, divide(total + least - 1, least));
         per = workers ? divide(total, workers) : 0;
         longer = (int)(total - per * workers);
     }
     __device__ __forceinline__ long long begin(int w) const { return w * per + min(w, longer); }
-    __device__ __forceinline__ int worker_of(long long unit) const {
+    __device__ __forceinline__ int worker_of(long long at) const {
         const long long border = (per + 1) * longer;
-        return (int)(unit < border ? divide(unit, per + 1) : longer + divide(unit - border, per));
+        return (int)(at < border ? divide(at, per + 1) : longer + divide(at - border, per));
+    }
+};
+
+// What an item costs: its beginning and end, and each of its units.  A place in the list of costs is the first unit whose end lies behind it.
+struct Cost {
+    int begin, unit;
+    __device__ __forceinline__ long long of(int units) const { return begin + (long long)units * unit; }
+    __device__ __forceinline__ int unit_at(long long at, int units) const {            // at: behind the item's beginning
+        return (int)min(max(divide(max(at - begin, 0ll) + unit - 1, unit), 0ll), (long long)units);
     }
 };
 
@@ -76,55 +86,73 @@ __device__ __forceinline__ Item item_at(const AttnArgs& a, long long p0, int tok
     return it;
 }
 
-// units of one block of heads of sequence s
 template <int SHIFT>
-__device__ __forceinline__ long long sequence_units(const AttnArgs& a, int s) {
+__device__ __forceinline__ Cost cost_of(const AttnArgs& a, int tokens) {
+    return Cost{a.begin_cost, tokens > a.tokens / 2 ? a.unit_cost : a.half_cost};
+}
+// cost of one block of heads of sequence s
+template <int SHIFT>
+__device__ __forceinline__ long long sequence_cost(const AttnArgs& a, int s) {
     const int r0 = a.batch.first(s), n = a.batch.count(s, r0);
     if (n == 0) return 0;
     const long long p = a.batch.position(s);
     long long sum = 0;
-    for (int t = 0; t < n; t += a.tokens) sum += item_at<SHIFT>(a, p + t, min(a.tokens, n - t)).units;
+    for (int t = 0; t < n; t += a.tokens) {
+        const int tokens = min(a.tokens, n - t);
+        sum += cost_of<SHIFT>(a, tokens).of(item_at<SHIFT>(a, p + t, tokens).units);
+    }
     return sum;
 }
 
-// Where a worker starts in the list.  Walks on from item to item.
+// A worker's way through the list, from item to item.
 template <int SHIFT>
 struct Walk {
     int s, kv, t;                                     // sequence, block of heads, first token of the item in the sequence
     int r0, n;                                        // rows of the sequence
     long long p;                                      // its position
-    int unit;                                         // next unit of the item
-    long long left;                                   // units that the worker still has, this item's among them
+    int unit, stop;                                   // the worker's units of the item
+    long long until;                                  // where the worker's share ends, from the item's beginning on
     Item item;
 
+    __device__ __forceinline__ bool live() const { return unit < stop; }
     __device__ __forceinline__ int item_tokens(const AttnArgs& a) const { return min(a.tokens, n - t); }
-    __device__ __forceinline__ void enter(const AttnArgs& a) { item = item_at<SHIFT>(a, p + t, item_tokens(a)); }
+    __device__ __forceinline__ Cost cost(const AttnArgs& a) const { return cost_of<SHIFT>(a, item_tokens(a)); }
+    // the share goes on behind this item
+    __device__ __forceinline__ bool goes_on(const AttnArgs& a) const { return until > cost(a).of(item.units); }
+    // place of the item's last unit, from its beginning on: whose share begins at or in front of it has that unit, or one in front
+    __device__ __forceinline__ long long last_unit(const AttnArgs& a) const { return cost(a).of(item.units - 1); }
     __device__ __forceinline__ void sequence(const AttnArgs& a, int seq) {
         s = seq;
         r0 = a.batch.first(s);
         n = a.batch.count(s, r0);
         p = a.batch.position(s);
     }
-    // to unit `at` of the sequence's list (of `per` units a block of heads)
-    __device__ __forceinline__ void start(const AttnArgs& a, int seq, long long at, long long per) {
+    __device__ __forceinline__ void enter(const AttnArgs& a, long long at) {
+        item = item_at<SHIFT>(a, p + t, item_tokens(a));
+        const Cost c = cost(a);
+        unit = at > 0 ? c.unit_at(at, item.units) : 0;
+        stop = until >= c.of(item.units) ? item.units : c.unit_at(until, item.units);
+    }
+    // to place `at` of the sequence's list (a block of heads costs `per`), with a share of `length`
+    __device__ __forceinline__ void start(const AttnArgs& a, int seq, long long at, long long per, long long length) {
         sequence(a, seq);
         kv = (int)divide(at, per);
         at -= kv * per;
-        t = 0;
-        enter(a);
-        while (at >= item.units && t + a.tokens < n) {
-            at -= item.units;
-            t += a.tokens;
-            enter(a);
+        for (t = 0;; t += a.tokens) {
+            const int tokens = item_tokens(a);
+            const long long c = cost_of<SHIFT>(a, tokens).of(item_at<SHIFT>(a, p + t, tokens).units);
+            if (at < c || t + a.tokens >= n) break;
+            at -= c;
         }
-        unit = (int)at;
+        until = at + length;
+        enter(a, at);
+        if (unit == item.units) next(a);              // (the share begins behind the item's last unit)
     }
-    // behind the units [unit, unit + count) of this item
-    __device__ __forceinline__ void next(const AttnArgs& a, int count) {
-        unit += count;
-        left -= count;
-        if (unit < item.units || left <= 0) return;
-        unit = 0;
+    // to the next item
+    __device__ __forceinline__ void next(const AttnArgs& a) {
+        until -= cost(a).of(item.units);
+        unit = stop = 0;
+        if (until <= 0) return;
         t += a.tokens;
         if (t >= n) {
             t = 0;
@@ -134,7 +162,7 @@ struct Walk {
                 while (n == 0 && s + 1 < a.batch.seqs);
             }
         }
-        enter(a);
+        enter(a, 0);
     }
 };
 
@@ -144,22 +172,22 @@ struct PlanScratch {
     long long ends[THREADS];                          // inclusive sums of a round's sequences
 };
 
-// Every thread of the block calls it with its warp's worker.  Returns how the units are dealt out, at least `least` to a worker; `walk` is set
-// where the warp's worker has some (walk.left > 0).
+// Every thread of the block calls it with its warp's worker.  Returns how the list is dealt out, at least `least` to a worker (no less than a
+// unit, so that a share inside an item has one); `walk` is at the worker's first unit, if it has any.
 template <int SHIFT, int THREADS>
 __device__ __forceinline__ Shares plan(const AttnArgs& a, PlanScratch<THREADS>* sc, int worker, int least, Walk<SHIFT>& walk) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     if (a.batch.seqs <= 128) {                        // a few sequences a lane: every warp by itself, in 32 bits
         const int each = (a.batch.seqs + 31) / 32;
-        int units[4], run = 0;
+        int cost[4], run = 0;
         bool big = false;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int s = lane * each + k;
-            long long u = k < each && s < a.batch.seqs ? sequence_units<SHIFT>(a, s) : 0;
-            big |= u > (1 << 23) / a.blocks;          // (128 of them stay below 2^30)
-            units[k] = (int)u * a.blocks;
-            run += units[k];
+            const long long c = k < each && s < a.batch.seqs ? sequence_cost<SHIFT>(a, s) : 0;
+            big |= c > (1 << 23) / a.blocks;          // (128 of them stay below 2^30)
+            cost[k] = (int)c * a.blocks;
+            run += cost[k];
         }
         if (!__any_sync(0xffffffffu, big)) {
 #pragma unroll
@@ -168,20 +196,20 @@ __device__ __forceinline__ Shares plan(const AttnArgs& a, PlanScratch<THREADS>* 
                 if (lane >= d) run += up;
             }
             const Shares shares(__shfl_sync(0xffffffffu, run, 31), a.workers, least);
-            const int begin = worker < shares.workers ? (int)shares.begin(worker) : (int)shares.total;
-            walk.left = worker < shares.workers ? shares.begin(worker + 1) - begin : 0;
-            if (walk.left > 0) {
+            walk.unit = walk.stop = 0;
+            if (worker < shares.workers) {
+                const int begin = (int)shares.begin(worker);
                 const int in = __popc(__ballot_sync(0xffffffffu, run <= begin));       // the lane that has it
-                int at = begin - (in > 0 ? __shfl_sync(0xffffffffu, run, in - 1) : 0), k = 0, n = 0;
+                int at = begin - (in > 0 ? __shfl_sync(0xffffffffu, run, in - 1) : 0), k = 0, c = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int u = __shfl_sync(0xffffffffu, units[i], in);
+                    const int u = __shfl_sync(0xffffffffu, cost[i], in);
                     if (k == i) {
-                        n = u;
+                        c = u;
                         if (at >= u) { at -= u; ++k; }
                     }
                 }
-                walk.start(a, in * each + k, at, n / a.blocks);
+                walk.start(a, in * each + k, at, c / a.blocks, shares.begin(worker + 1) - begin);
             }
             return shares;
         }
@@ -190,7 +218,7 @@ __device__ __forceinline__ Shares plan(const AttnArgs& a, PlanScratch<THREADS>* 
     long long mine = 0, sum = 0;
     for (int r = 0; r < rounds; ++r) {
         const int s = r * THREADS + t;
-        mine = s < a.batch.seqs ? sequence_units<SHIFT>(a, s) * a.blocks : 0;
+        mine = s < a.batch.seqs ? sequence_cost<SHIFT>(a, s) * a.blocks : 0;
         sum += mine;
     }
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -199,13 +227,14 @@ __device__ __forceinline__ Shares plan(const AttnArgs& a, PlanScratch<THREADS>* 
     long long total = 0;
     for (int w = 0; w < THREADS / 32; ++w) total += sc->sums[w];
     const Shares shares(total, a.workers, least);
-    const long long begin = worker < shares.workers ? shares.begin(worker) : total;
-    walk.left = worker < shares.workers ? shares.begin(worker + 1) - begin : 0;
+    const bool mine_too = worker < shares.workers;
+    const long long begin = mine_too ? shares.begin(worker) : total;
+    walk.unit = walk.stop = 0;
     long long base = 0;
     for (int r = 0; r < rounds; ++r) {
         if (rounds > 1) {
             const int s = r * THREADS + t;
-            mine = s < a.batch.seqs ? sequence_units<SHIFT>(a, s) * a.blocks : 0;
+            mine = s < a.batch.seqs ? sequence_cost<SHIFT>(a, s) * a.blocks : 0;
         }
         long long run = mine;
         for (int d = 1; d < 32; d <<= 1) {
@@ -222,12 +251,12 @@ __device__ __forceinline__ Shares plan(const AttnArgs& a, PlanScratch<THREADS>* 
         }
         sc->ends[t] = before + run;
         __syncthreads();
-        if (walk.left > 0 && begin >= base && begin < base + all) {
+        if (mine_too && begin >= base && begin < base + all) {
             int at = 0;                               // sequences of the round that end at or in front of `begin`
             for (int i = lane; i < THREADS; i += 32) at += sc->ends[i] <= begin;
             for (int d = 16; d; d >>= 1) at += __shfl_xor_sync(0xffffffffu, at, d);
             const long long first = at > 0 ? sc->ends[at - 1] : base;
-            walk.start(a, r * THREADS + at, begin - first, divide(sc->ends[at] - first, a.blocks));
+            walk.start(a, r * THREADS + at, begin - first, divide(sc->ends[at] - first, a.blocks), shares.begin(worker + 1) - begin);
         }
         base += all;
     }
@@ -330,6 +359,7 @@ cudaError_t launch_few(const AttnArgs& a, float* own /* [worker][kFewRows][head_
 
 // items of up to 256 rows, a positive scale (paged_attention_chunk.cu): two tiles of 128 rows, a worker per block
 constexpr int kChunkTile = 128;
+constexpr int kChunkBegin = 4, kChunkUnit = 3, kChunkHalf = 2;       // costs of an item's beginning and end, of a key tile with both and with one query tile
 cudaError_t launch_chunk(const AttnArgs& a, const mk_paged_cache* cache, int heads, cudaStream_t stream);
 cudaError_t chunk_status(int* failed, cudaStream_t stream);
 

@@ -182,10 +182,10 @@ __device__ __forceinline__ Part part_of(const AttnArgs& a, const Walk<kShift>& w
     p.lo = w.item.lo;
     p.hi = w.item.hi;
     p.key0 = w.item.key0 + (w.unit << kShift);
-    p.units = (int)min((long long)(w.item.units - w.unit), w.left);
+    p.units = w.stop - w.unit;
     p.tiles = p.tokens > a.tokens / 2 ? 2 : 1;
     p.begins = w.unit == 0;
-    p.ends = w.unit + p.units == w.item.units;
+    p.ends = w.stop == w.item.units;
     return p;
 }
 // keys that every token of [t0, t1) sees
@@ -205,7 +205,7 @@ __device__ __forceinline__ void load_role(const AttnArgs& a, const Maps& m, uint
     const uint32_t block_bits = (box == 128 ? 0xffu : (1u << (box >> 4)) - 1u);
     uint32_t c = 0, items = 0;                        // tiles and parts so far
     bool ok = true;
-    for (; w.left > 0 && ok; ++items) {
+    for (; w.live() && ok; ++items) {
         const Part p = part_of(a, w);
         const int kv = p.block / a.shared;
         ok = warp_wait(sy, &sy->q_free, (items & 1u) ^ 1u);
@@ -254,7 +254,7 @@ __device__ __forceinline__ void load_role(const AttnArgs& a, const Maps& m, uint
             }
             row = next;
         }
-        w.next(a, p.units);
+        w.next(a);
     }
     if (!ok) {                                        // copies that are under way land before the block's memory goes
         if (lane == 0) {
@@ -399,7 +399,7 @@ __device__ __forceinline__ void product_role(const AttnArgs& a, uint8_t* smem, S
     // MN-major: 8-key groups 1024 bytes apart (the descriptor's stride), sub-tiles of 64 columns 16 KB apart (its leading offset)
     p.vlo = D == 64 ? p.lo : p.lo - (1u << 16) + ((uint32_t)(kSubBytes >> 4) << 16);
     p.leader = elect_one();
-    while (w.left > 0) {
+    while (w.live()) {
         const Part part = part_of(a, w);
         const int units = __shfl_sync(0xffffffffu, part.units, 0), tiles = __shfl_sync(0xffffffffu, part.tiles, 0);
         if (!warp_wait(sy, &sy->q_full, p.items & 1u)) return;
@@ -407,7 +407,7 @@ __device__ __forceinline__ void product_role(const AttnArgs& a, uint8_t* smem, S
         ++p.items;
         ++p.outs[0];
         if (tiles == 2) ++p.outs[1];
-        w.next(a, part.units);
+        w.next(a);
     }
 }
 
@@ -417,7 +417,7 @@ __device__ __forceinline__ void value_role(const AttnArgs& a, uint8_t* smem, Syn
     using M = Map<D>;
     const int lane = threadIdx.x & 31, half = (threadIdx.x >> 5) & 1;
     uint32_t c = 0, items = 0;
-    for (; w.left > 0; ++items) {
+    for (; w.live(); ++items) {
         const Part p = part_of(a, w);
         int lo_all, hi_all, partial = 0;
         seen_by_all(a, p, 0, p.tokens, lo_all, hi_all);
@@ -497,7 +497,7 @@ __device__ __forceinline__ void value_role(const AttnArgs& a, uint8_t* smem, Syn
             }
             if (lane == 0) mbar_arrive(&sy->v_ready[c % kRingBars]);
         }
-        w.next(a, p.units);
+        w.next(a);
     }
 }
 
@@ -509,9 +509,8 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = warp >> 2, i = threadIdx.x & 127;     // tile and its row
     const int tile_tokens = a.tokens / 2, my_token = a.token_of(i), my_head = i - my_token * a.group;
     const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), ocol = tl + M::kO + D * t;
-    const long long end = shares.begin(worker + 1);
     uint32_t c = 0, items = 0, seq0 = 0, blocks = 0;
-    for (; w.left > 0; ++items) {
+    for (; w.live(); ++items) {
         const Part p = part_of(a, w);
         if (t < p.tiles) {
             const int token = t * tile_tokens + my_token;
@@ -650,8 +649,8 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
             const long long slot = (long long)worker * 2 + (p.begins ? 1 : 0);
             const float inv = l == 0.f ? 0.f : 1.f / l;
             if (p.begins && !p.ends && i == 0 && t == 0) {
-                const long long item_end = end + (w.item.units - p.units);     // (the item is not finished: the worker's last)
-                a.joins[worker] = make_int4(shares.worker_of(item_end - 1) - worker + 1, p.row0, p.tokens * a.group, p.block);
+                const long long last = shares.begin(worker + 1) - w.until + w.last_unit(a);
+                a.joins[worker] = make_int4(shares.worker_of(last) - worker + 1, p.row0, p.tokens * a.group, p.block);
             }
             uint16_t* const to = a.out + (long long)(p.row0 + token) * a.ld_out + (p.block * a.group + my_head) * D;
             const bool sectors = ((uintptr_t)a.out & 31) == 0 && a.ld_out % 16 == 0;       // rows of the result start on 32-byte boundaries
@@ -720,7 +719,7 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
         }
         seq0 += (uint32_t)(p.units * p.tiles);
         c += (uint32_t)p.units;
-        w.next(a, p.units);
+        w.next(a);
     }
 }
 
@@ -759,7 +758,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk(const __grid_co
     wait_for_previous_kernel();
     let_next_kernel_launch();
     Walk<kShift> w;
-    const Shares shares = plan<kShift, kChunkThreads>(a, reinterpret_cast<PlanScratch<kChunkThreads>*>(smem), worker, 1, w);
+    const Shares shares = plan<kShift, kChunkThreads>(a, reinterpret_cast<PlanScratch<kChunkThreads>*>(smem), worker, a.begin_cost + a.unit_cost, w);
     if (threadIdx.x == 0) a.joins[worker] = make_int4(0, 0, 0, 0);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");              // (copies go where the plan's sums were)
     tc_fence_before();

@@ -65,9 +65,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
     const uint32_t ring = smem_u32(smem) + warp * (kStagesFew * kUnitBytes);
     const int quad = lane >> 2, pair = (lane & 3) * 2;           // this thread's rows quad, quad + 8; columns pair, pair + 1 of each 8
 
-    while (w.left > 0) {
+    while (w.live()) {
         const int tokens = w.item_tokens(a), rows = tokens * a.group, u0 = w.unit;
-        const int count = (int)min((long long)(w.item.units - u0), w.left), base_row = w.r0 + w.t, kv = w.kv, s = w.s;
+        const int count = w.stop - u0, base_row = w.r0 + w.t, kv = w.kv, s = w.s;
         const Item it = w.item;
         const long long p0 = w.p + w.t;
         const int first_key = it.key0 + (u0 << SHIFT);
@@ -267,11 +267,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
         // ---- results, or this part's statistics and products
         const bool whole = u0 == 0 && count == it.units;
         // (the worker's last part has the ring to itself; one in front of others, of which there is one at most, goes to the workspace)
-        const bool far = w.left > count;
+        const bool far = w.goes_on(a);
         if (!whole && lane == 0) {
             // (an item that is begun and not finished is the worker's last)
             const bool ends = u0 + count == it.units;
-            const int last = ends || u0 > 0 ? 0 : shares.worker_of(shares.begin(worker + 1) + (it.units - count) - 1);
+            const int last = ends || u0 > 0 ? 0 : shares.worker_of(shares.begin(worker + 1) - w.until + w.last_unit(a));
             pieces[warp][u0 == 0 ? 1 : 0] = Piece{rows, base_row, kv, last, ends, far};
         }
 #pragma unroll
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
                 for (int n = 0; n < DN; ++n) *reinterpret_cast<float2*>(to + n * 8) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
             }
         }
-        w.next(a, count);
+        w.next(a);
     }
     // ---- the warps' parts of an item: results where the block has all of them, else a part of the block.
     // A run of parts is one, and slot 0 of the warps behind up to one that ends the item.  Its rows are dealt out to the warps, a quarter or half
