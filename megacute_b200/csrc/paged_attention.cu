@@ -145,7 +145,9 @@ extern "C" int mk_paged_attention(int device, const mk_batch* batch, const mk_pa
     a.stats = (float2*)((uint8_t*)workspace + lay.stats);
     a.parts = (float*)((uint8_t*)workspace + lay.parts);
     cudaStream_t st = (cudaStream_t)stream;
-    a.tokens = few ? kFewRows / a.group : kChunkTile / a.group * 2;
+    // (8 rows an item where these hold all new tokens: half of the matrix instruction's rows, and nothing is done for the others)
+    const int few_rows_of = (long long)max_new * a.group <= kFewRows / 2 ? kFewRows / 2 : kFewRows;
+    a.tokens = few ? few_rows_of / a.group : kChunkTile / a.group * 2;
     a.begin_cost = few ? 0 : kChunkBegin;
     a.unit_cost = few ? 1 : kChunkUnit;
     a.half_cost = few ? 1 : kChunkHalf;

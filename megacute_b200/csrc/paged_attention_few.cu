@@ -44,7 +44,8 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
     return (w & E) == E || ((w >> 16) & E) == E;
 }
 
-template <int DT, int D>
+// HALVES: 1 for items of at most 8 rows (the matrix instruction's other 8 are zeros, and nothing is done for them), else 2
+template <int DT, int D, int HALVES>
 __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_constant__ AttnArgs a, float* own) {
     constexpr int SHIFT = unit_shift<D>, U = 1 << SHIFT, NT = U / 8, KS = U / 16, DK = D / 16, DN = D / 8;
     constexpr int CH = D / 8, ROWS_PER_COPY = 32 / CH;          // 16-byte pieces of a row; rows that 32 lanes copy
@@ -72,9 +73,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
         const long long p0 = w.p + w.t;
         const int first_key = it.key0 + (u0 << SHIFT);
         // keys that this thread's rows see
-        int lo_r[2], hi_r[2];
+        int lo_r[HALVES], hi_r[HALVES];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < HALVES; ++i) {
             const long long p = p0 + a.token_of(quad + 8 * i);
             hi_r[i] = (int)min(max(p, -1ll), (long long)it.hi);
             lo_r[i] = a.window > 0 ? (int)min(max(p + 1 - a.window, 0ll), 0x7fffffffll) : 0;
@@ -96,9 +97,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
         hold(block0);
         // ---- Q fragments
         uint32_t q[DK][4];
-        long long row_at[2];                                     // element offset of this thread's two rows, -1: none
+        long long row_at[HALVES];                                // this thread's rows of the packed batch, -1: none
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int k = 0; k < DK; ++k) q[k][1] = q[k][3] = 0u;
+#pragma unroll
+        for (int i = 0; i < HALVES; ++i) {
             const int row = quad + 8 * i, tok = a.token_of(row);
             row_at[i] = row < rows ? (long long)(base_row + tok) : -1;
             const uint16_t* src = a.q + row_at[i] * a.ld_q + (kv * a.group + row - tok * a.group) * D + pair;
@@ -141,7 +144,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
         for (int i = 0; i < DN; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-        float m[2] = {NEG_INF, NEG_INF}, l[2] = {0.f, 0.f};
+        float m[HALVES], l[HALVES];
+#pragma unroll
+        for (int i = 0; i < HALVES; ++i) { m[i] = NEG_INF; l[i] = 0.f; }
         for (int u = 0; u < kStagesFew - 1; ++u) request(u);
         for (int u = 0; u < count; ++u) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kStagesFew - 2) : "memory");
@@ -164,55 +169,55 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
             }
             const bool partial = key0 < lo_all || key0 + U - 1 > hi_all;      // keys that some row does not see
             const uint32_t gone = (absent >> 2 * (u & 15)) & 3u;
-            float mx[2] = {NEG_INF, NEG_INF};
+            float mx[HALVES];
+#pragma unroll
+            for (int i = 0; i < HALVES; ++i) mx[i] = NEG_INF;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sc[n][e] *= a.scale2;
+                for (int e = 0; e < 2 * HALVES; ++e) sc[n][e] *= a.scale2;
                 if (partial || gone) {
                     const bool here = !((gone >> (n / 2)) & 1u);
                     const int key = key0 + n * 8 + pair;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
+                    for (int e = 0; e < 2 * HALVES; ++e) {
                         const int j = key + (e & 1);
                         if (!here || j < lo_r[e >> 1] || j > hi_r[e >> 1]) sc[n][e] = NEG_INF;
                     }
                 }
-                mx[0] = fmaxf(mx[0], fmaxf(sc[n][0], sc[n][1]));
-                mx[1] = fmaxf(mx[1], fmaxf(sc[n][2], sc[n][3]));
-            }
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < HALVES; ++i) mx[i] = fmaxf(mx[i], fmaxf(sc[n][2 * i], sc[n][2 * i + 1]));
+            }
+            bool raise = false;
+#pragma unroll
+            for (int i = 0; i < HALVES; ++i) {
                 mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
                 mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+                raise |= mx[i] > m[i] + kRaise || (m[i] == NEG_INF && mx[i] > NEG_INF);
             }
-            const bool raise = mx[0] > m[0] + kRaise || (m[0] == NEG_INF && mx[0] > NEG_INF) || mx[1] > m[1] + kRaise ||
-                               (m[1] == NEG_INF && mx[1] > NEG_INF);
             if (__any_sync(0xffffffffu, raise)) {
-                float f[2];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float to = fmaxf(m[i], mx[i]);
-                    f[i] = m[i] == NEG_INF ? 0.f : ex2(m[i] - to);
+                for (int i = 0; i < HALVES; ++i) {
+                    const float to = fmaxf(m[i], mx[i]), f = m[i] == NEG_INF ? 0.f : ex2(m[i] - to);
                     m[i] = to;
-                    l[i] *= f[i];
-                }
+                    l[i] *= f;
 #pragma unroll
-                for (int i = 0; i < DN; ++i) {
-                    o[i][0] *= f[0]; o[i][1] *= f[0];
-                    o[i][2] *= f[1]; o[i][3] *= f[1];
+                    for (int n = 0; n < DN; ++n) {
+                        o[n][2 * i] *= f;
+                        o[n][2 * i + 1] *= f;
+                    }
                 }
             }
-            const float off[2] = {m[0] == NEG_INF ? 0.f : m[0], m[1] == NEG_INF ? 0.f : m[1]};     // (no key so far: every score is -inf)
-            uint32_t p[KS][4];
+            uint32_t p[KS][4] = {};
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
+            for (int i = 0; i < HALVES; ++i) {
+                const float off = m[i] == NEG_INF ? 0.f : m[i];   // (no key so far: every score is -inf)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sc[n][e] = ex2(sc[n][e] - off[e >> 1]);
-                l[0] += sc[n][0] + sc[n][1];
-                l[1] += sc[n][2] + sc[n][3];
-                p[n >> 1][(n & 1) * 2] = pack16<DT>(sc[n][0], sc[n][1]);
-                p[n >> 1][(n & 1) * 2 + 1] = pack16<DT>(sc[n][2], sc[n][3]);
+                for (int n = 0; n < NT; ++n) {
+                    const float a0 = ex2(sc[n][2 * i] - off), a1 = ex2(sc[n][2 * i + 1] - off);
+                    l[i] += a0 + a1;
+                    p[n >> 1][(n & 1) * 2 + i] = pack16<DT>(a0, a1);
+                }
             }
             // a value that is no number must not reach the tokens that do not see its key through 0 * it
             bool odd = false;
@@ -240,7 +245,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
                         const long long at = p0 + t;
                         const int hi = (int)min(max(at, -1ll), (long long)it.hi);
                         const int lo = a.window > 0 ? (int)min(max(at + 1 - a.window, 0ll), 0x7fffffffll) : 0;
-                        const bool r0 = a.token_of(quad) == t, r1 = a.token_of(quad + 8) == t;
+                        const bool r0 = a.token_of(quad) == t, r1 = HALVES == 2 && a.token_of(quad + 8) == t;
                         uint32_t bt[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
@@ -260,7 +265,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncwarp();                                            // the ring is free for the next part
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < HALVES; ++i) {
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
         }
@@ -275,7 +280,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
             pieces[warp][u0 == 0 ? 1 : 0] = Piece{rows, base_row, kv, last, ends, far};
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < HALVES; ++i) {
             const int row = quad + 8 * i;
             if (row >= rows) continue;
             if (whole) {
@@ -341,11 +346,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
     }
 }
 
-template <int DT, int D>
+template <int DT, int D, int HALVES>
 cudaError_t launch(const AttnArgs& a, float* own, int blocks, cudaStream_t stream) {
     constexpr int bytes = kFewWarps * kStagesFew * kUnitBytes;
     static SharedMemory allowed;
-    const cudaError_t e = allowed.allow((const void*)attend_few<DT, D>, bytes);
+    const cudaError_t e = allowed.allow((const void*)attend_few<DT, D, HALVES>, bytes);
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute pdl;
     pdl.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -357,7 +362,12 @@ cudaError_t launch(const AttnArgs& a, float* own, int blocks, cudaStream_t strea
     cfg.stream = stream;
     cfg.attrs = &pdl;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attend_few<DT, D>, a, own);
+    return cudaLaunchKernelEx(&cfg, attend_few<DT, D, HALVES>, a, own);
+}
+
+template <int DT, int D>
+cudaError_t launch(const AttnArgs& a, float* own, int blocks, cudaStream_t stream) {
+    return a.tokens * a.group <= 8 ? launch<DT, D, 1>(a, own, blocks, stream) : launch<DT, D, 2>(a, own, blocks, stream);
 }
 
 }  // namespace
