@@ -148,9 +148,6 @@ extern "C" int mk_paged_attention(int device, const mk_batch* batch, const mk_pa
     // (8 rows an item where these hold all new tokens: half of the matrix instruction's rows, and nothing is done for the others)
     const int few_rows_of = (long long)max_new * a.group <= kFewRows / 2 ? kFewRows / 2 : kFewRows;
     a.tokens = few ? few_rows_of / a.group : kChunkTile / a.group * 2;
-    a.begin_cost = few ? 0 : kChunkBegin;
-    a.unit_cost = few ? 1 : kChunkUnit;
-    a.half_cost = few ? 1 : kChunkHalf;
     a.align = few ? 16 : cache->page_size < kChunkTile ? cache->page_size : kChunkTile;
     float* const own = (float*)((uint8_t*)workspace + lay.own);
     cudaError_t e = few ? launch_few(a, own, D, cache->dtype, sms, st) : launch_chunk(a, cache, heads, st);

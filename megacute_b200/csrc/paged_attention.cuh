@@ -27,7 +27,6 @@ struct AttnArgs {
     int group_inverse;                                // 65536 / group + 1: row * group_inverse >> 16 is row / group for rows below 256
     float scale2;                                     // scale * log2(e)
     int tokens;                                       // new tokens of an item
-    int begin_cost, unit_cost, half_cost;             // of an item: its beginning, a unit, a unit of an item of at most half as many tokens (Cost)
     int align;                                        // an item's first unit begins at a multiple of it, a power of two
     int workers, part_rows;                           // ... and rows of a part in the workspace
     __device__ __forceinline__ int token_of(int row) const { return row * group_inverse >> 16; }
@@ -66,11 +65,15 @@ struct Shares {
     }
 };
 
+// Costs of the chunk kernel: an item's beginning and end, a key tile with both query tiles, with one.
+constexpr int kChunkBegin = 4, kChunkUnit = 3, kChunkHalf = 2;
+
 // What an item costs: its beginning and end, and each of its units.  A place in the list of costs is the first unit whose end lies behind it.
 struct Cost {
     int begin, unit;
     __device__ __forceinline__ long long of(int units) const { return begin + (long long)units * unit; }
-    __device__ __forceinline__ int unit_at(long long at, int units) const {            // at: behind the item's beginning
+    __device__ __forceinline__ int unit_at(long long at, int units) const {            // at: from the item's beginning on
+        if (unit == 1) return (int)min(max(at - begin, 0ll), (long long)units);
         return (int)min(max(divide(max(at - begin, 0ll) + unit - 1, unit), 0ll), (long long)units);
     }
 };
@@ -88,7 +91,8 @@ __device__ __forceinline__ Item item_at(const AttnArgs& a, long long p0, int tok
 
 template <int SHIFT>
 __device__ __forceinline__ Cost cost_of(const AttnArgs& a, int tokens) {
-    return Cost{a.begin_cost, tokens > a.tokens / 2 ? a.unit_cost : a.half_cost};
+    if (SHIFT < 7) return Cost{0, 1};                 // (few rows: a unit is a unit)
+    return Cost{kChunkBegin, tokens > a.tokens / 2 ? kChunkUnit : kChunkHalf};
 }
 // cost of one block of heads of sequence s
 template <int SHIFT>
@@ -359,7 +363,6 @@ cudaError_t launch_few(const AttnArgs& a, float* own /* [worker][kFewRows][head_
 
 // items of up to 256 rows, a positive scale (paged_attention_chunk.cu): two tiles of 128 rows, a worker per block
 constexpr int kChunkTile = 128;
-constexpr int kChunkBegin = 4, kChunkUnit = 3, kChunkHalf = 2;       // costs of an item's beginning and end, of a key tile with both and with one query tile
 cudaError_t launch_chunk(const AttnArgs& a, const mk_paged_cache* cache, int heads, cudaStream_t stream);
 cudaError_t chunk_status(int* failed, cudaStream_t stream);
 

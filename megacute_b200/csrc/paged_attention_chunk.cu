@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk(const __grid_co
     wait_for_previous_kernel();
     let_next_kernel_launch();
     Walk<kShift> w;
-    const Shares shares = plan<kShift, kChunkThreads>(a, reinterpret_cast<PlanScratch<kChunkThreads>*>(smem), worker, a.begin_cost + a.unit_cost, w);
+    const Shares shares = plan<kShift, kChunkThreads>(a, reinterpret_cast<PlanScratch<kChunkThreads>*>(smem), worker, kChunkBegin + kChunkUnit, w);
     if (threadIdx.x == 0) a.joins[worker] = make_int4(0, 0, 0, 0);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");              // (copies go where the plan's sums were)
     tc_fence_before();

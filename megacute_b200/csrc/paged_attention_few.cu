@@ -323,18 +323,36 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
             const int row = r + lane / LANES, col = lane % LANES * 4;
             if ((turn & (kFewWarps - 1)) != warp || row >= head.rows) continue;
             float m = NEG_INF, l = 0.f;
-            for (int i = 0; i < n; ++i) m = fmaxf(m, stats[first + i][i ? 0 : begins][row].x);
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int i = 0; i < n; ++i) {
-                const int k = first + i, sl = i ? 0 : begins;
-                const float2 st = stats[k][sl][row];
-                if (st.x == NEG_INF) continue;                   // (it saw no key)
-                const float f = st.x == m ? 1.f : ex2(st.x - m);
-                const float* const src = pieces[k][sl].far ? own + (long long)(blockIdx.x * kFewWarps + k) * kFewRows * D
-                                                           : reinterpret_cast<const float*>(smem + k * (kStagesFew * kUnitBytes));
-                const float4 v = *reinterpret_cast<const float4*>(src + row * D + col);
-                l += f * st.y;
-                o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
+            for (int i0 = 0; i0 < n; i0 += 4) {                  // four parts asked for together
+                float2 st[4];
+                float4 v[4];
+                float to = m;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    st[i] = make_float2(NEG_INF, 0.f);
+                    v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (i0 + i < n) {
+                        const int k = first + i0 + i, sl = i0 + i ? 0 : begins;
+                        st[i] = stats[k][sl][row];
+                        const float* const src = pieces[k][sl].far ? own + (long long)(blockIdx.x * kFewWarps + k) * kFewRows * D
+                                                                   : reinterpret_cast<const float*>(smem + k * (kStagesFew * kUnitBytes));
+                        v[i] = *reinterpret_cast<const float4*>(src + row * D + col);
+                    }
+                    to = fmaxf(to, st[i].x);
+                }
+                if (to == NEG_INF) continue;                     // (they saw no key)
+                const float f = m == to ? 1.f : ex2(m - to);
+                l *= f;
+                o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+                m = to;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (st[i].x == NEG_INF) continue;
+                    const float g = st[i].x == to ? 1.f : ex2(st[i].x - to);
+                    l += g * st[i].y;
+                    o.x += g * v[i].x; o.y += g * v[i].y; o.z += g * v[i].z; o.w += g * v[i].w;
+                }
             }
             if (done) {
                 write_result<DT, D>(a, head.row0, head.block, row, col, l, o);
