@@ -299,8 +299,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
         w.next(a);
     }
     // ---- the warps' parts of an item: results where the block has all of them, else a part of the block.
-    // A run of parts is one, and slot 0 of the warps behind up to one that ends the item.  Its rows are dealt out to the warps, a quarter or half
-    // a row's columns to a thread: l = sum_i 2^(m_i - M) l_i and the like for o, in the order of the warps.
+    // A run of parts is one, and slot 0 of the warps behind up to one that ends the item.  Its rows are dealt out to the warps, eight columns to a
+    // thread: l = sum_i 2^(m_i - M) l_i and the like for o, in the order of the warps.
     __syncthreads();
     const int from = (lane >> 1) & (kFewWarps - 1), slot = lane & 1;
     int count = 0;
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
         ends = pieces[from][slot].ends;
         while (!ends && from + count < kFewWarps && pieces[from + count][0].rows > 0) ends = pieces[from + count++][0].ends;
     }
-    constexpr int LANES = D / 4, ROWS = 32 / LANES;               // threads of a row; rows of a warp at a time
+    constexpr int LANES = D / 8, ROWS = 32 / LANES;               // threads of a row; rows of a warp at a time
     int turn = 0;
     for (uint32_t runs = __ballot_sync(0xffffffffu, count > 0); runs; runs &= runs - 1) {
         const int at = __ffs(runs) - 1, n = __shfl_sync(0xffffffffu, count, at), first = at >> 1, begins = at & 1;
@@ -320,45 +320,55 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
         if (begins && !done && threadIdx.x == 0)
             a.joins[blockIdx.x] = make_int4(head.last / kFewWarps - (int)blockIdx.x + 1, head.row0, head.rows, head.block);
         for (int r = 0; r < head.rows; r += ROWS, ++turn) {
-            const int row = r + lane / LANES, col = lane % LANES * 4;
+            const int row = r + lane / LANES, col = lane % LANES * 8;
             if ((turn & (kFewWarps - 1)) != warp || row >= head.rows) continue;
             float m = NEG_INF, l = 0.f;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            float4 o[2] = {};
             for (int i0 = 0; i0 < n; i0 += 4) {                  // four parts asked for together
                 float2 st[4];
-                float4 v[4];
+                float4 v[4][2];
                 float to = m;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     st[i] = make_float2(NEG_INF, 0.f);
-                    v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    v[i][0] = v[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (i0 + i < n) {
                         const int k = first + i0 + i, sl = i0 + i ? 0 : begins;
                         st[i] = stats[k][sl][row];
                         const float* const src = pieces[k][sl].far ? own + (long long)(blockIdx.x * kFewWarps + k) * kFewRows * D
                                                                    : reinterpret_cast<const float*>(smem + k * (kStagesFew * kUnitBytes));
-                        v[i] = *reinterpret_cast<const float4*>(src + row * D + col);
+                        v[i][0] = reinterpret_cast<const float4*>(src + row * D + col)[0];
+                        v[i][1] = reinterpret_cast<const float4*>(src + row * D + col)[1];
                     }
                     to = fmaxf(to, st[i].x);
                 }
                 if (to == NEG_INF) continue;                     // (they saw no key)
                 const float f = m == to ? 1.f : ex2(m - to);
                 l *= f;
-                o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    o[e].x *= f; o[e].y *= f; o[e].z *= f; o[e].w *= f;
+                }
                 m = to;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     if (st[i].x == NEG_INF) continue;
                     const float g = st[i].x == to ? 1.f : ex2(st[i].x - to);
                     l += g * st[i].y;
-                    o.x += g * v[i].x; o.y += g * v[i].y; o.z += g * v[i].z; o.w += g * v[i].w;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        o[e].x += g * v[i][e].x; o[e].y += g * v[i][e].y; o[e].z += g * v[i][e].z; o[e].w += g * v[i][e].w;
+                    }
                 }
             }
             if (done) {
-                write_result<DT, D>(a, head.row0, head.block, row, col, l, o);
+                write_result<DT, D>(a, head.row0, head.block, row, col, l, o[0]);
+                write_result<DT, D>(a, head.row0, head.block, row, col + 4, l, o[1]);
             } else {
                 if (col == 0) a.stats[to * kFewRows + row] = make_float2(m, l);
-                *reinterpret_cast<float4*>(a.part(to, D, row, col)) = o;
+                float4* const at = reinterpret_cast<float4*>(a.part(to, D, row, col));
+                at[0] = o[0];
+                at[1] = o[1];
             }
         }
     }
