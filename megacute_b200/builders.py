@@ -68,6 +68,26 @@ def llama_stack(B: int, S: int, E: int, H: int, KVH: int, F: int, n: int, eps: f
     return g
 
 
+def llama_between_attentions(M: int, E: int, H: int, KVH: int, F: int, n: int, i: int, vocab: int, eps: float = 1e-6) -> Graph:
+    """What a prompt's M tokens go through between the attentions of layers i - 1 and i, for callers that attend outside a launch
+    (``paged_append``, ``paged_attention``): the rest of layer i - 1 behind its attention ``a`` -- or, for i = 0, the embedding of ``ids`` --,
+    then norm and QKV projection of layer i.  Returns the residual stream x (M, E), fp32 between launches as it is inside one, and
+    the projection (M, (H + 2 KVH) * D)."""
+    D = E // H
+    g = Graph()
+    layer = _stacked(g, llama_param_shapes(E, H, KVH, F), n)
+    x = g.temp((M, E), name="x_out", dtype=torch.float32)
+    if i == 0:
+        g.gather(g.param("lm_head", (vocab, E)), g.input("ids", (M, 1), torch.int32), out=x)
+    else:
+        p = layer(i - 1)
+        h = g.linear(g.input("a", (M, E)), p["wo"], residual=g.input("x", (M, E), torch.float32), out=g.temp((M, E), dtype=torch.float32))
+        g.linear(g.linear(g.rms_norm(h, p["mlp_norm"], eps), p["wgu"], act="swiglu"), p["wd"], residual=h, out=x)
+    p = layer(i)
+    g.output(x, g.linear(g.rms_norm(x, p["attn_norm"], eps), p["wqkv"]))
+    return g
+
+
 def llama_decode(B: int, E: int, H: int, KVH: int, F: int, n: int, max_seq: int, vocab: int | None = None,
                  eps: float = 1e-6, fused_step: bool = False, ragged: bool = False, window: int | None = None) -> Graph:
     """One decode step for B sequences.  States: x (B, E) embedded tokens, pos (1, 1) int32,

@@ -22,7 +22,7 @@ import pathlib
 
 import torch
 
-from .builders import llama_decode
+from .builders import llama_between_attentions, llama_decode
 from .graph import swiglu_weight
 
 BF = torch.bfloat16
@@ -98,9 +98,12 @@ class LlamaGenerator:
     The decode graph is built with ``fused_step=True``: the token ids live on the device, the launch
     gathers their embedding rows and overwrites them with the argmax of its logits, so the loop below
     is nothing but launches (the reference's loop wraps its launch in index_select / copy_ / argmax,
-    examples/llama/llama1b.py:103-121).  The prompt goes through the same program one token per step."""
+    examples/llama/llama1b.py:103-121).  The prompt goes through the same program one token per step, or, with ``prompt_chunk`` = c, c tokens at
+    a time as far as they go (``prefill``): the layers' linears as launches of their own, new keys and values into the same
+    cache with ``paged_append``, attention with ``paged_attention`` (the cache's rows of a sequence are pages that lie one behind the other).
+    Those launches keep packed copies of the weights, so device memory for the model doubles."""
 
-    def __init__(self, cfg: dict, sd: dict, batch: int = 1, max_seq: int = 1024, device=None, **compile_kw):
+    def __init__(self, cfg: dict, sd: dict, batch: int = 1, max_seq: int = 1024, device=None, prompt_chunk: int | None = None, **compile_kw):
         import megacute_b200 as mc
         self.cfg, self.batch, self.max_seq = cfg, batch, max_seq
         s = llama_shapes(cfg)
@@ -116,6 +119,42 @@ class LlamaGenerator:
                           k_cache=torch.zeros(s["n"] * batch * max_seq, kvd, dtype=BF, device=self.device),
                           v_cache=torch.zeros(s["n"] * batch * max_seq, kvd, dtype=BF, device=self.device))
         self.inputs = dict(cos=cos, sin=sin)
+        self.prompt_chunk, self._between = int(prompt_chunk or 0), None
+        if self.prompt_chunk < 0:
+            raise ValueError("prompt_chunk is a number of tokens")
+        self._compile_kw = compile_kw
+
+    def prefill(self, tokens: list[int]) -> int:
+        """Feed whole chunks of ``prompt_chunk`` tokens (the same for every sequence of the batch) into the cache, and return how many tokens these
+        are; the rest is for ``step``.  Nothing is sampled."""
+        import megacute_b200 as mc
+        c, b = self.prompt_chunk, self.batch
+        whole = len(tokens) // c * c if c else 0
+        if whole == 0:
+            return 0
+        if int(self.state["pos"]) + whole > self.max_seq:
+            raise ValueError("prompt exceeds max_seq")
+        s = llama_shapes(self.cfg)
+        n, d = s["n"], s["E"] // s["H"]
+        if self._between is None:                       # programs and page table of the first prompt serve all
+            dims = (s["E"], s["H"], s["KVH"], s["F"], n)
+            self._between = [mc.compile(llama_between_attentions(b * c, *dims, i, s["vocab"], s["eps"]), **self._compile_kw) for i in range(n)]
+            self._pages = torch.arange(b * self.max_seq // 128, dtype=torch.int32, device=self.device).view(b, -1)
+        kw = dict(heads=s["H"], kv_heads=s["KVH"], head_dim=d, page_size=128)
+        cos, sin = (t[:, :d // 2] for t in self.inputs.values())
+        pos, rows = self.state["pos"].expand(b, 1), b * self.max_seq
+        for at in range(0, whole, c):
+            ids = torch.tensor(tokens[at:at + c], dtype=torch.int32, device=self.device).repeat(b).view(-1, 1)
+            x = a = None
+            for i, prog in enumerate(self._between):
+                bound = {f.name for f in prog.g.inputs + prog.g.params}
+                x, qkv = prog(**{k: t for k, t in dict(self.params, ids=ids, x=x, a=a).items() if k in bound})
+                k, v = (self.state[name][i * rows:(i + 1) * rows] for name in ("k_cache", "v_cache"))
+                q = mc.paged_append(qkv, cos, sin, pos, k, v, self._pages, **kw)
+                if i + 1 < n:                           # (behind the last layer's keys and values nothing is asked for)
+                    a = mc.paged_attention(q, k, v, pos, self._pages, **kw)
+            self.state["pos"] += c
+        return whole
 
     def step(self):
         """One decode step: consumes ``state['ids']`` at ``state['pos']``, leaves the greedy tokens in ``ids``.
@@ -130,7 +169,7 @@ class LlamaGenerator:
             raise ValueError("empty prompt")
         if int(self.state["pos"]) + len(prompt) + n_tokens > self.max_seq:
             raise ValueError("prompt + generated tokens exceed max_seq")
-        for tok in prompt[:-1]:                         # the tokens the model is told, not asked
+        for tok in prompt[self.prefill(prompt[:-1]):-1]:        # the tokens the model is told, not asked
             self.state["ids"].fill_(int(tok))
             self.step()
         self.state["ids"].fill_(int(prompt[-1]))
@@ -164,9 +203,10 @@ def main(argv=None):
     ap.add_argument("--tokens", type=int, default=128)
     ap.add_argument("--batch", type=int, default=1)
     ap.add_argument("--max-seq", type=int, default=1024)
+    ap.add_argument("--prompt-chunk", type=int, default=0, help="prompt tokens that go through the model together (0: one per step)")
     a = ap.parse_args(argv)
     cfg, sd = load_local(a.model)
-    gen = LlamaGenerator(cfg, sd, a.batch, a.max_seq)
+    gen = LlamaGenerator(cfg, sd, a.batch, a.max_seq, prompt_chunk=a.prompt_chunk)
     prompt = [int(x) for x in a.prompt_ids.split(",")]
     torch.cuda.synchronize()
     t0 = time.time()

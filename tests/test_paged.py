@@ -696,3 +696,35 @@ def test_abi_refusals():
     # nothing to do: nothing is launched
     none = B(rows=0)
     assert attention(none) == append(none) == rotary(none) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,chunk", [(2, 16), (1, 3), (3, 64)])
+def test_generator_prompt_in_chunks(cuda, batch, chunk):
+    """LlamaGenerator feeding its prompt in chunks: the cache afterwards is that of the token-by-token prompt (both bf16, from
+    activations rounded at other places), and the logits behind it are those of the plain forward pass."""
+    from megacute_b200.checkpoint import LlamaGenerator, rope_tables_from_config
+    from tests.helpers import TOL, rel_l2
+    from tests.test_checkpoint import CFG, hf_forward, hf_state_dict
+    sd = hf_state_dict(CFG, seed=5)
+    prompt = torch.randint(0, CFG["vocab_size"], (71,), generator=gen(4)).tolist()
+    one = LlamaGenerator(CFG, sd, batch=batch, max_seq=128, device=cuda)
+    many = LlamaGenerator(CFG, sd, batch=batch, max_seq=128, device=cuda, prompt_chunk=chunk)
+    fed = many.prefill(prompt[:-1])
+    assert fed == 70 // chunk * chunk == int(many.state["pos"])
+    for g, start in ((one, 0), (many, fed)):
+        for tok in prompt[start:]:
+            g.state["ids"].fill_(tok)
+            logits = g.step()
+        g.logits = logits.float().cpu()
+    for name in ("k_cache", "v_cache"):
+        a, b = (g.state[name].view(CFG["num_hidden_layers"], batch, 128, -1) for g in (one, many))
+        assert rel_l2(b[:, :, :71].float().cpu(), a[:, :, :71].float().cpu()) < TOL and (b[:, :, 71:] == 0).all()
+    cos, sin = rope_tables_from_config(CFG, 128)
+    want = hf_forward(CFG, sd, prompt, cos, sin)[-1]
+    for g in (one, many):
+        assert rel_l2(g.logits[0], want) < TOL
+    again = LlamaGenerator(CFG, sd, batch=batch, max_seq=128, device=cuda, prompt_chunk=chunk)
+    assert again.generate(prompt, 5).shape == (batch, 5) and int(again.state["pos"]) == 75
+    with pytest.raises(ValueError):
+        again.prefill(prompt[:64])
