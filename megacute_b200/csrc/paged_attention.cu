@@ -126,8 +126,9 @@ extern "C" int mk_paged_attention(int device, const mk_batch* batch, const mk_pa
     a.batch = batch_of(batch);
     a.pages = pages_of(cache);
     a.q = (const uint16_t*)q;
-    a.k = (const uint16_t*)cache->k;
-    a.v = (const uint16_t*)cache->v;
+    // (without pages no row is read; the addresses are ones of this call all the same)
+    a.k = (const uint16_t*)(cache->pages ? cache->k : q);
+    a.v = (const uint16_t*)(cache->pages ? cache->v : q);
     a.out = (uint16_t*)out;
     a.ld_q = ld_q;
     a.ld_k = cache->ld_k;

@@ -339,6 +339,25 @@ def test_paged_attention_absent_pages(cuda, D, dtype, new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("rows,width", [(0, 3), (64, 0), (0, 0)])
+def test_paged_attention_no_pages(cuda, new, rows, width):
+    """A cache without pages, a page table without columns: nobody sees anything, nothing is appended."""
+    q = torch.randn(2 * new, 256, generator=gen(1)).to(BF)
+    args = dict(q=q, k_cache=torch.ones(rows, 128, dtype=BF), v_cache=torch.ones(rows, 128, dtype=BF), pos=torch.tensor([[5], [0]], dtype=torch.int32),
+                pages=torch.zeros(2, width, dtype=torch.int32), starts=None)
+    kw = dict(heads=4, kv_heads=2, head_dim=64, page_size=16)
+    got = mc.paged_attention(**on(cuda, args), **kw)
+    assert (got == 0).all()
+    cos, sin = tables(64, 32)
+    qkv = torch.randn(2 * new, 512, generator=gen(2)).to(BF)
+    a = on(cuda, {k: v for k, v in args.items() if k != "q"})
+    out = mc.paged_append(qkv.to(cuda), cos.to(cuda), sin.to(cuda), **a, **kw)
+    want = ref.paged_append(qkv, cos, sin, **{k: v for k, v in args.items() if k != "q"}, **kw)[0]
+    assert float((out.cpu().double() - want).abs().max()) < 0.02 and (a["k_cache"] == 1).all() and (a["v_cache"] == 1).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [2, 4, 9, 140])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
@@ -424,12 +443,16 @@ def test_paged_attention_far_rows(cuda):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("new,seqs,ctx", [(1, 1, 5000), (1, 70, 300), (3, 2, 2500), (200, 1, 3000), (33, 40, 100), (16, 16, 1500)])
-def test_paged_attention_repeats(cuda, new, seqs, ctx):
+@pytest.mark.parametrize("new,seqs,ctx", [(1, 1, 5000), (1, 70, 300), (3, 2, 2500), (200, 1, 3000), (33, 40, 100), (16, 16, 1500), (1, 900, 40),
+                                          (2, 900, 60)])
+@pytest.mark.parametrize("hint", [False, True])
+def test_paged_attention_repeats(cuda, new, seqs, ctx, hint):
     """Long and many sequences, against 64-bit torch on the GPU; a second call gives the same bits, on another stream beside other calls too."""
     H, KVH, D, page = 8, 2, 64, 32
     args, kw = make_attention([max(0, ctx - 13 * i) for i in range(seqs)], [new] * seqs, H, KVH, D, page, BF, seed=seqs)
     a = on(cuda, args)
+    if hint:
+        kw["max_new"] = new
     got = mc.paged_attention(**a, **kw)
     for s in range(0, seqs, max(1, seqs // 7)):
         p, b0 = int(args["pos"][s, 0]), int(args["starts"][s])
