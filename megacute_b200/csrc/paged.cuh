@@ -52,7 +52,7 @@ inline const char* cache_error(const mk_paged_cache* c) {
     if (c->dtype != DT_BF16 && c->dtype != DT_F16) return "paged cache: bf16 or fp16";
     if (c->page_size < 16 || (c->page_size & (c->page_size - 1))) return "paged cache: page_size is a power of two from 16 up";
     if ((long long)c->pages * c->page_size > 0x7fffffffll) return "paged cache: at most 2^31 - 1 rows";
-    if ((long long)c->table_cols * c->page_size > 0x7fffffffll) return "paged cache: a sequence has at most 2^31 - 1 rows";
+    if ((long long)c->table_cols * c->page_size > 0x7fff0000ll) return "paged cache: a sequence has at most 2^31 - 65536 rows";
     if (c->table_ld < 0) return "paged cache: table_ld is not negative";
     const long long width = (long long)c->kv_heads * c->head_dim;
     if (c->kv_heads <= 0 || c->head_dim <= 0 || c->ld_k < width || c->ld_v < width) return "paged cache: rows hold kv_heads heads";

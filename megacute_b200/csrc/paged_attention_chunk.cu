@@ -35,7 +35,7 @@ constexpr int kTileRows = 128;
 constexpr int kSubBytes = kTileRows * 128;            // 64 columns of a tile of 128 rows
 constexpr int kSeen = 32;                             // entries of the ring of tile descriptions, far more than tiles in flight
 constexpr int kRingBars = 8;                          // barriers of key tiles, more than tiles in the ring
-constexpr int kOddItems = 4, kOddTiles = 8;           // items, and tiles of an item, whose odd values are remembered
+constexpr int kOddTiles = 6;                          // tiles of an item that some tokens see in part: at most three at either end
 
 template <int D> struct Map {
     static constexpr int kSubs = D / 64;
@@ -46,6 +46,40 @@ template <int D> struct Map {
     static constexpr uint32_t kO = kScores * 128;     // ... then O of tile 0 and of tile 1
 };
 
+// What the block does to one item.  The loader finds it and tells the other roles through a short ring in shared memory.
+struct Part {
+    int tokens, row0, block, s;                       // its tokens, first row of the packed batch, block of heads, sequence
+    int lo, hi;                                       // keys some token sees
+    int first_lo, first_hi;                           // keys the first token sees, the next one's are one further (saturated far outside of what there is)
+    int key0, units, tiles;                           // first key of the part; key tiles (0: no more items); query tiles
+    int whole;                                        // bit 0: it begins the item, bit 1: it ends it
+};
+constexpr int kShift = 7;
+constexpr int kParts = 4;                             // entries of the ring
+__device__ __forceinline__ int saturated(long long x) { return (int)min(max(x, -0x7fff0000ll), 0x7fffff00ll); }
+__device__ __forceinline__ Part part_of(const AttnArgs& a, const Walk<kShift>& w) {
+    Part p;
+    p.tokens = w.item_tokens(a);
+    p.row0 = w.r0 + w.t;
+    p.block = w.kv;
+    p.s = w.s;
+    p.lo = w.item.lo;
+    p.hi = w.item.hi;
+    p.first_hi = saturated(w.p + w.t);
+    p.first_lo = a.window > 0 ? saturated(w.p + w.t + 1 - a.window) : -0x7fff0000;
+    p.key0 = w.item.key0 + (w.unit << kShift);
+    p.units = w.stop - w.unit;
+    p.tiles = p.tokens > a.tokens / 2 ? 2 : 1;
+    p.whole = (w.unit == 0 ? 1 : 0) | (w.stop == w.item.units ? 2 : 0);
+    return p;
+}
+// keys that every token of [t0, t1) sees
+__device__ __forceinline__ void seen_by_all(const Part& p, int t0, int t1, int& lo, int& hi) {
+    hi = min(p.first_hi + t0, p.hi);
+    lo = max(p.first_lo + t1 - 1, 0);
+}
+__device__ __forceinline__ void seen_by(const Part& p, int token, int& lo, int& hi) { seen_by_all(p, token, token + 1, lo, hi); }
+
 struct Sync {
     // (by parity a wait only tells a phase from the one in front of it: a barrier's phases are all waited for by the same threads, one after the
     // other, or the one in front is known to be over)
@@ -53,12 +87,13 @@ struct Sync {
     unsigned long long k_full[kRingBars], v_full[kRingBars], v_ready[kRingBars];           // key tile c: c % kRingBars
     unsigned long long slot_free[10];                 // slots of the ring of tiles
     unsigned long long s_full[2][4], p_full[2][4], pv_done[2][4];                          // tile t's k-th block of scores: k % 4
-    unsigned long long o_free[2], item_done[kOddItems];
+    unsigned long long o_free[2], part_full[kParts], part_free[kParts];
     uint32_t tmem;
     int abort;
     uint32_t there[kSeen];                            // bit b: keys [16 b, 16 b + 16) of the tile are loaded
-    uint32_t odd[kOddItems][2][kOddTiles][4];         // keys of the item's n-th partial tile with values that are no numbers, as either warp found them
-    int odd_any[kOddItems][2];
+    uint32_t odd[kParts][kOddTiles][4];               // keys of the item's n-th partial tile with values that are no numbers
+    int odd_any[kParts];
+    Part part[kParts];
 };
 
 // All lanes of a warp wait for one phase.  Asked once in line; the rest, with the limit, is a call, so that the roles' loops stay short.
@@ -79,6 +114,17 @@ __device__ __noinline__ bool wait_longer(Sync* s, uint32_t bar, uint32_t parity)
 __device__ __forceinline__ bool warp_wait(Sync* s, unsigned long long* bar, uint32_t parity) {
     if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
     return wait_longer(s, smem_u32(bar), parity);
+}
+// The next item: all lanes of a warp of a role other than the loader.  False: there is none, or a wait gave up.
+__device__ __forceinline__ bool next_part(Sync* s, uint32_t items, Part& p) {
+    if (!warp_wait(s, &s->part_full[items % kParts], (items / kParts) & 1u)) return false;
+    p = s->part[items % kParts];
+    return p.units > 0;
+}
+// ... and done with it
+__device__ __forceinline__ void done_part(Sync* s, uint32_t items) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&s->part_free[items % kParts]);
 }
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* m, int x, int y, unsigned long long* bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(m),
@@ -164,40 +210,9 @@ struct Maps {
     CUtensorMap q, k, v;
 };
 
-// What one worker does to one item, as every role sees it.
-struct Part {
-    long long p0;                                     // position of the item's first token
-    int tokens, row0, block, s;                       // its tokens, first row of the packed batch, block of heads, sequence
-    int lo, hi, key0, units, tiles;                   // keys some token sees; first key of the part; key tiles; query tiles
-    bool begins, ends;
-};
-constexpr int kShift = 7;
-__device__ __forceinline__ Part part_of(const AttnArgs& a, const Walk<kShift>& w) {
-    Part p;
-    p.p0 = w.p + w.t;
-    p.tokens = w.item_tokens(a);
-    p.row0 = w.r0 + w.t;
-    p.block = w.kv;
-    p.s = w.s;
-    p.lo = w.item.lo;
-    p.hi = w.item.hi;
-    p.key0 = w.item.key0 + (w.unit << kShift);
-    p.units = w.stop - w.unit;
-    p.tiles = p.tokens > a.tokens / 2 ? 2 : 1;
-    p.begins = w.unit == 0;
-    p.ends = w.stop == w.item.units;
-    return p;
-}
-// keys that every token of [t0, t1) sees
-__device__ __forceinline__ void seen_by_all(const AttnArgs& a, const Part& p, int t0, int t1, int& lo, int& hi) {
-    hi = (int)min(max(p.p0 + t0, -1ll), (long long)p.hi);
-    lo = a.window > 0 ? (int)min(max(p.p0 + t1 - a.window, 0ll), 0x7fffffffll) : 0;
-}
-__device__ __forceinline__ void seen_by(const AttnArgs& a, const Part& p, int token, int& lo, int& hi) { seen_by_all(a, p, token, token + 1, lo, hi); }
-
 // ---- loader -------------------------------------------------------------------------------------------------------------------
 template <int D>
-__device__ __forceinline__ void load_role(const AttnArgs& a, const Maps& m, uint8_t* smem, Sync* sy, Walk<kShift> w) {
+__device__ __forceinline__ void load_role(const AttnArgs& a, const Maps& m, uint8_t* smem, Sync* sy, Walk<kShift> w, int worker, const Shares& shares) {
     using M = Map<D>;
     const int lane = threadIdx.x & 31;
     const int box = min(1 << a.pages.shift, kTileRows), boxes = kTileRows / box, tile_tokens = a.tokens / 2;
@@ -205,8 +220,26 @@ __device__ __forceinline__ void load_role(const AttnArgs& a, const Maps& m, uint
     const uint32_t block_bits = (box == 128 ? 0xffu : (1u << (box >> 4)) - 1u);
     uint32_t c = 0, items = 0;                        // tiles and parts so far
     bool ok = true;
-    for (; w.live() && ok; ++items) {
-        const Part p = part_of(a, w);
+    if (lane == 0) a.joins[worker] = make_int4(0, 0, 0, 0);
+    for (;; ++items) {
+        Part p;
+        p.units = 0;
+        if (w.live()) p = part_of(a, w);
+        // (every role has done with the item that had the entry before)
+        ok = warp_wait(sy, &sy->part_free[items % kParts], ((items / kParts) & 1u) ^ 1u);
+        if (!ok) break;
+        if (lane < kOddTiles * 4) sy->odd[items % kParts][lane >> 2][lane & 3] = 0;
+        __syncwarp();
+        if (lane == 0) {
+            sy->odd_any[items % kParts] = 0;
+            sy->part[items % kParts] = p;
+            mbar_arrive(&sy->part_full[items % kParts]);
+            if (p.units > 0 && p.whole == 1) {        // (an item that is begun and not finished is the block's last)
+                const long long last = shares.begin(worker + 1) - w.until + w.last_unit(a);
+                a.joins[worker] = make_int4(shares.worker_of(last) - worker + 1, p.row0, p.tokens * a.group, p.block);
+            }
+        }
+        if (p.units == 0) break;
         const int kv = p.block / a.shared;
         ok = warp_wait(sy, &sy->q_free, (items & 1u) ^ 1u);
         if (!ok) break;
@@ -254,6 +287,7 @@ __device__ __forceinline__ void load_role(const AttnArgs& a, const Maps& m, uint
             }
             row = next;
         }
+        if (!ok) break;
         w.next(a);
     }
     if (!ok) {                                        // copies that are under way land before the block's memory goes
@@ -389,7 +423,7 @@ struct Products {
     }
 };
 template <int DT, int D>
-__device__ __forceinline__ void product_role(const AttnArgs& a, uint8_t* smem, Sync* sy, Walk<kShift> w, uint32_t tmem) {
+__device__ __forceinline__ void product_role(uint8_t* smem, Sync* sy, uint32_t tmem) {
     const uint64_t d0 = tc_smem_desc(smem_u32(smem));
     Products<DT, D> p;
     p.sy = sy;
@@ -399,33 +433,28 @@ __device__ __forceinline__ void product_role(const AttnArgs& a, uint8_t* smem, S
     // MN-major: 8-key groups 1024 bytes apart (the descriptor's stride), sub-tiles of 64 columns 16 KB apart (its leading offset)
     p.vlo = D == 64 ? p.lo : p.lo - (1u << 16) + ((uint32_t)(kSubBytes >> 4) << 16);
     p.leader = elect_one();
-    while (w.live()) {
-        const Part part = part_of(a, w);
+    Part part;
+    for (; next_part(sy, p.items, part); ++p.items) {
         const int units = __shfl_sync(0xffffffffu, part.units, 0), tiles = __shfl_sync(0xffffffffu, part.tiles, 0);
         if (!warp_wait(sy, &sy->q_full, p.items & 1u)) return;
         if (!(tiles == 2 ? p.two(units) : p.one(units))) return;
-        ++p.items;
         ++p.outs[0];
         if (tiles == 2) ++p.outs[1];
-        w.next(a);
+        done_part(sy, p.items);
     }
 }
 
 // ---- values -------------------------------------------------------------------------------------------------------------------
 template <int DT, int D>
-__device__ __forceinline__ void value_role(const AttnArgs& a, uint8_t* smem, Sync* sy, Walk<kShift> w) {
+__device__ __forceinline__ void value_role(uint8_t* smem, Sync* sy) {
     using M = Map<D>;
     const int lane = threadIdx.x & 31, half = (threadIdx.x >> 5) & 1;
-    uint32_t c = 0, items = 0;
-    for (; w.live(); ++items) {
-        const Part p = part_of(a, w);
+    uint32_t c = 0;
+    Part p;
+    for (uint32_t items = 0; next_part(sy, items, p); ++items) {
         int lo_all, hi_all, partial = 0;
-        seen_by_all(a, p, 0, p.tokens, lo_all, hi_all);
-        const uint32_t mem = items % kOddItems;
-        if (!warp_wait(sy, &sy->item_done[mem], ((items / kOddItems) & 1u) ^ 1u)) return;      // (the item that used it last has ended)
-        if (lane < kOddTiles * 4) sy->odd[mem][half][lane >> 2][lane & 3] = 0;
-        if (lane == 0) sy->odd_any[mem][half] = 0;
-        __syncwarp();
+        seen_by_all(p, 0, p.tokens, lo_all, hi_all);
+        const uint32_t mem = items % kParts;
         for (int u = 0; u < p.units; ++u, ++c) {
             const uint32_t slot = (2 * c + 1) % M::kSlots;
             if (!warp_wait(sy, &sy->v_full[c % kRingBars], (c / kRingBars) & 1u)) return;
@@ -486,8 +515,8 @@ __device__ __forceinline__ void value_role(const AttnArgs& a, uint8_t* smem, Syn
                         if (any) {
                             const int row = 8 * i + row0;
                             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
-                            atomicOr(&sy->odd[mem][half][partial][row >> 5], 1u << (row & 31));
-                            *(volatile int*)&sy->odd_any[mem][half] = 1;
+                            atomicOr(&sy->odd[mem][partial][row >> 5], 1u << (row & 31));
+                            *(volatile int*)&sy->odd_any[mem] = 1;
                         }
                     }
                 }
@@ -497,30 +526,30 @@ __device__ __forceinline__ void value_role(const AttnArgs& a, uint8_t* smem, Syn
             }
             if (lane == 0) mbar_arrive(&sy->v_ready[c % kRingBars]);
         }
-        w.next(a);
+        done_part(sy, items);
     }
 }
 
 // ---- softmax ------------------------------------------------------------------------------------------------------------------
 template <int DT, int D>
-__device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<kShift> w, uint32_t tmem, int worker, const Shares& shares) {
+__device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, uint32_t tmem, int worker) {
     using M = Map<D>;
     constexpr float NEG_INF = -__builtin_huge_valf();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = warp >> 2, i = threadIdx.x & 127;     // tile and its row
     const int tile_tokens = a.tokens / 2, my_token = a.token_of(i), my_head = i - my_token * a.group;
     const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), ocol = tl + M::kO + D * t;
-    uint32_t c = 0, items = 0, seq0 = 0, blocks = 0;
-    for (; w.live(); ++items) {
-        const Part p = part_of(a, w);
+    uint32_t c = 0, seq0 = 0, blocks = 0;
+    Part p;
+    for (uint32_t items = 0; next_part(sy, items, p); ++items) {
         if (t < p.tiles) {
             const int token = t * tile_tokens + my_token;
             const bool mine = my_token < tile_tokens && token < p.tokens;
             int lo, hi, lo_all, hi_all, lo_any, hi_any, unused;               // keys that this row, every row, some row of the tile sees
-            seen_by(a, p, min(token, p.tokens - 1), lo, hi);
+            seen_by(p, min(token, p.tokens - 1), lo, hi);
             const int last = min(p.tokens, (t + 1) * tile_tokens);
-            seen_by_all(a, p, t * tile_tokens, last, lo_all, hi_all);
-            seen_by(a, p, t * tile_tokens, lo_any, unused);
-            seen_by(a, p, last - 1, unused, hi_any);
+            seen_by_all(p, t * tile_tokens, last, lo_all, hi_all);
+            seen_by(p, t * tile_tokens, lo_any, unused);
+            seen_by(p, last - 1, unused, hi_any);
             float m = NEG_INF, l = 0.f;
             for (int u = 0; u < p.units; ++u) {
                 const uint32_t n = seq0 + (uint32_t)(u * p.tiles + t), buf = n % M::kScores;
@@ -644,18 +673,14 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
             // ---- results, or this part's statistics and products
             if (!warp_wait(sy, &sy->pv_done[t][(blocks - 1u) & 3u], ((blocks - 1u) >> 2) & 1u)) return;
             tc_fence_after();
-            const bool whole = p.begins && p.ends;
+            const bool whole = p.whole == 3;
             const int part_row = token * a.group + my_head;
-            const long long slot = (long long)worker * 2 + (p.begins ? 1 : 0);
+            const long long slot = (long long)worker * 2 + (p.whole & 1);
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            if (p.begins && !p.ends && i == 0 && t == 0) {
-                const long long last = shares.begin(worker + 1) - w.until + w.last_unit(a);
-                a.joins[worker] = make_int4(shares.worker_of(last) - worker + 1, p.row0, p.tokens * a.group, p.block);
-            }
             uint16_t* const to = a.out + (long long)(p.row0 + token) * a.ld_out + (p.block * a.group + my_head) * D;
             const bool sectors = ((uintptr_t)a.out & 31) == 0 && a.ld_out % 16 == 0;       // rows of the result start on 32-byte boundaries
-            const uint32_t mem = items % kOddItems;
-            const bool odd = (*(volatile int*)&sy->odd_any[mem][0] | *(volatile int*)&sy->odd_any[mem][1]) != 0;
+            const uint32_t mem = items % kParts;
+            const bool odd = *(volatile int*)&sy->odd_any[mem] != 0;
             if (mine && !whole) a.stats[slot * a.part_rows + part_row] = make_float2(l != l ? 0.f : m, l);       // (no result: a maximum that counts)
 #pragma unroll 1
             for (int ch = 0; ch < D; ch += 64) {
@@ -672,13 +697,13 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
                 }
                 if (odd && mine) {                                             // values that are no numbers, for the tokens that see them
                     int n = 0, alo, ahi;
-                    seen_by_all(a, p, 0, p.tokens, alo, ahi);
+                    seen_by_all(p, 0, p.tokens, alo, ahi);
                     for (int u = 0; u < p.units; ++u) {
                         const int key0 = p.key0 + (u << kShift);
                         if (!(key0 < alo || key0 + 127 > ahi)) continue;
                         for (int r = 0; r < 128 && n < kOddTiles; ++r) {
                             const int key = key0 + r;
-                            const uint32_t bits = *(volatile uint32_t*)&sy->odd[mem][0][n][r >> 5] | *(volatile uint32_t*)&sy->odd[mem][1][n][r >> 5];
+                            const uint32_t bits = *(volatile uint32_t*)&sy->odd[mem][n][r >> 5];
                             if (!((bits >> (r & 31)) & 1u) || key < lo || key > hi) continue;
                             const int first = a.pages.page_row(p.s, key >> a.pages.shift);
                             if (first < 0) continue;
@@ -711,15 +736,10 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, Walk<k
                 }
                 __syncwarp();
             }
-            // (eight arrivals an item, all from warps that took part: one that passes an item by must not run ahead into the barrier's next phase)
-            if (lane == 0) {
-                mbar_arrive(&sy->item_done[items % kOddItems]);
-                if (p.tiles == 1) mbar_arrive(&sy->item_done[items % kOddItems]);
-            }
         }
         seq0 += (uint32_t)(p.units * p.tiles);
         c += (uint32_t)p.units;
-        w.next(a);
+        done_part(sy, items);
     }
 }
 
@@ -746,7 +766,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk(const __grid_co
             }
             mbar_init(&sy.o_free[t], 4);
         }
-        for (int i = 0; i < kOddItems; ++i) mbar_init(&sy.item_done[i], 8);
+        for (int i = 0; i < kParts; ++i) {
+            mbar_init(&sy.part_full[i], 1);
+            mbar_init(&sy.part_free[i], 8 + 3);       // the warps of the other roles
+        }
         sy.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -758,19 +781,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk(const __grid_co
     wait_for_previous_kernel();
     let_next_kernel_launch();
     Walk<kShift> w;
-    const Shares shares = plan<kShift, kChunkThreads>(a, reinterpret_cast<PlanScratch<kChunkThreads>*>(smem), worker, kChunkBegin + kChunkUnit, w);
-    if (threadIdx.x == 0) a.joins[worker] = make_int4(0, 0, 0, 0);
+    const Shares shares = plan<kShift, kChunkThreads>(a, reinterpret_cast<PlanScratch<kChunkThreads>*>(smem), warp == 8 ? worker : 0x7fffffff, kChunkBegin + kChunkUnit, w);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");              // (copies go where the plan's sums were)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *(volatile uint32_t*)&sy.tmem;
     if (warp < 8) {
-        softmax_role<DT, D>(a, &sy, w, tmem, worker, shares);
+        softmax_role<DT, D>(a, &sy, tmem, worker);
     } else {
-        if (warp == 8) load_role<D>(a, m, smem, &sy, w);
-        else if (warp == 9) product_role<DT, D>(a, smem, &sy, w, tmem);
-        else value_role<DT, D>(a, smem, &sy, w);
+        if (warp == 8) load_role<D>(a, m, smem, &sy, w, worker, shares);
+        else if (warp == 9) product_role<DT, D>(smem, &sy, tmem);
+        else value_role<DT, D>(smem, &sy);
     }
     tc_fence_before();
     __syncthreads();

@@ -165,8 +165,8 @@ def _cache(what, k_cache, v_cache, pages, seqs, kv_heads, head_dim, page_size, d
     table, table_ld, shape = _ints(what, "pages", pages, device, 2)
     if shape[0] != seqs:
         raise ValueError(f"{what}: pages has {shape[0]} rows, pos {seqs}")
-    if rows > 2 ** 31 - 1 or shape[1] * page_size > 2 ** 31 - 1:
-        raise ValueError(f"{what}: at most 2^31 - 1 rows in the cache and of a sequence")
+    if rows > 2 ** 31 - 1 or shape[1] * page_size > 2 ** 31 - 65536:
+        raise ValueError(f"{what}: at most 2^31 - 1 rows in the cache, 2^31 - 65536 of a sequence")
     return _lib.PagedCache(k[_PTR], v[_PTR], table, k[_LD], v[_LD], table_ld, rows // page_size, page_size, shape[1], kv_heads, head_dim,
                            DTYPE_CODE[dtype]), k, v
 
