@@ -110,6 +110,7 @@ extern "C" int mk_paged_attention(int device, const mk_batch* batch, const mk_pa
     if (!why && window < 0) why = "paged attention: window is a number of rows (0: the whole context)";
     if (why) return report(MK_E_ARG, why);
     if (batch->rows == 0 || batch->seqs == 0) return MK_OK;
+    if (max_new < 1) max_new = 1;                     // (a hint; an item has a token at least)
     const int D = cache->head_dim, group = heads / cache->kv_heads;
     const long long width = (long long)heads * D;
     if (!q || !out || ld_q < width || ld_out < width || !aligned16(q, ld_q, 2) || !aligned16(out, ld_out, 2))

@@ -127,6 +127,8 @@ def _batch(what, rows, pos, starts, device) -> _lib.Batch:
     seqs = shape[0]
     if shape[1] != 1:
         raise ValueError(f"{what}: pos has one column, one row per sequence")
+    if rows > 2 ** 31 - 1 or seqs > 2 ** 31 - 2:
+        raise ValueError(f"{what}: at most 2^31 - 1 rows and 2^31 - 2 sequences")
     bounds = None
     if starts is not None:
         bounds, _, shape = _ints(what, "starts", starts, device, 1)

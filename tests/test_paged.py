@@ -313,6 +313,15 @@ def test_paged_attention_any_form(cuda, D, H, KVH, new, max_new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("max_new", [0, -3])
+@pytest.mark.parametrize("H,KVH", [(12, 1), (32, 2), (3, 3)])
+def test_paged_attention_hint_below_one(cuda, H, KVH, max_new):
+    """... is taken as one token, also where a group has more heads than half of an item has rows."""
+    args, kw = make_attention([33, 0], [2, 1], H, KVH, 64, 16, BF, seed=8)
+    check_attention(cuda, args, dict(kw, max_new=max_new))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [1, 4, 150])
 @pytest.mark.parametrize("D,dtype", [(64, BF), (128, HALF)])
 def test_paged_attention_absent_pages(cuda, D, dtype, new):
