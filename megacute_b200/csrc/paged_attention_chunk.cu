@@ -551,6 +551,7 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, uint32
             seen_by(p, t * tile_tokens, lo_any, unused);
             seen_by(p, last - 1, unused, hi_any);
             float m = NEG_INF, l = 0.f;
+            bool low = true;                                                   // some row of the warp has no maximum yet
             for (int u = 0; u < p.units; ++u) {
                 const uint32_t n = seq0 + (uint32_t)(u * p.tiles + t), buf = n % M::kScores;
                 const uint32_t scol = tl + 128 * buf;
@@ -609,6 +610,7 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, uint32
                 if (__any_sync(0xffffffffu, raise)) {
                     const float factor = !raise ? 1.f : m == NEG_INF ? 0.f : ex2(m - mx);
                     if (raise) m = mx;
+                    low = __any_sync(0xffffffffu, m == NEG_INF);
                     if (u > 0) {
                         if (!warp_wait(sy, &sy->pv_done[t][(blocks - 1u) & 3u], ((blocks - 1u) >> 2) & 1u)) return;      // O is complete up to here
                         tc_fence_after();
@@ -625,6 +627,7 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, uint32
                     }
                 }
                 const float mm = m == NEG_INF ? 0.f : m;                       // (no key so far: every score is -inf)
+                const bool exact = edge || low;                                // (-inf must become 0)
                 const float2 scale2 = make_float2(a.scale2, a.scale2), off2 = make_float2(-mm, -mm);
                 float2 l4[4] = {};
                 // P of 32 columns: of each 16, the pairs of `fma` without the special function units (where every key is seen: a hidden one must be 0)
@@ -642,7 +645,7 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, uint32
                     }
                     tmem_st16(scol + ch * 16, x);
                 };
-                if (!edge) {
+                if (!exact) {
 #pragma unroll 1
                     for (int ch = 0; ch < 4; ++ch) {
                         tmem_ld32(scol + ch * 32, va);

@@ -262,7 +262,7 @@ extern "C" int mk_rotary(int device, const mk_batch* batch, const mk_rotation* r
     if (batch->rows == 0 || batch->seqs == 0) return MK_OK;
     const long long width = (long long)heads * head_dim;
     const int es = elem_bytes(dtype);
-    if (!x || !out || width > 0x3fffffff || ld_x < width || ld_out < width || !aligned16(x, ld_x, es) || !aligned16(out, ld_out, es))
+    if (!x || !out || width > 0x1fffffff || ld_x < width || ld_out < width || !aligned16(x, ld_x, es) || !aligned16(out, ld_out, es))
         return report(MK_E_ARG, "rotary: rows hold all heads and start on 16-byte boundaries");
     OnDevice on(device);
     if (!on.ok) return report(MK_E_CUDA, "cudaSetDevice");
@@ -285,7 +285,7 @@ extern "C" int mk_paged_append(int device, const mk_batch* batch, const mk_rotat
     if (why) return report(MK_E_ARG, why);
     if (batch->rows == 0 || batch->seqs == 0) return MK_OK;
     const long long width = ((long long)heads + 2ll * cache->kv_heads) * cache->head_dim, q_width = (long long)heads * cache->head_dim;
-    if (!qkv || !q_out || width > 0x3fffffff || ld_qkv < width || ld_q < q_width || !aligned16(qkv, ld_qkv, 2) || !aligned16(q_out, ld_q, 2))
+    if (!qkv || !q_out || width > 0x1fffffff || ld_qkv < width || ld_q < q_width || !aligned16(qkv, ld_qkv, 2) || !aligned16(q_out, ld_q, 2))
         return report(MK_E_ARG, "paged append: rows hold all heads and start on 16-byte boundaries");
     OnDevice on(device);
     if (!on.ok) return report(MK_E_CUDA, "cudaSetDevice");

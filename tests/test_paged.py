@@ -403,6 +403,30 @@ def test_paged_attention_large_scores(cuda, new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new", [1, 40])
+def test_paged_attention_scores_of_minus_infinity(cuda, new, D):
+    """A key whose score overflows to -inf has no weight, like one that is masked; a row of such keys alone becomes zeros."""
+    args, kw = make_attention([300, 280], [new, new], 4, 2, D, 16, BF, seed=15)
+    q, k = args["q"], args["k_cache"]
+    q[:, 0] = 2.0 ** 120                                                       # head 0
+    k[:, 0] = -2.0 ** 120                                                      # every key of its kv head
+    got = mc.paged_attention(**on(cuda, args), **kw).cpu()
+    assert (got[:, :D] == 0).all()
+    assert torch.isfinite(got[:, 2 * D:]).all()
+    rows = args["pages"][0, :4].repeat_interleave(16) * 16 + torch.arange(16).repeat(4)      # the first 64 rows of sequence 0
+    k[rows.long(), 0] = 0.0
+    got = mc.paged_attention(**on(cuda, args), **kw).cpu()[:new, :D]
+    only = dict(args, q=q[:new], pos=torch.full((new, 1), 63, dtype=torch.int32), pages=args["pages"][:1].expand(new, -1).contiguous(), starts=None)
+    only["q"] = only["q"].clone()
+    only["k_cache"] = k.clone()
+    only["k_cache"][:, 0] = 0.0
+    want, mag, size = ref.paged_attention(**only, **kw)
+    tol = attention_tolerance(want, mag, size, BF, D, 64, float(args["v_cache"].double().abs().max()))
+    close(got, want[:, :D], tol[:, :D])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [1, 40])
 def test_paged_attention_strided(cuda, new):
     """q a column range of qkv, caches column ranges of one tensor, a page table and an out with a pitch: the same bits as contiguous ones."""
