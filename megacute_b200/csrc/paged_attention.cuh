@@ -1,10 +1,10 @@
 // How attention over a paged cache is divided among workers, and what its kernels share.
 //
 // An item is up to `tokens` consecutive new tokens of one sequence and `group` query heads of one kv head: rows token * group + head of one
-// operand tile.  (Where more heads share a kv head than the tile has rows, `shared` such blocks of heads read it.)  Its keys are cut into units of 2^shift keys.  All units of all items -- in the order
-// sequence, block of heads, tokens -- make one list, which is dealt out evenly by what they cost (Cost): each worker has the next N / W of the
-// list's whole cost N, the first N % W one more.  Lengths are known on
-// the device only, so every block works out its part itself, and batches of the most unlike lengths load all SMs alike.
+// operand tile.  (Where more heads share a kv head than the tile has rows, `shared` such blocks of heads read it.)  Its keys are cut into units of
+// 2^shift keys.  All units of all items -- in the order sequence, block of heads, tokens -- make one list, which is dealt out evenly by what they
+// cost (Cost): each worker has the next N / W of the list's whole cost N, the first N % W one more.  Lengths are known on the device only, so every
+// block works out its part itself (about 2 us for up to 128 sequences), and batches of the most unlike lengths load all SMs alike.
 // A worker that has an item's units from the first to the last writes results.  Else it leaves the running maximum, the sum and the products of its
 // part in the workspace (slot 0: a part that does not begin the item; slot 1: one that begins it); a block joins the parts that its
 // own workers have of an item, and a second kernel (paged_attention.cu) those of several blocks, always in the same order.
@@ -65,7 +65,8 @@ struct Shares {
     }
 };
 
-// Costs of the chunk kernel: an item's beginning and end, a key tile with both query tiles, with one.
+// Costs of the chunk kernel: an item's beginning and end, a key tile with both query tiles, with one.  (Key tiles alone, all alike: 4 x 4096 tokens 433
+// instead of 413 us for 64-wide heads, 311 instead of 283 for 128-wide, 24 sequences of up to 700 tokens with a window 125 instead of 115.)
 constexpr int kChunkBegin = 4, kChunkUnit = 3, kChunkHalf = 2;
 
 // What an item costs: its beginning and end, and each of its units.  A place in the list of costs is the first unit whose end lies behind it.

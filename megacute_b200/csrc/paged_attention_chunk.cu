@@ -2,17 +2,25 @@
 // mix them with single tokens.
 //
 // An item is two tiles of 128 query rows that share every tile of 128 keys (paged_attention.cuh: a unit).  One block per SM, one worker per block:
-//   warps 0-3, 4-7   softmax of tile 0 and 1, one thread per row (a lane of tensor memory): the row's 128 scores are held in registers, so
-//                    nothing is exchanged between threads; log2 domain, scale * log2(e) folded into the subtraction; the maximum is only
-//                    raised when it grows by more than 2^8, and then the row of O in tensor memory is scaled down; results
-//   warp 8           loader: Q as boxes of 64 columns x group heads x tokens, K and V as boxes of 64 columns x the rows of a page (at most 128), found
+//   warps 0-3, 4-7   softmax of tile 0 and 1, one thread per row (a lane of tensor memory), so that nothing is exchanged between threads: the
+//                    row's 128 scores are read twice, 64 columns at a time for the maximum, 32 for the weights; log2 domain, scale * log2(e)
+//                    folded into the subtraction; the maximum is only raised when it grows by more than 2^8, and then the row of O in tensor
+//                    memory is scaled down; results
+//   warp 8           loader: walks the block's items and tells the other roles; Q as boxes of 64 columns x group heads x tokens, K and V as boxes of 64 columns x the rows of a page (at most 128), found
 //                    through the page table, into one ring of tiles in the order K, V, K, V, ...
 //   warp 9           products: S = Q K^T and O += P V on tcgen05, S, P (over S) and O in tensor memory
 //   warps 10, 11     look at every V tile before it is multiplied: rows that no token of the item sees become zeros (they may hold anything, and
 //                    0 * inf is no number); where some tokens see a row and others do not, values that are no numbers are taken out and added back
 //                    to the rows that see them when the item ends
-// A score product of 128 x 128 x 64 takes 256 cycles, its exponentials 1024 (16 a cycle), so for head_dim 64 the special function units
-// bound it, for 128 both do.
+// P is rounded to the operand type, which the second product takes; sums of weights are of the unrounded ones, O and both statistics fp32.
+//
+// What bounds it: a score product of 128 x 128 x 64 and its P V take 256 cycles each of the tensor cores, the 16384 exponentials 1024 of the special
+// function units (16 a cycle) or 768 with a quarter of them on the fp32 units, and the maxima, conversions and accesses to tensor memory of the same
+// threads come on top.  So head_dim 64 is bound by the softmax; for 128, whose products take twice as long, the chain from S over P to P V and the next S
+// through two buffers of scores counts as much.  Measured: 4 prompts of 4096 tokens, bf16, 32 heads and 8 kv heads of 64: 400 us, 687 TFLOP/s; 16 heads
+// and 4 kv heads of 128: 283 us, 970 TFLOP/s; 509 tokens behind 16001, 32 heads of 64: 103 to 106 us, 640 TFLOP/s.
+// Both sides of the choices, for the first two of these (us): the maximum raised whenever it grows 459 and 333; the row's scores held in registers
+// (spills) 467; two threads a row 429; the two tiles' exponentials in turns 458.
 // Every wait has a limit, after which the block raises a flag that all its waits ask for, waits for its copies, frees its tensor memory and ends;
 // mk_paged_attention_status tells.
 #include <cuda.h>          // CUtensorMap
@@ -27,8 +35,10 @@ __device__ int g_paged_failed;                        // a block gave up waiting
 namespace {
 
 constexpr int kChunkThreads = 384;
-constexpr float kLazy = 8.0f;
-constexpr uint32_t kFmaPairs = 0b00010001;            // of eight pairs of exponentials, those that the fp32 units take
+constexpr float kLazy = 8.0f;                         // (log2; fp32 sums and products of weights up to 2^8 lose nothing, and fp16 weights stay in range)
+// Of eight pairs of exponentials, those that the fp32 units take.  4 x 4096 tokens with none, one, two, three, four of them: 419, 404, 400, 406, 419 us
+// (64-wide heads), 292, 287, 283, 279, 284 (128-wide).
+constexpr uint32_t kFmaPairs = 0b00010001;
 template <bool V> struct Const { static constexpr bool value = V; };
 constexpr unsigned long long kWaitNs = 2000000000ull;
 constexpr int kTileRows = 128;
@@ -55,7 +65,7 @@ struct Part {
     int whole;                                        // bit 0: it begins the item, bit 1: it ends it
 };
 constexpr int kShift = 7;
-constexpr int kParts = 4;                             // entries of the ring
+constexpr int kParts = 4;                             // entries of that ring
 __device__ __forceinline__ int saturated(long long x) { return (int)min(max(x, -0x7fff0000ll), 0x7fffff00ll); }
 __device__ __forceinline__ Part part_of(const AttnArgs& a, const Walk<kShift>& w) {
     Part p;

@@ -34,8 +34,8 @@ import torch
 from . import _lib
 from .graph import DTYPE_CODE
 
-_HALVES = (torch.bfloat16, torch.float16)
-_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_HALVES = {torch.bfloat16: 2, torch.float16: 2}      # types and their sizes
+_FLOATS = {torch.bfloat16: 2, torch.float16: 2, torch.float32: 4}
 
 
 def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: dict | None = None, max_pos: int | None = None):
@@ -96,7 +96,8 @@ _PTR, _LD, _ROWS, _COLS, _SIZE = range(5)
 
 def _rows(what, name, t, dtypes, device=None, cols=None):
     """(address, elements between rows, rows, columns, element size) of a 2-D tensor whose rows start on 16-byte boundaries."""
-    if t.dtype not in dtypes:
+    size = dtypes.get(t.dtype)
+    if size is None:
         raise TypeError(f"{what}: {name} has unsupported dtype {t.dtype}")
     shape = t.shape
     if len(shape) != 2:
@@ -107,7 +108,7 @@ def _rows(what, name, t, dtypes, device=None, cols=None):
     if cols is not None and width != cols:
         raise ValueError(f"{what}: {name} has {width} columns, expected {cols}")
     ld, inner = t.stride()
-    ptr, size = t.data_ptr(), t.itemsize
+    ptr = t.data_ptr()
     if (inner != 1 and width > 1) or (ld < width and rows > 1) or ld * size % 16 or ptr % 16:
         raise ValueError(f"{what}: {name} needs unit inner stride and rows that start on 16-byte boundaries")
     return ptr, ld if ld > width else width, rows, width, size          # (a single row's stride says nothing)
@@ -174,11 +175,11 @@ def _cache(what, k_cache, v_cache, pages, seqs, kv_heads, head_dim, page_size, d
 
 
 def _out(what, out, like, device, dtype, rows, cols):
-    """The result tensor, what _rows says of it, and whether it is the caller's."""
+    """The result tensor (of the type and on the device of `like`), what _rows says of it, and whether it is the caller's."""
     if out is None:
-        out = torch.empty((rows, cols), dtype=dtype, device=device)
-        return out, (out.data_ptr(), cols, rows, cols, like[_SIZE]), False
-    o = _rows(what, "out", out, (dtype,), device, cols)
+        out = like.new_empty((rows, cols))
+        return out, (out.data_ptr(), cols, rows, cols, _FLOATS[dtype]), False
+    o = _rows(what, "out", out, {dtype: _FLOATS[dtype]}, device, cols)
     if o[_ROWS] != rows:
         raise ValueError(f"{what}: out has {rows} rows")
     return out, o, True
@@ -209,7 +210,7 @@ def _workspace_bytes(device_index, heads, kv_heads, head_dim, max_new) -> int:
 def _stream(what, device):
     if device.type != "cuda":
         raise ValueError(f"{what}: expected CUDA tensors")
-    return torch.cuda.current_stream(device.index).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)      # (torch.cuda.current_stream makes an object, 1.2 us)
 
 
 def _heads(what, heads, head_dim):
@@ -232,7 +233,7 @@ def rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Ten
     device, dtype, rows = x.device, x.dtype, src[_ROWS]
     rot = _rotation(what, cos, sin, interleaved, head_dim, device)
     batch = _batch(what, rows, pos, starts, device)
-    out, dst, given = _out(what, out, src, device, dtype, rows, heads * head_dim)
+    out, dst, given = _out(what, out, x, device, dtype, rows, heads * head_dim)
     if given and dst != src:
         _apart(what, "out", dst, src)
     stream = _stream(what, device)
@@ -258,7 +259,7 @@ def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: t
     rot = _rotation(what, cos, sin, interleaved, head_dim, device)
     batch = _batch(what, rows, pos, starts, device)
     cache, k, v = _cache(what, k_cache, v_cache, pages, batch.seqs, kv_heads, head_dim, page_size, dtype, device)
-    out, dst, given = _out(what, out, src, device, dtype, rows, heads * head_dim)
+    out, dst, given = _out(what, out, qkv, device, dtype, rows, heads * head_dim)
     if given:
         for t in (src, k, v):
             _apart(what, "out", dst, t)
@@ -281,8 +282,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     A row at position p attends rows [0, p] of its sequence, or the last ``window`` of these; grouped queries: head h reads kv head
     h // (heads / kv_heads).  Rows of absent pages and rows behind the page table are not there; a row that sees none becomes zeros.  (A key whose
-    score overflows to -inf has no weight; a row that sees a score of +inf or NaN has no result, NaN.)  ``scale`` is head_dim ** -0.5 by default.  head_dim 64 or 128.  Statistics and sums are fp32; the probabilities are rounded to q's type in front of the product
-    with V.
+    score overflows to -inf has no weight; a row that sees a score of +inf or NaN has no result, NaN.)  ``scale`` is head_dim ** -0.5 by default.
+    head_dim 64 or 128.  Statistics and sums are fp32; the probabilities are rounded to q's type in front of the product with V.
 
     ``max_new``: the largest number of rows a sequence has in this call, where ``starts`` is given (it is on the device): the kernel is chosen by it, and
     a wrong value costs time but changes no more than the order of sums."""
@@ -299,7 +300,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     batch = _batch(what, rows, pos, starts, device)
     seqs = batch.seqs
     cache, k, v = _cache(what, k_cache, v_cache, pages, seqs, kv_heads, head_dim, page_size, dtype, device)
-    out, dst, given = _out(what, out, src, device, dtype, rows, heads * head_dim)
+    out, dst, given = _out(what, out, q, device, dtype, rows, heads * head_dim)
     if given:
         for t in (src, k, v):
             _apart(what, "out", dst, t)
@@ -311,7 +312,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     elif max_new is None:
         max_new = rows
     nbytes = _workspace_bytes(device.index, heads, kv_heads, head_dim, max_new)
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    workspace = q.new_empty(nbytes // 2)               # (of 2-byte elements)
     _lib.check(_lib.load().mk_paged_attention(device.index, batch, cache, src[_PTR], src[_LD], dst[_PTR], dst[_LD], heads,
                                       head_dim ** -0.5 if scale is None else scale, window, max_new, workspace.data_ptr(), nbytes, stream),
                "mk_paged_attention")

@@ -5,10 +5,10 @@ Tolerances, from the arithmetic.  u is half a step of the type (finfo.eps / 2), 
     of the result; a result below the type's normal range is off by half of its smallest step.
   attention: one rounding of the result, u |y|.  A probability is rounded to the type (u of it).  A score of D products summed in fp32 is off by at
     most (D + 4) w times the sum of the products' magnitudes, in every order; it goes through 2^(s log2(e)), whose argument is off by two further
-    roundings (of the scaled score and of the difference, 2 w of its size, itself at most the scaled magnitudes) and whose value by 2^-21 (the
-    hardware's approximation and what may replace it).  The sum of probabilities has these errors too, and those of at most n + 64 additions,
-    w each, taken here as 2^-14 for all n up to a thousand: so every weight is off by u + 2 (D + 6) w S + 2^-13, S the largest sum of magnitudes, and the result
-    by that times sum_j w_j |v_j|.  fp16 probabilities below the normal range: half a smallest step (2^-25) each, of a largest probability of at least one.
+    roundings (of the scaled score and of the difference, 2 w of its size, itself at most the scaled magnitudes) and whose value by 2^-18.5 (the
+    polynomial that replaces some of the hardware's approximations, which are closer).  The sum of probabilities has these errors too, and those of at
+    most n + 64 additions, w each, taken here as 2^-14 for all n up to a thousand; 2^-14 + 2 * 2^-18.5 is below 2^-13: so every weight is off by
+    u + 2 (D + 6) w S + 2^-13, S the largest sum of magnitudes, and the result by that times sum_j w_j |v_j|.  fp16 probabilities below the normal range: half a smallest step (2^-25) each, of a largest probability of at least one.
 """
 import ctypes
 
