@@ -224,7 +224,7 @@ int mk_argmax(const void* logits, int dtype, int rows, int cols, long long ld, l
  *
  * The tokens of a call are rows of a packed batch: sequence s has rows starts[s] .. starts[s + 1] - 1 (never decreasing), or, with
  * starts NULL, rows / seqs rows each.  Its first row is at position pos[s * pos_ld], the next one behind it.  Rows in front of the first
- * sequence and behind the last one are neither read nor written.  All arrays are device memory, read when the kernel runs, so a captured call
+ * sequence and behind the last one are not written.  All arrays are device memory, read when the kernel runs, so a captured call
  * replays with the values of that time.  Every entry runs on `device`, whichever device is current, and is asynchronous
  * on `stream`; it allocates nothing and keeps nothing, so calls on different streams do not disturb one another.  dtype: 0 bf16, 1 fp32, 2 fp16. */
 typedef struct mk_batch {
