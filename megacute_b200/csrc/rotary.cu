@@ -7,7 +7,7 @@
 // A thread's piece is 16 elements of a head (8 pairs: two 16-byte accesses of a 16-bit type, the same 8 table columns in both layouts) in up to four heads
 // of a row (fp32: two), so that cosines and sines are fetched once for all of them; the next piece's elements are asked for before this one is turned.  A block has up
 // to eight rows; its warps find the rows' sequences, positions and cache rows while the first elements come.
-// Measured (5 prompts of up to 3271 rows, 32 heads of 128, 96 rotated; append of 4 x 4096 rows, 48 heads of 64): 24.2 and 41.5 us, 82 % and 75 % of the
+// Measured (5 prompts of up to 3271 rows, 32 heads of 128, 96 rotated; append of 4 x 4096 rows, 48 heads of 64): 23.5 and 40.5 us, 85 % and 77 % of the
 // measured copy rate; blocks of 256 threads, one piece a thread, looked up first 26 and 49 us; two heads a piece 28.7 and 41.9.
 #include "paged.cuh"
 
@@ -207,8 +207,10 @@ int launch(RotArgs& a, int dtype, bool inter, bool append, void* stream) {
     const int each = dtype == DT_F32 ? heads_of_thread<4> : heads_of_thread<2>;
     a.groups = (heads + each - 1) / each;
     const int per_row = slots * a.groups;
-    // rows of a block: as many as give each thread a piece, more where there are blocks enough (a block begins with a chain of look-ups)
-    a.block_rows = min(kRotRows, max(max(1, kRotThreads / per_row), a.batch.rows / kRotBlocks));
+    // rows of a block: at least as many as give each thread a piece, else so many that the blocks fill whole rounds of the SMs (a block begins with a chain of
+    // look-ups, so few rounds; 4 x 4096 rows in 3.5 rounds of 8 rows 41.4 us, in 4 of 7 40.4, in 2 of 14 40.2; 5 prompts 24.7, 23.5 and 30)
+    const int least = max(1, kRotThreads / per_row), rounds = (a.batch.rows - 1) / (kRotBlocks * kRotRows) + 1;
+    a.block_rows = min(kRotRows, max(least, (a.batch.rows - 1) / (kRotBlocks * rounds) + 1));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((a.batch.rows + a.block_rows - 1) / a.block_rows));
     cfg.blockDim = dim3(kRotThreads);
