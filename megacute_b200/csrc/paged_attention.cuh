@@ -54,7 +54,7 @@ struct Shares {
     int workers, longer;                              // `longer` workers have per + 1, the others per
     __device__ __forceinline__ Shares(long long cost, int most, int least) {
         total = cost;
-        workers = (int)min((long long)most, divide(total + least - 1, least));
+        workers = total ? (int)min((long long)most, max(divide(total, least), 1ll)) : 0;       // (no share below `least`, but of one worker)
         per = workers ? divide(total, workers) : 0;
         longer = (int)(total - per * workers);
     }

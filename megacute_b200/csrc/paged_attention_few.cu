@@ -3,7 +3,7 @@
 // Bound by memory: K and V are read once (heads of a group and tokens of a sequence share them), 2 * 2 * head_dim bytes a key, for 4 * 16 * head_dim
 // products, far below what warp-level matrix instructions give.  Measured: 64 sequences of 1 to 4096 keys, bf16, 4 kv heads of 128: 56 us, 78 % of the
 // measured copy rate; short of that by what comes before and after the keys, 8 to 10 us (launches, the plan, the first look-ups, the joins):
-// one sequence of 1024 keys 11.4 us, of 16384 15.6.  So every warp is a worker of its own (paged_attention.cuh): it
+// one sequence of 1024 keys 9.4 us, of 16384 15.5.  So every warp is a worker of its own (paged_attention.cuh): it
 // copies units of 8 KB (16 keys of head_dim 128, 32 of 64) into its own ring of three with 16-byte asynchronous copies, which follow the
 // page table row by row and write zeros for keys that are not there, and meets no other warp.  16 rows x unit:
 //   S = Q K^T   mma m16n8k16, K rows through ldmatrix (16-byte pieces swizzled by row: no bank conflicts), fp32
@@ -21,7 +21,8 @@ namespace {
 constexpr int kStagesFew = 3;
 constexpr int kUnitBytes = 8192;                      // K and V of a unit
 constexpr float kRaise = 8.0f;
-constexpr int kLeastUnits = 2;                        // units that a worker has at least, where there are few
+// Units that a worker has at least, where there are few: one sequence of 1024 keys 9.4 us with one, 11.4 with two, 13.6 with four.
+constexpr int kLeastUnits = 1;
 
 struct Piece {                                        // a part that a warp has of an item (rows 0: none)
     int rows, row0, block;
