@@ -271,10 +271,11 @@ __device__ __forceinline__ Shares plan(const AttnArgs& a, PlanScratch<THREADS>* 
 // Joins `count` parts of rows [row_begin, row_end) of an item, ROWS of them: part i has slot(i).  With M the largest of their maxima m_i
 //   l = sum_i 2^(m_i - M) l_i,   o = sum_i 2^(m_i - M) o_i,   always in the same order.
 // A thread has eight columns of a row; where that leaves threads over they share a row's parts and add through shared memory.  What a thread waits for
-// is memory, so it asks for kAtOnce parts together.  All threads of the block call it.  write(row, column, l, o) takes eight columns.
+// is memory, so it asks for kAtOnce parts together: two, as most items have; four take half as many threads again in registers (4 x 4096 tokens 402 us
+// instead of 399, a prompt of 2000 50 instead of 46), one after the other one sequence of 16384 keys 17 instead of 16.  All threads of the block call it.  write(row, column, l, o) takes eight columns.
 template <int D, int ROWS, int THREADS>
 struct Join {
-    static constexpr int kTasks = ROWS * (D / 8), kSplits = THREADS / kTasks, kAtOnce = 4;
+    static constexpr int kTasks = ROWS * (D / 8), kSplits = THREADS / kTasks, kAtOnce = 2;
     static_assert(kSplits * kTasks == THREADS, "threads of a join");
     float o[kSplits > 1 ? 8 : 1][kSplits > 1 ? THREADS : 1];
     float m[kSplits > 1 ? THREADS : 1], l[kSplits > 1 ? THREADS : 1];
@@ -348,13 +349,14 @@ struct Join {
     }
 };
 
-// four columns of an item's row (of `a.group` heads a token) of the result
+// eight columns of an item's row (of `a.group` heads a token) of the result
 template <int DT, int D>
-__device__ __forceinline__ void write_result(const AttnArgs& a, int row0, int block, int row, int col, float l, const float4& o) {
+__device__ __forceinline__ void write_result(const AttnArgs& a, int row0, int block, int row, int col, float l, const float4& x, const float4& y) {
     const float inv = l == 0.f ? 0.f : 1.f / l;       // (no key: zeros)
     const int tok = a.token_of(row);
     uint16_t* to = a.out + (long long)(row0 + tok) * a.ld_out + (block * a.group + row - tok * a.group) * D + col;
-    *reinterpret_cast<uint2*>(to) = make_uint2(pack16<DT>(o.x * inv, o.y * inv), pack16<DT>(o.z * inv, o.w * inv));
+    *reinterpret_cast<uint4*>(to) = make_uint4(pack16<DT>(x.x * inv, x.y * inv), pack16<DT>(x.z * inv, x.w * inv),
+                                               pack16<DT>(y.x * inv, y.y * inv), pack16<DT>(y.z * inv, y.w * inv));
 }
 
 // items of few rows (paged_attention_few.cu): rows of an item, workers of a block

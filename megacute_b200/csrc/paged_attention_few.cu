@@ -367,8 +367,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
                 }
             }
             if (done) {
-                write_result<DT, D>(a, head.row0, head.block, row, col, l, o[0]);
-                write_result<DT, D>(a, head.row0, head.block, row, col + 4, l, o[1]);
+                write_result<DT, D>(a, head.row0, head.block, row, col, l, o[0], o[1]);
             } else {
                 if (col == 0) a.stats[to * kFewRows + row] = make_float2(m, l);
                 float4* const at = reinterpret_cast<float4*>(a.part(to, D, row, col));
