@@ -95,17 +95,19 @@ __device__ __forceinline__ Cost cost_of(const AttnArgs& a, int tokens) {
     if (SHIFT < 7) return Cost{0, 1};                 // (few rows: a unit is a unit)
     return Cost{kChunkBegin, tokens > a.tokens / 2 ? kChunkUnit : kChunkHalf};
 }
-// cost of one block of heads of sequence s
 template <int SHIFT>
-__device__ __forceinline__ long long sequence_cost(const AttnArgs& a, int s) {
+__device__ __forceinline__ long long item_cost(const AttnArgs& a, long long p0, int tokens) {
+    return cost_of<SHIFT>(a, tokens).of(item_at<SHIFT>(a, p0, tokens).units);
+}
+// cost of one block of heads of sequence s, its items first, first + step, ...
+template <int SHIFT>
+__device__ __forceinline__ long long sequence_cost(const AttnArgs& a, int s, int first = 0, int step = 1) {
     const int r0 = a.batch.first(s), n = a.batch.count(s, r0);
     if (n == 0) return 0;
     const long long p = a.batch.position(s);
     long long sum = 0;
-    for (int t = 0; t < n; t += a.tokens) {
-        const int tokens = min(a.tokens, n - t);
-        sum += cost_of<SHIFT>(a, tokens).of(item_at<SHIFT>(a, p + t, tokens).units);
-    }
+    for (long long t = (long long)first * a.tokens; t < n; t += (long long)step * a.tokens)
+        sum += item_cost<SHIFT>(a, p + t, (int)min((long long)a.tokens, n - t));
     return sum;
 }
 
@@ -138,16 +140,43 @@ struct Walk {
         unit = at > 0 ? c.unit_at(at, item.units) : 0;
         stop = until >= c.of(item.units) ? item.units : c.unit_at(until, item.units);
     }
-    // to place `at` of the sequence's list (a block of heads costs `per`), with a share of `length`
+    // to place `at` of the sequence's list (a block of heads costs `per`), with a share of `length`.  All lanes of a warp;
+    // where items are many each lane looks at one (one after the other, here and for the sums: 4 x 4096 tokens 397 us instead of 390)
     __device__ __forceinline__ void start(const AttnArgs& a, int seq, long long at, long long per, long long length) {
         sequence(a, seq);
         kv = (int)divide(at, per);
         at -= kv * per;
-        for (t = 0;; t += a.tokens) {
-            const int tokens = item_tokens(a);
-            const long long c = cost_of<SHIFT>(a, tokens).of(item_at<SHIFT>(a, p + t, tokens).units);
-            if (at < c || t + a.tokens >= n) break;
-            at -= c;
+        const int lane = threadIdx.x & 31;
+        t = 0;
+        if (n < 8 * a.tokens) {                       // (few items: one after the other)
+            for (;; t += a.tokens) {
+                const long long c = item_cost<SHIFT>(a, p + t, item_tokens(a));
+                if (at < c || t + a.tokens >= n) break;
+                at -= c;
+            }
+        } else {
+            long long base = 0;                       // first token of lane 0's item
+            for (;;) {
+                const long long mine = base + (long long)lane * a.tokens;
+                long long run = mine < n ? item_cost<SHIFT>(a, p + mine, (int)min((long long)a.tokens, n - mine)) : 0;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const long long up = __shfl_up_sync(0xffffffffu, run, d);
+                    if (lane >= d) run += up;
+                }
+                int in = __popc(__ballot_sync(0xffffffffu, run <= at));                    // items in front of it
+                if (in == 32 && base + 32ll * a.tokens < n) {
+                    base += 32ll * a.tokens;
+                    at -= __shfl_sync(0xffffffffu, run, 31);
+                    continue;
+                }
+                in = min(in, (int)(n - 1 - base) / a.tokens);
+                const long long front = __shfl_sync(0xffffffffu, run, max(in - 1, 0));
+                if (in > 0) at -= front;
+                base += (long long)in * a.tokens;
+                break;
+            }
+            t = (int)base;
         }
         until = at + length;
         enter(a, at);
@@ -186,10 +215,19 @@ __device__ __forceinline__ Shares plan(const AttnArgs& a, PlanScratch<THREADS>* 
         const int each = (a.batch.seqs + 31) / 32;
         int cost[4], run = 0;
         bool big = false;
+        long long only = 0;                           // where each lane has a sequence at most and items are many: lanes share one
+        const bool share = SHIFT >= 7 && a.batch.seqs <= 16 && a.batch.rows / 8 >= a.batch.seqs * a.tokens;
+        if (share) {
+            const int log = a.batch.seqs > 1 ? __clz(a.batch.seqs - 1) - 27 : 5;       // 2^log lanes of a sequence
+            const int s = lane >> log;
+            only = s < a.batch.seqs ? sequence_cost<SHIFT>(a, s, lane & ((1 << log) - 1), 1 << log) : 0;
+            for (int d = 1; d < 1 << log; d <<= 1) only += __shfl_xor_sync(0xffffffffu, only, d);
+            only = __shfl_sync(0xffffffffu, only, (lane << log) & 31);
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int s = lane * each + k;
-            const long long c = k < each && s < a.batch.seqs ? sequence_cost<SHIFT>(a, s) : 0;
+            const long long c = k < each && s < a.batch.seqs ? (share ? only : sequence_cost<SHIFT>(a, s)) : 0;
             big |= c > (1 << 23) / a.blocks;          // (128 of them stay below 2^30)
             cost[k] = (int)c * a.blocks;
             run += cost[k];

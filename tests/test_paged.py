@@ -533,6 +533,16 @@ def test_paged_attention_many_items(cuda, D, H, KVH, dtype, window):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("window", [0, 33])
+@pytest.mark.parametrize("H,max_new", [(128, 1000), (64, 1000), (16, 1)])
+@pytest.mark.parametrize("pos,new", [([0], [150]), ([0, 500, 3, 40, 7], [100, 70, 0, 131, 1]), ([0] * 17, [3, 140] + [1] * 15)])
+def test_paged_attention_many_items_of_a_sequence(cuda, pos, new, H, max_new, window):
+    """Sequences of more items than a warp has lanes: an item is 2 or 4 tokens of one kv head, or (few rows) one."""
+    args, kw = make_attention(pos, new, H, 1, 64, 16, BF, seed=len(pos) + H)
+    check_attention(cuda, args, dict(kw, window=window, max_new=max_new))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [1, 24])
 def test_captured_steps_follow_their_arguments(cuda, new):
     """A captured append and attention: each replay works with the positions, pages and rows of its own time; two graphs beside each other."""
