@@ -26,6 +26,7 @@ or is skipped, as each function says.
 
 from __future__ import annotations
 
+import ctypes
 import functools
 import math
 
@@ -88,6 +89,20 @@ def rotary_tables(max_pos: int, rotary_dim: int, theta: float = 10000.0, scaling
     inv, factor = rotary_frequencies(rotary_dim, theta, scaling, max_pos)
     ang = torch.arange(max_pos, dtype=torch.float64, device=device)[:, None] * inv.to(device)[None]
     return (ang.cos() * factor).to(dtype), (ang.sin() * factor).to(dtype)
+
+
+# -- the binding (csrc/binding.cpp) takes calls whose arguments are plainly right and that have no ``out``; it answers None to others, whose
+# checks, errors and results are the ones below
+@functools.lru_cache(maxsize=1)
+def _direct():
+    lib = _lib.load()
+    try:
+        from . import _binding
+    except ImportError:                              # not built for this interpreter: every call goes through ctypes
+        return None
+    names = ("mk_rotary", "mk_paged_append", "mk_paged_attention", "mk_paged_attention_workspace")
+    _binding.bind(*[ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names])
+    return _binding
 
 
 # -- arguments: each tensor is looked at once, into a tuple of plain numbers
@@ -227,6 +242,11 @@ def rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Ten
     ``cos`` and ``sin`` are (positions, n), row p the angles of position p (``rotary_tables``); the first ``2 n`` elements of a head are rotated, the rest is
     copied.  Pair i is elements (i, i + n), or (2 i, 2 i + 1) if ``interleaved``.  fp32 arithmetic, rounded once.  A row at a position outside the tables
     becomes zeros.  ``out`` may be x itself."""
+    direct = _direct() if out is None else None
+    if direct is not None:
+        y = direct.rotary(x, cos, sin, pos, starts, heads, head_dim, interleaved)
+        if y is not None:
+            return y
     what = "rotary"
     _heads(what, heads, head_dim)
     src = _rows(what, "x", x, _FLOATS, None, heads * head_dim)
@@ -252,6 +272,11 @@ def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: t
     Rotation as in ``rotary``.  A row at a position outside the tables or the page table (a negative one, say, for the padding of a batch) is not
     appended, and its q becomes zeros; a row whose page is absent is not appended.  ``pos`` is not changed.  Two rows of a call must not have one cache
     row: pages that sequences share lie below their positions."""
+    direct = _direct() if out is None else None
+    if direct is not None:
+        y = direct.paged_append(qkv, cos, sin, pos, k_cache, v_cache, pages, starts, heads, kv_heads, head_dim, page_size, interleaved)
+        if y is not None:
+            return y
     what = "paged_append"
     _heads(what, heads, head_dim)
     src = _rows(what, "qkv", qkv, _HALVES, None, (heads + 2 * kv_heads) * head_dim)
@@ -287,6 +312,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     ``max_new``: the largest number of rows a sequence has in this call, where ``starts`` is given (it is on the device): the kernel is chosen by it, and
     a wrong value costs time but changes no more than the order of sums."""
+    direct = _direct() if out is None else None
+    if direct is not None:
+        y = direct.paged_attention(q, k_cache, v_cache, pos, pages, starts, heads, kv_heads, head_dim, page_size, scale, window, max_new)
+        if y is not None:
+            return y
     what = "paged_attention"
     if head_dim not in (64, 128):
         raise ValueError(f"{what}: head_dim must be 64 or 128")

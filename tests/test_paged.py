@@ -16,7 +16,7 @@ import pytest
 import torch
 
 import megacute_b200 as mc
-from megacute_b200 import _lib
+from megacute_b200 import _lib, paged
 from oracle import paged_oracle as ref
 
 BF, HALF, F32 = torch.bfloat16, torch.float16, torch.float32
@@ -716,6 +716,79 @@ def test_refusals(i):
         args["k_cache"], args["v_cache"] = kv[:, :128], kv[:, 64:]
     with pytest.raises(exc, match=words):
         fn(**args, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i", [i for i, r in enumerate(REFUSED) if r[3] != "CUDA"])
+def test_refusals_of_device_tensors(cuda, i):
+    """The same of tensors on the device, which the binding looks at first."""
+    call, change, exc, words = REFUSED[i]
+    fn, args, kw = cpu_calls()[call]
+    args, kw = on(cuda, args), dict(kw)
+    for k, f in change.items():
+        if k == "out":
+            kw["out"] = f(args).to(cuda)
+        elif k in args:
+            args[k] = f(args[k])
+            if words == "16-byte":
+                args[k] = torch.zeros(5 * 256 + 8, dtype=BF, device=cuda)[1:1 + 5 * 256].view(5, 256)
+        else:
+            kw[k] = f
+    if "shares memory" in words and call == "append":
+        kv = torch.zeros(64, 192, dtype=BF, device=cuda)
+        args["k_cache"], args["v_cache"] = kv[:, :128], kv[:, 64:]
+    with pytest.raises(exc, match=words):
+        fn(**args, **kw)
+
+
+def test_binding_refuses_other_objects():
+    """None, no exception, for what is no tensor on a device; the callers' checks go on from there."""
+    direct = paged._direct()
+    assert direct is not None
+    t = torch.zeros(4, 64, dtype=BF)
+    for call, n in ((direct.rotary, 8), (direct.paged_append, 13), (direct.paged_attention, 13)):
+        for args in ((), (None,) * n, (t,) * n, (1,) * n, ("x",) * n, (t, *[10 ** 30] * (n - 1)), (t,) * (n + 1)):
+            assert call(*args) is None
+    with pytest.raises(ValueError):
+        direct.bind(1, 2, 3)
+
+
+@pytest.mark.gpu
+def test_binding_and_ctypes_agree(cuda, monkeypatch):
+    """The calls that the binding takes, and the same through the checks in Python."""
+    def calls():
+        for dtype in (BF, HALF):
+            for starts in (True, False):
+                a, kw = make_append([3, 40, 7], [4, 4, 4], 4, 2, 64, 16, 16, dtype, F32, 3)
+                kc, vc = a["k_cache"], a["v_cache"]
+                a = on(cuda, dict(a, starts=a["starts"] if starts else None, k_cache=kc.clone(), v_cache=vc.clone()))
+                for inter in (False, True):
+                    yield mc.paged_append, a, dict(kw, interleaved=inter), ("k_cache", "v_cache")
+                b, kw = make_attention([3, 40, 70], [4, 4, 4], 4, 2, 64, 16, dtype, 3, starts=starts)
+                b = on(cuda, b)
+                for more in ({}, dict(window=9, scale=0.3), dict(max_new=4), dict(scale=2, window=None), dict(max_new=0)):
+                    yield mc.paged_attention, b, dict(kw, **more), ()
+        x = torch.randn(6, 3 * 64, generator=gen(5)).to(cuda)[:, 64:]                             # (strided, fp32)
+        cos, sin = (t.to(cuda) for t in tables(64, 24))
+        yield mc.rotary, dict(x=x, cos=cos, sin=sin, pos=torch.tensor([[2], [9]], dtype=torch.int32, device=cuda)), dict(heads=2, head_dim=64), ()
+
+    def results():
+        got = []
+        for fn, args, kw, state in calls():
+            args = dict(args, **{k: args[k].clone() for k in state})
+            y = fn(**args, **kw)
+            got.append([y[1:13] if state else y, *[args[k] for k in state]])         # (appended rows 1 .. 12 have a sequence)
+        return got
+
+    used = []
+    real = paged._direct()
+    monkeypatch.setattr(paged, "_direct", lambda: type("D", (), {n: staticmethod(lambda *a, f=getattr(real, n): (used.append(f(*a)), used[-1])[1])
+                                                                 for n in ("rotary", "paged_append", "paged_attention")}))
+    first = results()
+    assert len(used) == len(first) and all(y is not None for y in used)       # the binding took them all
+    monkeypatch.setattr(paged, "_direct", lambda: None)
+    for a, b in zip(first, results()):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
 def test_column_ranges_of_one_tensor_are_apart():
