@@ -3,7 +3,7 @@
 //
 // An item is two tiles of 128 query rows that share every tile of 128 keys (paged_attention.cuh: a unit).  One block per SM, one worker per block:
 //   warps 0-3, 4-7   softmax of tile 0 and 1, one thread per row (a lane of tensor memory), so that nothing is exchanged between threads: the
-//                    row's 128 scores are read twice, 64 columns at a time for the maximum, 32 for the weights; log2 domain, scale * log2(e)
+//                    row's 128 scores are read twice, 64 columns at a time, for the maximum and for the weights; log2 domain, scale * log2(e)
 //                    folded into the subtraction; the maximum is only raised when it grows by more than 2^8, and then the row of O in tensor
 //                    memory is scaled down; results
 //   warp 8           loader: walks the block's items and tells the other roles; Q as boxes of 64 columns x group heads x tokens, K and V as boxes of 64 columns x the rows of a page (at most 128), found
@@ -17,8 +17,8 @@
 // What bounds it: a score product of 128 x 128 x 64 and its P V take 256 cycles each of the tensor cores, the 16384 exponentials 1024 of the special
 // function units (16 a cycle) or 768 with a quarter of them on the fp32 units, and the maxima, conversions and accesses to tensor memory of the same
 // threads come on top.  So head_dim 64 is bound by the softmax; for 128, whose products take twice as long, the chain from S over P to P V and the next S
-// through two buffers of scores counts as much.  Measured: 4 prompts of 4096 tokens, bf16, 32 heads and 8 kv heads of 64: 390 us, 705 TFLOP/s; 16 heads
-// and 4 kv heads of 128: 281 us, 980 TFLOP/s; 509 tokens behind 16001, 32 heads of 64: 100 us, 675 TFLOP/s.
+// through two buffers of scores counts as much.  Measured: 4 prompts of 4096 tokens, bf16, 32 heads and 8 kv heads of 64: 386 us, 712 TFLOP/s; 16 heads
+// and 4 kv heads of 128: 271 us, 1014 TFLOP/s; 509 tokens behind 16001, 32 heads of 64: 100 us, 675 TFLOP/s.
 // Both sides of the choices, for the first two of these when they took 400 and 283 us: the maximum raised whenever it grows 459 and 333; the row's scores held in registers
 // (spills) 467; two threads a row 429; the two tiles' exponentials in turns 458.
 // Every wait has a limit, after which the block raises a flag that all its waits ask for, waits for its copies, frees its tensor memory and ends;
@@ -36,8 +36,8 @@ namespace {
 
 constexpr int kChunkThreads = 384;
 constexpr float kLazy = 8.0f;                         // (log2; fp32 sums and products of weights up to 2^8 lose nothing, and fp16 weights stay in range)
-// Of eight pairs of exponentials, those that the fp32 units take.  4 x 4096 tokens with none, one, two, three, four of them: 419, 404, 400, 406, 419 us
-// (64-wide heads), 292, 287, 283, 279, 284 (128-wide).
+// Of eight pairs of exponentials, those that the fp32 units take.  4 x 4096 tokens with none, one, two, three, four of them, when two took 400 and 283 us:
+// 419, 404, 400, 406, 419 (64-wide heads), 292, 287, 283, 279, 284 (128-wide; since then 271, 270, 282 with two, three, four).
 constexpr uint32_t kFmaPairs = 0b00010001;
 template <bool V> struct Const { static constexpr bool value = V; };
 constexpr unsigned long long kWaitNs = 2000000000ull;
@@ -657,10 +657,13 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Sync* sy, uint32
                 };
                 if (!exact) {
 #pragma unroll 1
-                    for (int ch = 0; ch < 4; ++ch) {
+                    for (int ch = 0; ch < 4; ch += 2) {
                         tmem_ld32(scol + ch * 32, va);
+                        tmem_ld32(scol + ch * 32 + 32, vb);                    // (one after the other: 4 x 4096 tokens 389 and 278 us)
                         tmem_wait_ld();
+                        use32(vb);
                         weigh(ch, va, Const<false>{});
+                        weigh(ch + 1, vb, Const<false>{});
                     }
                 } else {
 #pragma unroll 1
