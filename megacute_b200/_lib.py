@@ -164,7 +164,7 @@ def build_binding(force: bool = False) -> pathlib.Path:
     includes = [header.parent, home / "include", home / "include" / "torch" / "csrc" / "api" / "include", nvcc.parent.parent / "include",
                 sysconfig.get_paths()["include"]]
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *[f"-I{i}" for i in includes], "-o", str(BINDING_PATH), str(source),
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f'-DMK_TORCH_VERSION="{torch.__version__}"', *[f"-I{i}" for i in includes], "-o", str(BINDING_PATH), str(source),
            f"-L{home / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

@@ -227,4 +227,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, n
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__binding(void) { return PyModule_Create(&module); }
+// (the module's view of a tensor is that of the torch it was built against: `built_for` names it)
+PyMODINIT_FUNC PyInit__binding(void) {
+    PyObject* const m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "built_for", MK_TORCH_VERSION)) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

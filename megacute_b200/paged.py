@@ -100,6 +100,8 @@ def _direct():
         from . import _binding
     except ImportError:                              # not built for this interpreter: every call goes through ctypes
         return None
+    if _binding.built_for != torch.__version__:
+        return None
     names = ("mk_rotary", "mk_paged_append", "mk_paged_attention", "mk_paged_attention_workspace")
     _binding.bind(*[ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names])
     return _binding
