@@ -57,6 +57,8 @@ int heads_of_block(int group, int rows) {
 // Few rows and chunk kernel in us, 16 sequences of 4000 keys, bf16, group x tokens: 4 kv heads of 128, 4 x 2 33 and 37, 4 x 4 35 and 38, 4 x 5 60 and 38 (keys
 // read twice); 8 kv heads of 64, 8 x 1 32 and 45, 8 x 2 34 and 45; 12 kv heads of 128, 1 x 16 78 and 86.
 bool few_rows(int group, long long max_new) { return max_new * group <= kFewRows; }
+// The hint as both entries take it: an item has a token at least.
+int tokens_hinted(int max_new) { return max(max_new, 1); }
 
 // what the workspace holds, one behind the other: joins, stats and parts of the blocks, parts of the warps (few rows)
 struct Layout {
@@ -101,7 +103,7 @@ extern "C" long long mk_paged_attention_workspace(int device, int heads, int kv_
     if (!sms) return report(MK_E_CUDA, "no such device");
     const size_t few = layout_of(sms, head_dim, true).bytes, chunk = layout_of(sms, head_dim, false).bytes;
     // (a scale that is not positive is for the kernel for few rows, whatever max_new)
-    return (long long)(few_rows(heads / kv_heads, max_new) || few > chunk ? few : chunk);
+    return (long long)(few_rows(heads / kv_heads, tokens_hinted(max_new)) || few > chunk ? few : chunk);
 }
 
 extern "C" int mk_paged_attention(int device, const mk_batch* batch, const mk_paged_cache* cache, const void* q, int64_t ld_q, void* out,
@@ -113,7 +115,7 @@ extern "C" int mk_paged_attention(int device, const mk_batch* batch, const mk_pa
     if (!why && window < 0) why = "paged attention: window is a number of rows (0: the whole context)";
     if (why) return report(MK_E_ARG, why);
     if (batch->rows == 0 || batch->seqs == 0) return MK_OK;
-    if (max_new < 1) max_new = 1;                     // (a hint; an item has a token at least)
+    max_new = tokens_hinted(max_new);
     const int D = cache->head_dim, group = heads / cache->kv_heads;
     const long long width = (long long)heads * D;
     if (!q || !out || ld_q < width || ld_out < width || !aligned16(q, ld_q, 2) || !aligned16(out, ld_out, 2))
