@@ -39,54 +39,97 @@ _HALVES = {torch.bfloat16: 2, torch.float16: 2}      # types and their sizes
 _FLOATS = {torch.bfloat16: 2, torch.float16: 2, torch.float32: 4}
 
 
-def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: dict | None = None, max_pos: int | None = None):
+# The keys of a scaling dict that each type is defined by.  Those of every type say how it was made, or repeat what is an argument here.
+_SCALING_KEYS = {
+    "default": (),
+    "linear": ("factor",),
+    "dynamic": ("factor",),
+    "llama3": ("factor", "low_freq_factor", "high_freq_factor"),
+    "yarn": ("factor", "beta_fast", "beta_slow", "attention_factor", "mscale", "mscale_all_dim", "truncate"),
+}
+_ANY_SCALING = ("rope_type", "type", "rope_theta", "original_max_position_embeddings", "partial_rotary_factor", "finetuned")
+
+
+def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: dict | None = None, max_pos: int | None = None,
+                       max_position_embeddings: int | None = None):
     """Inverse frequencies of the ``rotary_dim / 2`` pairs, fp64, and the factor on cosines and sines.
 
     ``scaling`` is a ``rope_scaling`` dict of a Hugging Face config: type ``linear`` (angles divided by ``factor``), ``dynamic`` (theta raised
     so that the slowest pair covers ``max_pos`` positions), ``llama3`` (slow pairs stretched by ``factor``, a linear blend between the two
     corner wavelengths) or ``yarn`` (pairs below ``beta_slow`` turns over the original length stretched, those above ``beta_fast`` kept, a ramp over
-    the pairs between; cosines and sines times ``attention_factor``, 0.1 ln(factor) + 1 by default)."""
+    the pairs between, whose corners are rounded outwards unless ``truncate`` is false).  Cosines and sines of ``yarn`` are times ``attention_factor``, by default
+    m(1) with m(s) = 0.1 s ln(factor) + 1, or m(mscale) / m(mscale_all_dim) where the dict has both.
+
+    ``max_position_embeddings``: the config's.  It is the original length of ``dynamic`` and ``yarn`` dicts that hold none, and over the original
+    length the factor of a ``yarn`` dict without one.  A key that holds None counts as absent.  A dict that lacks what its type needs, or holds a key that would be
+    ignored, is refused; so is a ``rope_theta`` that is not ``theta``."""
     if rotary_dim < 4 or rotary_dim % 2:
         raise ValueError("rotary_frequencies: rotary_dim is even and at least 4")
     expo = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
     inv = float(theta) ** -expo
-    sc = scaling or {}
+    sc = {k: v for k, v in (scaling or {}).items() if v is not None}
     kind = sc.get("rope_type", sc.get("type", "default"))
+    if kind not in _SCALING_KEYS:
+        raise ValueError(f"rotary_frequencies: unknown scaling {kind!r}")
+    ignored = sorted(set(sc) - set(_SCALING_KEYS[kind]) - set(_ANY_SCALING))
+    if ignored:
+        raise ValueError(f"rotary_frequencies: scaling {kind!r} does not take {', '.join(ignored)}")
+    if float(sc.get("rope_theta", theta)) != float(theta):
+        raise ValueError(f"rotary_frequencies: theta is {theta}, rope_theta of the scaling {sc['rope_theta']}")
+
+    def need(key, instead=None):
+        value = sc.get(key, instead)
+        if value is None:
+            raise ValueError(f"rotary_frequencies: scaling {kind!r} needs {key}")
+        if not float(value) > 0:
+            raise ValueError(f"rotary_frequencies: {key} of scaling {kind!r} is {value}, expected a positive number")
+        return float(value)
+
     if kind == "default":
         return inv, 1.0
-    if kind not in ("linear", "dynamic", "llama3", "yarn"):
-        raise ValueError(f"rotary_frequencies: unknown scaling {kind!r}")
-    factor = float(sc["factor"])
     if kind == "linear":
-        return inv / factor, 1.0
-    orig = float(sc["original_max_position_embeddings"])
+        return inv / need("factor"), 1.0
     if kind == "dynamic":
+        factor, orig = need("factor"), need("original_max_position_embeddings", max_position_embeddings)
         length = max(float(max_pos or orig), orig)
         base = float(theta) * (factor * length / orig - (factor - 1.0)) ** (rotary_dim / (rotary_dim - 2))
         return base ** -expo, 1.0
     if kind == "llama3":
-        lo, hi = float(sc["low_freq_factor"]), float(sc["high_freq_factor"])
+        factor, lo, hi, orig = (need(k) for k in (*_SCALING_KEYS["llama3"], "original_max_position_embeddings"))
         blend = ((orig * inv / (2 * math.pi) - lo) / (hi - lo)).clamp(0.0, 1.0)          # 0: stretched, 1: as it is
         return (1.0 - blend) * inv / factor + blend * inv, 1.0
+    orig = need("original_max_position_embeddings", max_position_embeddings)
+    factor = need("factor", max_position_embeddings / orig if max_position_embeddings else None)
+
     def pair_with(turns):                        # the pair that turns so often over the original length
         return rotary_dim * math.log(orig / (turns * 2 * math.pi)) / (2 * math.log(float(theta)))
-    first = max(math.floor(pair_with(float(sc.get("beta_fast", 32.0)))), 0)
-    last = min(math.ceil(pair_with(float(sc.get("beta_slow", 1.0)))), rotary_dim - 1)
+    first, last = pair_with(need("beta_fast", 32.0)), pair_with(need("beta_slow", 1.0))
+    if sc.get("truncate", True):
+        first, last = math.floor(first), math.ceil(last)
+    first, last = max(first, 0), min(last, rotary_dim - 1)
     ramp = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - first) / max(last - first, 1e-3)).clamp(0.0, 1.0)
-    attention = sc.get("attention_factor")
-    if attention is None:
-        attention = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
-    return inv / factor * ramp + inv * (1.0 - ramp), float(attention)
+
+    def m(s):
+        return 0.1 * s * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+    if "attention_factor" in sc:
+        attention = float(sc["attention_factor"])
+    elif sc.get("mscale") and sc.get("mscale_all_dim"):
+        attention = m(float(sc["mscale"])) / m(float(sc["mscale_all_dim"]))
+    elif sc.get("mscale", 1.0) == 1.0 and not sc.get("mscale_all_dim"):
+        attention = m(1.0)
+    else:                                        # (those who publish such dicts differ in what one of them alone means)
+        raise ValueError("rotary_frequencies: mscale and mscale_all_dim are for each other, both not zero")
+    return inv / factor * ramp + inv * (1.0 - ramp), attention
 
 
 def rotary_tables(max_pos: int, rotary_dim: int, theta: float = 10000.0, scaling: dict | None = None, dtype: torch.dtype = torch.float32,
-                  device=None):
-    """cos and sin, (max_pos, rotary_dim / 2), of positions 0 .. max_pos - 1: angles in fp64, rounded once to ``dtype``.  ``scaling`` as in
-    ``rotary_frequencies``.  (``checkpoint.rope_tables_from_config`` makes the graph's tables, which hold each column twice; their
+                  device=None, max_position_embeddings: int | None = None):
+    """cos and sin, (max_pos, rotary_dim / 2), of positions 0 .. max_pos - 1: angles in fp64, rounded once to ``dtype``.  ``scaling`` and
+    ``max_position_embeddings`` as in ``rotary_frequencies``.  (``checkpoint.rope_tables_from_config`` makes the graph's tables, which hold each column twice; their
     first half of columns serves here too.)"""
     if dtype not in _FLOATS:
         raise TypeError(f"rotary_tables: unsupported dtype {dtype}")
-    inv, factor = rotary_frequencies(rotary_dim, theta, scaling, max_pos)
+    inv, factor = rotary_frequencies(rotary_dim, theta, scaling, max_pos, max_position_embeddings)
     ang = torch.arange(max_pos, dtype=torch.float64, device=device)[:, None] * inv.to(device)[None]
     return (ang.cos() * factor).to(dtype), (ang.sin() * factor).to(dtype)
 

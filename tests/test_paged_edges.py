@@ -2,6 +2,8 @@
 
 Tolerances are those of tests/test_paged.py, or derived where they stand.
 """
+import math
+
 import pytest
 import torch
 
@@ -44,3 +46,103 @@ def test_workspace_query_suffices(cuda, H, KVH, D, max_new):
         out.fill_(1.0)
         assert call(nbytes) == 0, lib.mk_last_cuda_error()
         assert (out == 0).all()
+
+
+# -- scalings of the frequencies --------------------------------------------------------------------------------------------
+YARN = {"rope_type": "yarn", "factor": 40.0, "original_max_position_embeddings": 4096}
+
+
+def yarn(rotary_dim, theta, factor, orig, fast=32.0, slow=1.0, rounded=True):
+    """Pair by pair: 1 / factor of the angle for pairs of at most `slow` turns over the original length, all of it from `fast` on, linear between."""
+    def pair(turns):
+        return rotary_dim * math.log(orig / (2 * math.pi * turns)) / (2 * math.log(theta))
+    a, b = pair(fast), pair(slow)
+    a, b = (math.floor(a), math.ceil(b)) if rounded else (a, b)
+    a, b = max(a, 0), min(b, rotary_dim - 1)
+    out = []
+    for i in range(rotary_dim // 2):
+        stretched = min(max((i - a) / (b - a), 0.0), 1.0)
+        w = theta ** (-2.0 * i / rotary_dim)
+        out.append(w * (stretched / factor + 1.0 - stretched))
+    return torch.tensor(out, dtype=torch.float64)
+
+
+@pytest.mark.parametrize("mscale,all_dim", [(1.0, 1.0), (0.707, 0.707), (0.707, 1.0), (1.0, 0.8), (2.0, 0.5), (None, None), (1.0, None), (1.0, 0.0), (1, 0)])
+def test_yarn_mscale(mscale, all_dim):
+    inv, f = mc.rotary_frequencies(64, 10000.0, dict(YARN, mscale=mscale, mscale_all_dim=all_dim))
+    term = lambda s: 0.1 * s * math.log(40.0) + 1.0
+    want = term(mscale) / term(all_dim) if mscale and all_dim else term(1.0)
+    assert abs(f - want) < 1e-12
+    assert torch.allclose(inv, yarn(64, 10000.0, 40.0, 4096.0), rtol=1e-12, atol=0)
+    cos, _ = mc.rotary_tables(2, 64, 10000.0, dict(YARN, mscale=mscale, mscale_all_dim=all_dim))
+    assert abs(float(cos[0, 0]) - want) < 1e-6
+    assert mc.rotary_frequencies(64, 10000.0, dict(YARN, mscale=mscale, mscale_all_dim=all_dim, attention_factor=1.25))[1] == 1.25
+
+
+@pytest.mark.parametrize("rotary_dim,theta,factor,orig,fast,slow", [(64, 150000.0, 32.0, 4096, 32.0, 1.0), (128, 10000.0, 16.0, 4096, 32.0, 1.0),
+                                                                    (48, 1e6, 4.0, 32768, 20.0, 2.0)])
+def test_yarn_corners(rotary_dim, theta, factor, orig, fast, slow):
+    sc = {"rope_type": "yarn", "factor": factor, "original_max_position_embeddings": orig, "beta_fast": fast, "beta_slow": slow}
+    for more, rounded in (({}, True), ({"truncate": True}, True), ({"truncate": None}, True), ({"truncate": False}, False)):
+        got, _ = mc.rotary_frequencies(rotary_dim, theta, dict(sc, **more))
+        assert torch.allclose(got, yarn(rotary_dim, theta, factor, float(orig), fast, slow, rounded), rtol=1e-12, atol=0)
+    assert not torch.allclose(got, mc.rotary_frequencies(rotary_dim, theta, sc)[0], rtol=1e-6, atol=0)
+
+
+def test_scaling_lengths_of_the_config():
+    """What a dict leaves to the config's own length."""
+    full = {"type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 2048}
+    part = {"type": "dynamic", "factor": 2.0}
+    for n in (None, 100, 8192):
+        a, b = mc.rotary_frequencies(64, 1e4, full, n), mc.rotary_frequencies(64, 1e4, part, n, max_position_embeddings=2048)
+        assert torch.equal(a[0], b[0]) and a[1] == b[1] == 1.0
+    assert torch.equal(mc.rotary_tables(8192, 64, 1e4, full)[0], mc.rotary_tables(8192, 64, 1e4, part, max_position_embeddings=2048)[0])
+    want = mc.rotary_frequencies(64, 1e4, YARN)
+    for sc, n in (({"rope_type": "yarn", "factor": 40.0}, 4096), ({"rope_type": "yarn", "factor": None, "original_max_position_embeddings": 4096}, 163840),
+                  ({"rope_type": "yarn", "original_max_position_embeddings": 4096}, 163840), (YARN, 7)):
+        got = mc.rotary_frequencies(64, 1e4, sc, max_position_embeddings=n)
+        assert torch.equal(got[0], want[0]) and got[1] == want[1]
+    got = mc.rotary_frequencies(64, 1e4, {"rope_type": "yarn"}, max_position_embeddings=4096)      # as long as it was: as it is
+    assert torch.allclose(got[0], mc.rotary_frequencies(64, 1e4)[0], rtol=1e-12, atol=0) and got[1] == 1.0
+
+
+@pytest.mark.parametrize("kind", ["default", "linear", "dynamic", "llama3", "yarn"])
+def test_scaling_keys_without_effect(kind):
+    """Keys that repeat an argument or say how the config was made, and keys that hold None."""
+    sc = {"rope_type": kind, "original_max_position_embeddings": 4096}
+    if kind != "default":
+        sc["factor"] = 8.0
+    if kind == "llama3":
+        sc.update(low_freq_factor=1.0, high_freq_factor=4.0)
+    want = mc.rotary_frequencies(64, 5e5, sc)
+    got = mc.rotary_frequencies(64, 500000, dict(sc, type=kind, rope_theta=500000.0, partial_rotary_factor=0.5, finetuned=True, mscale=None, long_factor=None))
+    assert torch.equal(got[0], want[0]) and got[1] == want[1]
+
+
+@pytest.mark.parametrize("scaling,words", [
+    ({"rope_type": "yarn", "factor": 4.0}, "needs original_max_position_embeddings"),
+    ({"rope_type": "yarn", "factor": None, "original_max_position_embeddings": 4096}, "needs factor"),
+    ({"rope_type": "yarn", "original_max_position_embeddings": 4096}, "needs factor"),
+    ({"type": "dynamic", "factor": 2.0}, "needs original_max_position_embeddings"),
+    ({"type": "dynamic", "original_max_position_embeddings": 4096}, "needs factor"),
+    ({"type": "linear"}, "needs factor"),
+    ({"type": "linear", "factor": 0.0}, "positive"),
+    ({"type": "linear", "factor": float("nan")}, "positive"),
+    ({"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "original_max_position_embeddings": 8192}, "needs high_freq_factor"),
+    ({"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0}, "needs original_max_position_embeddings"),
+    (dict(YARN, mscale=0.707), "for each other"),
+    (dict(YARN, mscale_all_dim=1.0), "for each other"),
+    (dict(YARN, mscale=0.707, mscale_all_dim=0.0), "for each other"),
+    (dict(YARN, mscale=0.0, mscale_all_dim=0.0), "for each other"),
+    (dict(YARN, low_freq_factor=1.0), "does not take low_freq_factor"),
+    (dict(YARN, attn_factor=2.0), "does not take attn_factor"),
+    ({"type": "linear", "factor": 2.0, "mscale": 1.0, "beta_fast": 32}, "does not take beta_fast, mscale"),
+    ({"rope_type": "default", "mrope_section": [16, 24, 24]}, "does not take mrope_section"),
+    ({"rope_type": "linear", "factor": 2.0, "rope_theta": 500000.0}, "rope_theta"),
+    ({"rope_type": "default", "rope_theta": 500000.0}, "rope_theta"),
+])
+def test_scalings_refused(scaling, words):
+    with pytest.raises(ValueError, match=words):
+        mc.rotary_frequencies(64, 10000.0, scaling)
+    with pytest.raises(ValueError, match=words):
+        mc.rotary_tables(4, 64, 10000.0, scaling)
