@@ -226,7 +226,7 @@ int mk_argmax(const void* logits, int dtype, int rows, int cols, long long ld, l
  * starts NULL, rows / seqs rows each.  Its first row is at position pos[s * pos_ld], the next one behind it.  Rows in front of the first
  * sequence and behind the last one are not written.  All arrays are device memory, read when the kernel runs, so a captured call
  * replays with the values of that time.  Every entry runs on `device`, whichever device is current, and is asynchronous
- * on `stream`; it allocates nothing and keeps nothing, so calls on different streams do not disturb one another.  dtype: 0 bf16, 1 fp32, 2 fp16. */
+ * on `stream`; it allocates nothing and keeps nothing (but the count of mk_paged_attention_failures), so calls on different streams do not disturb one another.  dtype: 0 bf16, 1 fp32, 2 fp16. */
 typedef struct mk_batch {
     const int32_t* pos;
     const int32_t* starts;       /* seqs + 1 entries, or NULL */
@@ -273,8 +273,10 @@ long long mk_paged_attention_workspace(int device, int heads, int kv_heads, int 
 int mk_paged_attention(int device, const mk_batch* batch, const mk_paged_cache* cache, const void* q, int64_t ld_q, void* out, int64_t ld_out,
                        int heads, float scale, int window, int max_new, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Waits for `stream`; MK_E_DEVICE if a kernel of mk_paged_attention on `device` gave up waiting inside since the last call (its results
- * are not to be used; no wait of a kernel lasts longer than two seconds). */
+/* A wait inside a kernel of mk_paged_attention ends after two seconds at most; the results of such a call are not to be used.  Both wait for
+ * `stream` first.  _failures: a count that has grown if that happened to a call on `device`, whatever its stream, since it was asked last; it is
+ * never put back, so that every caller may compare it with what it saw before.  _status: MK_E_DEVICE if it is not zero. */
+int mk_paged_attention_failures(int device, void* stream, uint32_t* count);
 int mk_paged_attention_status(int device, void* stream);
 
 #ifdef __cplusplus

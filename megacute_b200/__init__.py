@@ -16,7 +16,7 @@ written as ``from megacute import Graph`` run unchanged.
 import sys as _sys
 
 from .graph import Buffer, Graph, View, swiglu_weight  # noqa: F401
-from .paged import paged_append, paged_attention, rotary, rotary_frequencies, rotary_tables  # noqa: F401
+from .paged import paged_append, paged_attention, paged_attention_check, rotary, rotary_frequencies, rotary_tables  # noqa: F401
 from .schedule import schedule  # noqa: F401
 
 

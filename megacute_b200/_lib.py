@@ -103,6 +103,7 @@ SYMBOLS = {
     "mk_paged_attention": (ctypes.c_int, [ctypes.c_int, _BATCH, _CACHE, _P, ctypes.c_int64, _P, ctypes.c_int64, ctypes.c_int, ctypes.c_float,
                                           ctypes.c_int, ctypes.c_int, _P, ctypes.c_size_t, _P]),
     "mk_paged_attention_status": (ctypes.c_int, [ctypes.c_int, _P]),
+    "mk_paged_attention_failures": (ctypes.c_int, [ctypes.c_int, _P, ctypes.POINTER(ctypes.c_uint32)]),
     "mk_argmax": (ctypes.c_int, [_P, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_longlong, _P, _P]),
 }
 

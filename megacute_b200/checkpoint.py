@@ -126,7 +126,7 @@ class LlamaGenerator:
 
     def prefill(self, tokens: list[int]) -> int:
         """Feed whole chunks of ``prompt_chunk`` tokens (the same for every sequence of the batch) into the cache, and return how many tokens these
-        are; the rest is for ``step``.  Nothing is sampled."""
+        are; the rest is for ``step``.  Nothing is sampled.  Raises ``MegakernelTimeout`` if a launch or a call gave up a wait: the cache is then not to be used."""
         import megacute_b200 as mc
         c, b = self.prompt_chunk, self.batch
         whole = len(tokens) // c * c if c else 0
@@ -143,6 +143,7 @@ class LlamaGenerator:
         kw = dict(heads=s["H"], kv_heads=s["KVH"], head_dim=d, page_size=128)
         cos, sin = (t[:, :d // 2] for t in self.inputs.values())
         pos, rows = self.state["pos"].expand(b, 1), b * self.max_seq
+        seen = mc.paged_attention_check(self.device, None)
         for at in range(0, whole, c):
             ids = torch.tensor(tokens[at:at + c], dtype=torch.int32, device=self.device).repeat(b).view(-1, 1)
             x = a = None
@@ -154,6 +155,9 @@ class LlamaGenerator:
                 if i + 1 < n:                           # (behind the last layer's keys and values nothing is asked for)
                     a = mc.paged_attention(q, k, v, pos, self._pages, **kw)
             self.state["pos"] += c
+        mc.paged_attention_check(self.device, seen)
+        for prog in self._between:
+            prog.check()
         return whole
 
     def step(self):

@@ -171,14 +171,22 @@ extern "C" int mk_paged_attention(int device, const mk_batch* batch, const mk_pa
     return report(MK_E_CUDA, cudaGetErrorString(e));
 }
 
-extern "C" int mk_paged_attention_status(int device, void* stream) {
+extern "C" int mk_paged_attention_failures(int device, void* stream, uint32_t* count) {
+    if (!count) return report(MK_E_ARG, "paged attention: no place for the count");
     OnDevice on(device);
     if (!on.ok) return report(MK_E_CUDA, "cudaSetDevice");
-    int failed = 0;
-    const cudaError_t e = chunk_status(&failed, (cudaStream_t)stream);
+    unsigned failed = 0;
+    const cudaError_t e = chunk_failures(&failed, (cudaStream_t)stream);
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
         return report(MK_E_CUDA, cudaGetErrorString(e));
     }
-    return failed ? MK_E_DEVICE : MK_OK;
+    *count = failed;
+    return MK_OK;
+}
+
+extern "C" int mk_paged_attention_status(int device, void* stream) {
+    uint32_t failed = 0;
+    const int rc = mk_paged_attention_failures(device, stream, &failed);
+    return rc != MK_OK ? rc : failed ? MK_E_DEVICE : MK_OK;
 }

@@ -405,7 +405,7 @@ cudaError_t launch_few(const AttnArgs& a, float* own /* [worker][kFewRows][head_
 // items of up to 256 rows, a positive scale (paged_attention_chunk.cu): two tiles of 128 rows, a worker per block
 constexpr int kChunkTile = 128;
 cudaError_t launch_chunk(const AttnArgs& a, const mk_paged_cache* cache, int heads, cudaStream_t stream);
-cudaError_t chunk_status(int* failed, cudaStream_t stream);
+cudaError_t chunk_failures(unsigned* count, cudaStream_t stream);
 
 // A kernel's shared memory beyond 48 KB, asked for once per device.
 struct SharedMemory {

@@ -21,8 +21,8 @@
 // and 4 kv heads of 128: 271 us, 1014 TFLOP/s; 509 tokens behind 16001, 32 heads of 64: 100 us, 675 TFLOP/s.
 // Both sides of the choices, for the first two of these when they took 400 and 283 us: the maximum raised whenever it grows 459 and 333; the row's scores held in registers
 // (spills) 467; two threads a row 429; the two tiles' exponentials in turns 458.
-// Every wait has a limit, after which the block raises a flag that all its waits ask for, waits for its copies, frees its tensor memory and ends;
-// mk_paged_attention_status tells.
+// Every wait has a limit, after which the block counts it, raises a flag that all its waits ask for, waits for its copies, frees its tensor memory and
+// ends; mk_paged_attention_failures tells the count.
 #include <cuda.h>          // CUtensorMap
 
 #include "paged_attention.cuh"
@@ -30,7 +30,7 @@
 
 namespace mk {
 
-__device__ int g_paged_failed;                        // a block gave up waiting (read and cleared by mk_paged_attention_status)
+__device__ unsigned g_paged_failed;                   // grows when a block gives up waiting; never put back, so that no reader takes it from another
 
 namespace {
 
@@ -115,7 +115,7 @@ __device__ __noinline__ bool wait_longer(Sync* s, uint32_t bar, uint32_t parity)
     while (!(ok = mbar_try_wait(at, parity)) && !*(volatile int*)&s->abort) {
         if (globaltimer() - t0 > kWaitNs) {
             *(volatile int*)&s->abort = 1;
-            atomicExch(&g_paged_failed, 1);
+            atomicAdd(&g_paged_failed, 1u);
             break;
         }
     }
@@ -879,15 +879,9 @@ cudaError_t launch_chunk(const AttnArgs& a, const mk_paged_cache* c, int heads, 
     return D == 64 ? launch<DT_BF16, 64>(a, m, stream) : launch<DT_BF16, 128>(a, m, stream);
 }
 
-cudaError_t chunk_status(int* failed, cudaStream_t stream) {
-    const int zero = 0;
-    cudaError_t e = cudaMemcpyFromSymbolAsync(failed, g_paged_failed, sizeof(int), 0, cudaMemcpyDeviceToHost, stream);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
-    if (e == cudaSuccess && *failed) {
-        e = cudaMemcpyToSymbolAsync(g_paged_failed, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream);
-        if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
-    }
-    return e;
+cudaError_t chunk_failures(unsigned* count, cudaStream_t stream) {
+    const cudaError_t e = cudaMemcpyFromSymbolAsync(count, g_paged_failed, sizeof(unsigned), 0, cudaMemcpyDeviceToHost, stream);
+    return e == cudaSuccess ? cudaStreamSynchronize(stream) : e;
 }
 
 }  // namespace mk

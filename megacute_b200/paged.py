@@ -20,7 +20,7 @@ token, ``pos`` counts the tokens a sequence has before the call.
   last one are left as they are (in a new ``out``: undefined).
 
 Positions, starts and page tables are read on the device when the call runs: nothing synchronises, and a captured call replays with
-what they hold then.  The contents are the caller's: a position or page outside its range is never followed out of memory, but gives zeros
+what they hold then.  (``paged_attention_check`` synchronises and tells whether a wait inside a kernel gave up.)  The contents are the caller's: a position or page outside its range is never followed out of memory, but gives zeros
 or is skipped, as each function says.
 """
 
@@ -392,3 +392,21 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                                       head_dim ** -0.5 if scale is None else scale, window, max_new, workspace.data_ptr(), nbytes, stream),
                "mk_paged_attention")
     return out
+
+
+def paged_attention_check(device=None, seen: int | None = 0) -> int:
+    """Synchronise the current stream of ``device`` (the current one by default) and raise ``MegakernelTimeout`` if a call of ``paged_attention`` on that
+    device, on whichever stream, gave up a wait (they end after two seconds; what it returned is then not to be used).
+
+    What is returned counts up with each such wait and is never put back.  ``seen`` is the count that the caller knows of already, from an
+    earlier call, say, behind which it goes on; None raises nothing."""
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise ValueError(f"paged_attention_check: {device} is no CUDA device")
+    if device.index is None:
+        device = torch.device(device.type, torch.cuda.current_device())
+    count = ctypes.c_uint32()
+    _lib.check(_lib.load().mk_paged_attention_failures(device.index, _stream("paged_attention_check", device), count), "mk_paged_attention_failures")
+    if seen is not None and count.value != seen:
+        raise _lib.MegakernelTimeout(f"paged_attention: a wait inside a call on {device} timed out (count {count.value}, {seen} seen before)")
+    return count.value

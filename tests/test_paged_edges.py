@@ -146,3 +146,73 @@ def test_scalings_refused(scaling, words):
         mc.rotary_frequencies(64, 10000.0, scaling)
     with pytest.raises(ValueError, match=words):
         mc.rotary_tables(4, 64, 10000.0, scaling)
+
+
+# -- waits that gave up -------------------------------------------------------------------------------------------------------
+class Failing:
+    """The library with a count of failed waits of its own (no wait is made to fail): one more of `counts` each time it is asked."""
+
+    def __init__(self, lib, counts):
+        self.lib, self.counts = lib, list(counts)
+
+    def __getattr__(self, name):
+        return getattr(self.lib, name)
+
+    def mk_paged_attention_failures(self, device, stream, count):
+        count.value = self.counts.pop(0)
+        return 0
+
+
+def test_failed_waits_raise(monkeypatch):
+    """Every caller learns of a failure, however often and by whom the count was read before."""
+    lib = Failing(_lib.load(), [0, 3, 3, 3, 3, 5])
+    monkeypatch.setattr(_lib, "load", lambda: lib)
+    monkeypatch.setattr(paged, "_stream", lambda what, device: 0)
+    dev = torch.device("cuda", 0)
+    assert mc.paged_attention_check(dev) == 0
+    for _ in range(2):
+        with pytest.raises(_lib.MegakernelTimeout, match="timed out"):
+            mc.paged_attention_check(dev)
+    assert mc.paged_attention_check("cuda:0", None) == 3
+    assert mc.paged_attention_check(dev, seen=3) == 3
+    with pytest.raises(_lib.MegakernelTimeout):
+        mc.paged_attention_check(dev, seen=3)
+    with pytest.raises(ValueError, match="no CUDA device"):
+        mc.paged_attention_check("cpu")
+
+
+def test_failures_needs_a_place():
+    assert _lib.load().mk_paged_attention_failures(0, None, None) == -2
+
+
+@pytest.mark.gpu
+def test_no_failures(cuda):
+    args, kw = make_attention([33, 0], [40, 1], 4, 2, 64, 16, BF, seed=8)
+    check_attention(cuda, args, kw)
+    assert mc.paged_attention_check() == mc.paged_attention_check(cuda) == mc.paged_attention_check("cuda", None) == 0
+    with torch.cuda.stream(torch.cuda.Stream()):
+        assert mc.paged_attention_check(cuda) == 0
+    assert _lib.load().mk_paged_attention_status(0, torch.cuda.current_stream().cuda_stream) == 0
+
+
+@pytest.mark.gpu
+def test_generator_tells_of_failed_waits(cuda, monkeypatch):
+    """A prompt in chunks behind which a wait is known to have failed, in an attention call or in one of its launches (a wait target that
+    nothing reaches, with a limit of 50 ms), is an error and not a sequence of tokens."""
+    from megacute_b200.checkpoint import LlamaGenerator
+    from tests.test_checkpoint import CFG, hf_state_dict
+    gen = LlamaGenerator(CFG, hf_state_dict(CFG, seed=5), max_seq=128, device=cuda, prompt_chunk=16)
+    assert gen.generate(list(range(1, 20)), 2).shape == (1, 2)
+    real = _lib.load()
+    lib = Failing(real, [2, 2, 2, 3])
+    with monkeypatch.context() as m:
+        m.setattr(_lib, "load", lambda: lib)
+        assert gen.prefill(list(range(16))) == 16                             # (what failed before it began is not its own)
+        with pytest.raises(_lib.MegakernelTimeout):
+            gen.generate(list(range(1, 20)), 2)
+    prog = gen._between[1]
+    s = prog.sched
+    prog.set_timeout(0.05)
+    _lib.check(real.mk_program_poke_wait(prog._handle, 0, int(s.wait_cnt[0]), int(s.wait_tgt[0]) + 1000))
+    with pytest.raises(_lib.MegakernelTimeout):
+        gen.prefill(list(range(16)))
