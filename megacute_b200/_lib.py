@@ -12,6 +12,7 @@ import pathlib
 import shutil
 import subprocess
 import tempfile
+import warnings
 
 PKG = pathlib.Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
@@ -121,13 +122,20 @@ def needs_build_of(path: pathlib.Path) -> bool:
 
 
 def build(force: bool = False, verbose: bool = False, check: bool | None = None) -> pathlib.Path:
-    """Compile the library with nvcc (cross-compiles without a GPU).  `check`: the -DMK_CHECK build (default: the
-    one this process loads)."""
+    """Compile the library with nvcc (cross-compiles without a GPU), and the Python module beside it, without which calls go through
+    ctypes: where that does not compile there is a warning.  `check`: the -DMK_CHECK build (default: the one this process loads)."""
     check = CHECK_BUILD if check is None else check
     out = LIB_PATH if check == CHECK_BUILD else PKG / ("libmegacute_b200_check.so" if check else "libmegacute_b200.so")
-    if not force and not needs_build_of(out):
-        build_binding()
-        return out
+    if force or needs_build_of(out):
+        _build_library(out, check, verbose)
+    try:
+        build_binding(force)
+    except (RuntimeError, OSError) as e:
+        warnings.warn(f"{BINDING_PATH.name} was not built, its calls go through ctypes: {e}", RuntimeWarning, stacklevel=2)
+    return out
+
+
+def _build_library(out: pathlib.Path, check: bool, verbose: bool):
     nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
     define, loud = ["-DMK_CHECK"] if check else [], ["-Xptxas", "-v"] if verbose else []
     with tempfile.TemporaryDirectory() as tmp:
@@ -145,28 +153,28 @@ def build(force: bool = False, verbose: bool = False, check: bool | None = None)
             raise RuntimeError(f"nvcc failed:\n{' '.join(cmd)}\n{stdout}\n{stderr}")
         if verbose:
             print(stderr)
-    build_binding(force)
-    return out
 
 
 BINDING_PATH = PKG / "_binding.so"
 
 
 def build_binding(force: bool = False) -> pathlib.Path:
-    """Compile csrc/binding.cpp, the Python module through which paged.py calls the library, against this interpreter and its torch."""
+    """Compile csrc/binding.cpp, the Python module through which paged.py calls the library, against this interpreter and its torch.  Raises
+    if that fails, and leaves no module of older sources behind."""
     import sysconfig
 
     import torch
     source, header = CSRC / "binding.cpp", PKG.parent / "include" / "megacute_b200.h"
     if not force and BINDING_PATH.exists() and all(f.stat().st_mtime <= BINDING_PATH.stat().st_mtime for f in (source, header)):
         return BINDING_PATH
+    BINDING_PATH.unlink(missing_ok=True)
     home = pathlib.Path(torch.__file__).resolve().parent
     nvcc = pathlib.Path(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc").resolve()
     includes = [header.parent, home / "include", home / "include" / "torch" / "csrc" / "api" / "include", nvcc.parent.parent / "include",
                 sysconfig.get_paths()["include"]]
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f'-DMK_TORCH_VERSION="{torch.__version__}"', *[f"-I{i}" for i in includes], "-o", str(BINDING_PATH), str(source),
-           f"-L{home / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f'-DMK_TORCH_VERSION="{torch.__version__}"',
+           *[f"-I{i}" for i in includes], "-o", str(BINDING_PATH), str(source), f"-L{home / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")

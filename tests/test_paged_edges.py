@@ -3,6 +3,8 @@
 Tolerances are those of tests/test_paged.py, or derived where they stand.
 """
 import math
+import os
+import subprocess
 
 import pytest
 import torch
@@ -216,3 +218,35 @@ def test_generator_tells_of_failed_waits(cuda, monkeypatch):
     _lib.check(real.mk_program_poke_wait(prog._handle, 0, int(s.wait_cnt[0]), int(s.wait_tgt[0]) + 1000))
     with pytest.raises(_lib.MegakernelTimeout):
         gen.prefill(list(range(16)))
+
+
+# -- building the binding -----------------------------------------------------------------------------------------------------
+@pytest.fixture
+def own_binding(tmp_path, monkeypatch):
+    """A place for the module of this test's own, and a compiler that only makes the file; the list of its runs."""
+    runs = []
+
+    def run(cmd, **kw):
+        runs.append(cmd)
+        (tmp_path / "_binding.so").write_text("module")
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+    monkeypatch.setattr(_lib, "BINDING_PATH", tmp_path / "_binding.so")
+    monkeypatch.setattr(_lib.subprocess, "run", run)
+    return runs
+
+
+def test_library_without_a_compiler_for_the_binding(own_binding, monkeypatch):
+    """Where the Python module cannot be compiled the library is there all the same, with a warning, and no module of other sources is loaded."""
+    monkeypatch.setattr(_lib, "needs_build_of", lambda path: False)
+    assert _lib.build() == _lib.LIB_PATH and _lib.BINDING_PATH.exists()
+    for error in (lambda cmd, **kw: subprocess.CompletedProcess(cmd, 1, "", "Python.h: No such file"), None):
+        def missing(cmd, **kw):
+            raise FileNotFoundError("g++")
+        monkeypatch.setattr(_lib.subprocess, "run", error or missing)
+        _lib.BINDING_PATH.write_text("of older sources")
+        os.utime(_lib.BINDING_PATH, (0, 0))
+        with pytest.warns(RuntimeWarning, match="ctypes"):
+            assert _lib.build() == _lib.LIB_PATH
+        assert not _lib.BINDING_PATH.exists()
+        with pytest.raises((RuntimeError, FileNotFoundError)):
+            _lib.build_binding()
