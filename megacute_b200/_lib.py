@@ -165,9 +165,13 @@ def build_binding(force: bool = False) -> pathlib.Path:
 
     import torch
     source, header = CSRC / "binding.cpp", PKG.parent / "include" / "megacute_b200.h"
-    if not force and BINDING_PATH.exists() and all(f.stat().st_mtime <= BINDING_PATH.stat().st_mtime for f in (source, header)):
+    built_for = f"{torch.__version__} {sysconfig.get_config_var('SOABI')}"
+    stamp = BINDING_PATH.with_suffix(".built_for")
+    if not force and BINDING_PATH.exists() and stamp.exists() and stamp.read_text() == built_for and \
+            all(f.stat().st_mtime <= BINDING_PATH.stat().st_mtime for f in (source, header)):
         return BINDING_PATH
-    BINDING_PATH.unlink(missing_ok=True)
+    for f in (stamp, BINDING_PATH):
+        f.unlink(missing_ok=True)
     home = pathlib.Path(torch.__file__).resolve().parent
     nvcc = pathlib.Path(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc").resolve()
     includes = [header.parent, home / "include", home / "include" / "torch" / "csrc" / "api" / "include", nvcc.parent.parent / "include",
@@ -178,6 +182,7 @@ def build_binding(force: bool = False) -> pathlib.Path:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    stamp.write_text(built_for)
     return BINDING_PATH
 
 

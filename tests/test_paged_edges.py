@@ -250,3 +250,21 @@ def test_library_without_a_compiler_for_the_binding(own_binding, monkeypatch):
         assert not _lib.BINDING_PATH.exists()
         with pytest.raises((RuntimeError, FileNotFoundError)):
             _lib.build_binding()
+
+
+def test_binding_is_built_again_for_another_torch(own_binding, monkeypatch):
+    """A module that was built against another torch, or of which that is not known, would be left aside at run time."""
+    _lib.build_binding()
+    assert len(own_binding) == 1 and any(torch.__version__ in word for word in own_binding[0])
+    _lib.build_binding()
+    assert len(own_binding) == 1
+    monkeypatch.setattr(torch, "__version__", "0.0.1+other")
+    _lib.build_binding()
+    assert len(own_binding) == 2 and any("0.0.1+other" in word for word in own_binding[1])
+    _lib.build_binding()
+    assert len(own_binding) == 2
+    _lib.BINDING_PATH.with_suffix(".built_for").unlink()
+    _lib.build_binding()
+    assert len(own_binding) == 3
+    _lib.build_binding(force=True)
+    assert len(own_binding) == 4
