@@ -9,9 +9,10 @@
 //   S = Q K^T   mma m16n8k16, K rows through ldmatrix (16-byte pieces swizzled by row: no bank conflicts), fp32
 //   P = 2^(S scale log2(e) - m), rounded to the operand type, in registers the A operand of
 //   O += P V    V through transposing ldmatrix
-// P's rounding is the second product's operand type; sums of weights are of the unrounded ones, everything else is fp32.
-// The maximum is only raised when it grows by more than 2^8, so that O is seldom scaled.  Items of at most 8 rows: nothing is done for the others
-// (64 ragged sequences, 8 kv heads of 64: 63.5 us instead of 65.3).
+// P is rounded to the second product's operand type; sums of weights are of the unrounded ones, everything else is fp32.  Items of at most 8 rows: the
+// operand's other 8 rows take what the rounding left over, so that 16 bits more of P count, at no cost (64 ragged sequences 56.7 us with and without,
+// one of 1024 keys 9.1); nothing else is done for them (8 kv heads of 64: 63.5 us instead of 65.3).  Items of 16 rows would need products of their own for it.
+// The maximum is only raised when it grows by more than 2^8, so that O is seldom scaled.
 #include "mma.cuh"
 #include "paged_attention.cuh"
 
@@ -49,7 +50,7 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
     return (w & E) == E || ((w >> 16) & E) == E;
 }
 
-// HALVES: 1 for items of at most 8 rows (the matrix instruction's other 8 are zeros, and nothing is done for them), else 2
+// HALVES: 1 for items of at most 8 rows (the matrix instruction's other 8 are zeros in Q and what P lost to rounding in the second product), else 2
 template <int DT, int D, int HALVES>
 __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_constant__ AttnArgs a, float* own) {
     constexpr int SHIFT = unit_shift<D>, U = 1 << SHIFT, NT = U / 8, KS = U / 16, DK = D / 16, DN = D / 8;
@@ -210,6 +211,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
                     for (int n = 0; n < DN; ++n) {
                         o[n][2 * i] *= f;
                         o[n][2 * i + 1] *= f;
+                        if (HALVES == 1) {
+                            o[n][2] *= f;
+                            o[n][3] *= f;
+                        }
                     }
                 }
             }
@@ -221,7 +226,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
                 for (int n = 0; n < NT; ++n) {
                     const float a0 = ex2(sc[n][2 * i] - off), a1 = ex2(sc[n][2 * i + 1] - off);
                     l[i] += a0 + a1;
-                    p[n >> 1][(n & 1) * 2 + i] = pack16<DT>(a0, a1);
+                    const uint32_t high = pack16<DT>(a0, a1);
+                    p[n >> 1][(n & 1) * 2 + i] = high;
+                    if (HALVES == 1) {
+                        const float2 h = unpack16<DT>(high);
+                        p[n >> 1][(n & 1) * 2 + 1] = pack16<DT>(a0 - h.x, a1 - h.y);
+                    }
                 }
             }
             // a value that is no number must not reach the tokens that do not see its key through 0 * it
@@ -250,7 +260,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
                         const long long at = p0 + t;
                         const int hi = (int)min(max(at, -1ll), (long long)it.hi);
                         const int lo = a.window > 0 ? (int)min(max(at + 1 - a.window, 0ll), 0x7fffffffll) : 0;
-                        const bool r0 = a.token_of(quad) == t, r1 = HALVES == 2 && a.token_of(quad + 8) == t;
+                        const bool r0 = a.token_of(quad) == t, r1 = HALVES == 2 ? a.token_of(quad + 8) == t : r0;
                         uint32_t bt[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
@@ -273,6 +283,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attend_few(const __grid_con
         for (int i = 0; i < HALVES; ++i) {
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        }
+        if (HALVES == 1) {                                       // (where a value is infinite the low half's sum may be of the other sign: left out)
+#pragma unroll
+            for (int n = 0; n < DN; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (fabsf(o[n][e]) < -NEG_INF) o[n][e] += o[n][e + 2];
         }
         // ---- results, or this part's statistics and products
         const bool whole = u0 == 0 && count == it.units;

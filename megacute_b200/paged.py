@@ -353,7 +353,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     A row at position p attends rows [0, p] of its sequence, or the last ``window`` of these; grouped queries: head h reads kv head
     h // (heads / kv_heads).  Rows of absent pages and rows behind the page table are not there; a row that sees none becomes zeros.  (A key whose
     score overflows to -inf has no weight; a row that sees a score of +inf or NaN has no result, NaN.)  ``scale`` is head_dim ** -0.5 by default.
-    head_dim 64 or 128.  Statistics and sums are fp32; the probabilities are rounded to q's type in front of the product with V.
+    head_dim 64 or 128.  Statistics and sums are fp32; the probabilities are rounded to q's type in front of the product with V,
+    which in calls of at most 8 rows (heads of a kv head times ``max_new``) takes what the rounding left over as well.
 
     ``max_new``: the largest number of rows a sequence has in this call, where ``starts`` is given (it is on the device): the kernel is chosen by it, and
     a wrong value costs time but changes no more than the order of sums."""

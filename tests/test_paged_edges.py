@@ -11,7 +11,8 @@ import torch
 
 import megacute_b200 as mc
 from megacute_b200 import _lib, paged
-from tests.test_paged import BF, check_attention, make_attention
+from oracle import paged_oracle as ref
+from tests.test_paged import BF, HALF, W, check_attention, close, half_step, make_attention, on, smallest
 
 
 # -- the hint of the largest number of new tokens ---------------------------------------------------------------------------
@@ -268,3 +269,36 @@ def test_binding_is_built_again_for_another_torch(own_binding, monkeypatch):
     assert len(own_binding) == 3
     _lib.build_binding(force=True)
     assert len(own_binding) == 4
+
+
+# -- probabilities of single tokens -----------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [None, 0.02])
+@pytest.mark.parametrize("D,H,KVH,new,dtype", [(64, 4, 2, 1, BF), (128, 8, 1, 1, BF), (128, 8, 2, 2, BF), (64, 7, 1, 1, BF), (64, 32, 8, 1, BF),
+                                               (128, 6, 3, 3, HALF), (64, 8, 1, 1, HALF)])
+def test_probabilities_of_few_rows_in_two_halves(cuda, D, H, KVH, new, dtype, scale):
+    """Up to 8 rows an item: a probability is handed on as a rounded value and its rounded rest, off by u^2 of it; with the error of a score (2 (D + 6) w S),
+    of the sum (w for each of n + 64 additions) and of an exponential (2^-22, in the weight and in the sum), and no 2^-13 for a polynomial, which this
+    kernel has not.  Little more than the result's own rounding is left."""
+    args, kw = make_attention([700, 0, 1023, 16, 300], [new] * 5, H, KVH, D, 32, dtype, seed=H + new)
+    got = mc.paged_attention(**on(cuda, args), **kw, scale=scale, max_new=new)
+    want, mag, size = ref.paged_attention(**args, **kw, scale=scale)
+    u, keys = half_step(dtype), 1024 + new
+    under = keys * 2.0 ** -25 * float(args["v_cache"].double().abs().max()) if dtype == HALF else 0.0
+    per = u ** 2 + 2 * (D + 6) * W * size + (keys + 64) * W + 2.0 ** -21
+    close(got, want, u * want.abs() + (1 + u) * (per * mag + under) + smallest(dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,H,KVH,new,dtype", [(64, 4, 2, 1, BF), (128, 4, 1, 2, HALF), (64, 4, 1, 2, BF), (128, 16, 1, 1, BF)])
+def test_infinite_values_of_few_rows(cuda, D, H, KVH, new, dtype):
+    """An infinite value gives the tokens that see it an infinite result, not none, whatever the sign of a probability's rounding."""
+    args, kw = make_attention([300, 40], [new, new], H, KVH, D, 16, dtype, seed=D + new, qstd=0.3)
+    n = args["k_cache"].shape[0] // 16
+    for s, p in ((0, 7), (0, 300 + new - 1), (1, 33)):
+        args["v_cache"][ref.cache_row(args["pages"], s, p, 16, n), s::5] = float("inf") if s else float("-inf")
+    got = mc.paged_attention(**on(cuda, args), **kw, max_new=new).cpu().double()
+    want = ref.paged_attention(**args, **kw)[0]
+    for f in (torch.isposinf, torch.isneginf, torch.isnan):
+        assert torch.equal(f(got), f(want))
+    assert torch.isinf(want).any() and torch.isfinite(want).any()
