@@ -12,7 +12,7 @@ import torch
 import megacute_b200 as mc
 from megacute_b200 import _lib, paged
 from oracle import paged_oracle as ref
-from tests.test_paged import BF, HALF, W, check_attention, close, half_step, make_attention, on, smallest
+from tests.test_paged import BF, HALF, W, attention_tolerance, check_attention, close, half_step, make_attention, on, smallest
 
 
 # -- the hint of the largest number of new tokens ---------------------------------------------------------------------------
@@ -302,3 +302,75 @@ def test_infinite_values_of_few_rows(cuda, D, H, KVH, new, dtype):
     for f in (torch.isposinf, torch.isneginf, torch.isnan):
         assert torch.equal(f(got), f(want))
     assert torch.isinf(want).any() and torch.isfinite(want).any()
+
+
+# -- messages of the C entries --------------------------------------------------------------------------------------------------
+def test_messages_of_the_c_entries():
+    """Each refusal leaves its own message (addresses here are never followed; the one before is of another kind each time)."""
+    lib = _lib.load()
+    batch = lambda **k: _lib.Batch(**{**dict(pos=4096, starts=None, pos_ld=1, rows=4, seqs=2), **k})
+    rot = lambda **k: _lib.Rotation(**{**dict(cos=4096, sin=4096, ld_cos=32, ld_sin=32, rows=8, columns=32, dtype=1, interleaved=0), **k})
+    cache = lambda **k: _lib.PagedCache(**{**dict(k=4096, v=4096, table=4096, ld_k=128, ld_v=128, table_ld=4, pages=4, page_size=16, table_cols=4,
+                                                  kv_heads=2, head_dim=64, dtype=0), **k})
+    rotary = lambda b=batch(), r=rot(), x=4096, ld=256, dim=64: lib.mk_rotary(0, b, r, x, ld, 8192, 256, 0, 4, dim, None)
+    append = lambda c=cache(), r=rot(), q=8192, heads=4: lib.mk_paged_append(0, batch(), r, c, 4096, 512, q, 256, heads, None)
+    attend = lambda c=cache(), ws=4096, window=0, heads=4, q=4096: lib.mk_paged_attention(0, batch(), c, q, 256, 8192, 256, heads, 1.0, window, 1, ws, 1 << 40, None)
+    for call, words in ((lambda: rotary(x=4104), b"16-byte"), (lambda: rotary(batch(rows=5)), b"same number of rows"), (lambda: rotary(ld=128), b"hold all heads"),
+                        (lambda: rotary(dim=60), b"multiple of 16"), (lambda: rotary(r=rot(columns=12)), b"are rotated"), (lambda: rotary(r=rot(rows=0)), b"no tables"),
+                        (lambda: rotary(r=rot(dtype=3)), b"tables are"), (lambda: append(q=8200), b"16-byte"), (lambda: append(cache(page_size=24)), b"power of two"),
+                        (lambda: append(heads=0), b"multiple of 16"), (lambda: append(cache(k=4098)), b"16-byte"), (lambda: append(cache(k=None)), b"no memory"),
+                        (lambda: append(cache(dtype=1)), b"bf16 or fp16"), (lambda: attend(cache(pages=2 ** 30)), b"2^31 - 1 rows"),
+                        (lambda: attend(ws=None), b"256-byte"), (lambda: attend(cache(table_cols=2 ** 30)), b"65536"), (lambda: attend(ws=4100), b"256-byte"),
+                        (lambda: attend(window=-1), b"window"), (lambda: attend(heads=3), b"multiple of kv_heads"), (lambda: attend(q=None), b"16-byte"),
+                        (lambda: attend(cache(head_dim=32)), b"64 or 128"), (lambda: attend(cache(ld_k=120)), b"kv_heads heads"),
+                        (lambda: lib.mk_paged_attention_workspace(0, 3, 2, 64, 1), b"multiple of kv_heads"),
+                        (lambda: lib.mk_paged_attention_workspace(0, 4, 2, 96, 1), b"64 or 128")):
+        assert call() == -2 and words in lib.mk_last_cuda_error(), (words, lib.mk_last_cuda_error())
+
+
+# -- chunks: windows over values that are no numbers, far contexts -----------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,H,KVH,dtype,page", [(64, 4, 2, BF, 16), (128, 4, 1, HALF, 128), (64, 3, 3, HALF, 64), (128, 2, 2, BF, 256)])
+@pytest.mark.parametrize("window", [1, 30, 100, 128, 200, 300])
+@pytest.mark.parametrize("new", [3, 140, 256, 300])
+def test_window_over_values_not_finite(cuda, D, H, KVH, dtype, page, window, new):
+    """Infinite values and ones that are no numbers anywhere in a chunk and the window in front of it: for the tokens whose window holds them what the definition
+    gives, for those in front of them and those whose window has passed them nothing."""
+    pos = [300, 77]
+    args, kw = make_attention(pos, [new, new], H, KVH, D, page, dtype, seed=new + window)
+    n, g, v = args["k_cache"].shape[0] // page, torch.Generator().manual_seed(window), args["v_cache"]
+    for s, p in enumerate(pos):
+        for i, at in enumerate(torch.randint(max(0, p - window), p + new, (9,), generator=g).tolist()):
+            v[ref.cache_row(args["pages"], s, at, page, n), i::11] = (float("inf"), float("-inf"), float("nan"))[i % 3]
+    got = mc.paged_attention(**on(cuda, args), **kw, window=window).cpu().double()
+    want = ref.paged_attention(**args, **kw, window=window)[0]
+    finite = torch.isfinite(want)
+    clean = dict(args, v_cache=torch.where(torch.isfinite(v), v, torch.zeros((), dtype=dtype)))
+    _, mag, size = ref.paged_attention(**clean, **kw, window=window)
+    tol = attention_tolerance(want, mag, size, dtype, D, args["pages"].shape[1] * page, float(clean["v_cache"].double().abs().max()))
+    close(got[finite], want[finite], tol[finite])
+    for f in (torch.isposinf, torch.isneginf, torch.isnan):
+        assert torch.equal(f(got), f(want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,H,KVH,new,window", [(64, 8, 2, 509, 0), (128, 4, 1, 300, 0), (64, 8, 2, 130, 5000), (128, 16, 2, 1, 0), (64, 4, 4, 17, 0)])
+def test_far_context(cuda, D, H, KVH, new, window):
+    """Tokens behind 16001 others, against 64 bits on the GPU."""
+    page, ctx = 128, 16001
+    args, kw = make_attention([ctx], [new], H, KVH, D, page, BF, seed=new)
+    a = on(cuda, args)
+    got = mc.paged_attention(**a, **kw, window=window)
+    idx = torch.arange(ctx + new, device=cuda)
+    rows = a["pages"][0].long()[idx // page] * page + idx % page
+    at = torch.arange(ctx, ctx + new, device=cuda)[:, None]
+    hidden = (idx[None] > at) | (idx[None] <= at - (window or 2 ** 40))
+    for h in range(H):
+        j = h // (H // KVH)
+        k, v = (a[x][rows][:, j * D:(j + 1) * D].double() for x in ("k_cache", "v_cache"))
+        x = a["q"][:, h * D:(h + 1) * D].double()
+        w = torch.softmax((x @ k.T * D ** -0.5).masked_fill(hidden, float("-inf")), -1)
+        want, mag = (w @ v).cpu(), (w @ v.abs()).cpu()
+        size = torch.full_like(want, float((x.abs() @ k.abs().T).max()) * D ** -0.5)
+        # (the sum of more than a thousand probabilities: w each)
+        close(got[:, h * D:(h + 1) * D], want, attention_tolerance(want, mag, size, BF, D, ctx + new, 6.0) + ((ctx + new) * W) * mag)
