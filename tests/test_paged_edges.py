@@ -374,3 +374,16 @@ def test_far_context(cuda, D, H, KVH, new, window):
         size = torch.full_like(want, float((x.abs() @ k.abs().T).max()) * D ** -0.5)
         # (the sum of more than a thousand probabilities: w each)
         close(got[:, h * D:(h + 1) * D], want, attention_tolerance(want, mag, size, BF, D, ctx + new, 6.0) + ((ctx + new) * W) * mag)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("chunk,steps", [(0, 9), (4, 5), (6, 3), (100, 9)])
+def test_command_counts_its_steps(cuda, monkeypatch, capsys, chunk, steps):
+    """The command's time of a step is over the steps it takes: the tokens that go in chunks are none of them."""
+    from megacute_b200 import checkpoint
+    from tests.test_checkpoint import CFG, hf_state_dict
+    monkeypatch.setattr(checkpoint, "load_local", lambda path: (CFG, hf_state_dict(CFG, seed=5)))
+    checkpoint.main(["--model", "here", "--prompt-ids", "1,2,3,4,5,6,7", "--tokens", "3", "--max-seq", "128", "--prompt-chunk", str(chunk)])
+    lines = capsys.readouterr().out.splitlines()
+    want = [f"{9 - steps} prompt tokens x batch 1 in chunks"] * (steps < 9) + [f"{steps} steps x batch 1"]
+    assert [s.split(":")[0] for s in lines[:-1]] == want and len(eval(lines[-1])) == 3
