@@ -27,7 +27,8 @@ LIB_PATH = pathlib.Path(os.environ.get("MEGACUTE_B200_LIB", PKG / ("libmegacute_
 # not see the kernel's __launch_bounds__.
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-rdc=true",
               "-maxrregcount=168", "-shared", "-Xcompiler", "-fPIC"]
-# Sources of kernels of their own, compiled as whole programs: ptxas ignores setmaxnreg in relocatable device code.
+# Sources of kernels of their own, compiled as whole programs: in relocatable device code their functions would get the registers of a
+# separate call, under the cap above.
 WHOLE_PROGRAM = ("rotary.cu", "paged_attention.cu", "paged_attention_few.cu", "paged_attention_chunk.cu")
 WHOLE_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-c"]
 

@@ -1,9 +1,9 @@
 // Attention over a paged cache for items of at most 16 rows (new tokens x heads of a group): single tokens, a few speculative ones.
 //
 // Bound by memory: K and V are read once (heads of a group and tokens of a sequence share them), 2 * 2 * head_dim bytes a key, for 4 * 16 * head_dim
-// products, far below what warp-level matrix instructions give.  Measured: 64 sequences of 1 to 4096 keys, bf16, 4 kv heads of 128: 56 us, 78 % of the
+// products, far below what warp-level matrix instructions give.  Measured: 64 sequences of 1 to 4096 keys, bf16, 4 kv heads of 128: 57 us, 77 % of the
 // measured copy rate; short of that by what comes before and after the keys, 8 to 10 us (launches, the plan, the first look-ups, the joins):
-// one sequence of 1024 keys 9.3 us, of 16384 15.7.  So every warp is a worker of its own (paged_attention.cuh): it
+// one sequence of 1024 keys 9.1 us, of 16384 15.7.  So every warp is a worker of its own (paged_attention.cuh): it
 // copies units of 8 KB (16 keys of head_dim 128, 32 of 64) into its own ring of three with 16-byte asynchronous copies, which follow the
 // page table row by row and write zeros for keys that are not there, and meets no other warp.  16 rows x unit:
 //   S = Q K^T   mma m16n8k16, K rows through ldmatrix (16-byte pieces swizzled by row: no bank conflicts), fp32
