@@ -126,7 +126,8 @@ class LlamaGenerator:
 
     def prefill(self, tokens: list[int]) -> int:
         """Feed whole chunks of ``prompt_chunk`` tokens (the same for every sequence of the batch) into the cache, and return how many tokens these
-        are; the rest is for ``step``.  Nothing is sampled.  Raises ``MegakernelTimeout`` if a launch or a call gave up a wait: the cache is then not to be used."""
+        are; the rest is for ``step``.  Nothing is sampled.  Raises ``MegakernelTimeout`` if a launch or a call gave up a wait: the cache
+        is then not to be used."""
         import megacute_b200 as mc
         c, b = self.prompt_chunk, self.batch
         whole = len(tokens) // c * c if c else 0

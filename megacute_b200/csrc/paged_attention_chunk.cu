@@ -17,9 +17,9 @@
 // What bounds it: a score product of 128 x 128 x 64 and its P V take 256 cycles each of the tensor cores, the 16384 exponentials 1024 of the special
 // function units (16 a cycle) or 768 with a quarter of them on the fp32 units, and the maxima, conversions and accesses to tensor memory of the same
 // threads come on top.  So head_dim 64 is bound by the softmax; for 128, whose products take twice as long, the chain from S over P to P V and the next S
-// through two buffers of scores counts as much.  Measured as captured graphs: 4 prompts of 4096 tokens, bf16, 32 heads and 8 kv heads of 64: 386 to 394 us, 697 to
-// 712 TFLOP/s (called one by one 409 to 420); 16 heads
-// and 4 kv heads of 128: 271 us, 1014 TFLOP/s; 509 tokens behind 16001, 32 heads of 64: 100 us, 675 TFLOP/s.
+// through two buffers of scores counts as much.  Measured as captured graphs: 4 prompts of 4096 tokens, bf16, 32 heads and 8 kv heads of 64: 386 to 394 us,
+// 697 to 712 TFLOP/s (called one by one 409 to 420 us); 16 heads and 4 kv heads of 128: 271 us, 1014 TFLOP/s; 509 tokens behind 16001, 32 heads of 64: 100 us,
+// 675 TFLOP/s (104).
 // Both sides of the choices, for the first two of these when they took 400 and 283 us: the maximum raised whenever it grows 459 and 333; the row's scores held in registers
 // (spills) 467; two threads a row 429; the two tiles' exponentials in turns 458.
 // Every wait has a limit, after which the block counts it, raises a flag that all its waits ask for, waits for its copies, frees its tensor memory and
